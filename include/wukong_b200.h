@@ -323,6 +323,62 @@ int wkb_paged_kv_append(const float* ksrc, const float* vsrc, int64_t src_row_st
                         int64_t kv_heads, int64_t head_dim, int64_t page_tokens, int64_t max_blocks_per_seq,
                         void* stream);
 
+/* ---- Speculative decoding over the paged cache: the target model checks a tree of drafted tokens in one step -------------
+ * (no counterpart in the reference, which decodes one token a sequence a step).  A tree hangs off a sequence of
+ * tree_ctx[t] committed tokens in block-table row tree_slot[t].  Node 0 is the last token that the target emitted, every
+ * other node a drafted token whose parent comes before it.  The nodes of all trees are the rows of one flat batch: tree t
+ * owns rows tree_row0[t] .. tree_row0[t + 1] - 1 (tree_row0 ascends, n_trees + 1 entries), at most max_nodes <= 256 of them,
+ * and node i's K / V lie at position tree_ctx[t] + i (wkb_paged_kv_append with row_pos = ctx + i; a rotary position is
+ * ctx + the node's depth).  A tree with tree_slot[t] < 0 or tree_ctx[t] < 0 is switched off: its rows, and rows behind the
+ * last tree, are left as they were.  All arrays are DEVICE arrays, so that a captured step follows new trees.
+ *
+ * Attention: row r = node i of tree t sees every position below tree_ctx[t] and the node at tree_ctx[t] + j where bit j % 32
+ * of tree_mask[r * mask_words + j / 32] is set (the node itself and its ancestors; other patterns are allowed).  What a row
+ * does not see never reaches its output, NaN included; a row that sees nothing gives zeros.  q and out: dtype 0 f32, 1 bf16,
+ * row strides in elements, multiples of 8; all bases 16-byte aligned.  bf16 outputs carry bf16 softmax weights; f32 outputs
+ * keep f32 accuracy.  head_dim in {64, 128}; q_heads / kv_heads in {1, 2, 4, 8}; page_tokens a power of two >= 4;
+ * n_trees <= 4096.  A block-table entry >= num_pages reads as a page of zeros, positions past the table row are not seen.
+ * `scratch`: wkb_paged_attn_tree_scratch_bytes(...) bytes, uninitialised, one per stream (calls that may overlap need their
+ * own, two captured graphs that may replay at the same time too). */
+int64_t wkb_paged_attn_tree_scratch_bytes(int64_t max_nodes, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+int wkb_paged_attn_tree(const void* q, int q_dtype, int64_t q_row_stride, const void* kcache, const void* vcache, int64_t num_pages,
+                        const uint32_t* block_table, const int* tree_slot, const int* tree_ctx, const int* tree_row0,
+                        const uint32_t* tree_mask, int64_t mask_words, void* out, int out_dtype, int64_t out_row_stride, int64_t rows,
+                        int64_t n_trees, int64_t max_nodes, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                        int64_t max_blocks_per_seq, float scale, void* scratch, int64_t scratch_bytes, void* stream);
+/* Vocabulary probabilities: out[r, :] = softmax(logits[r, :] / temperature[r]) in f32 (in_dtype 0 f32, 1 bf16; temperature
+ * null: 1).  Temperature <= 0 gives the greedy row: 1 at the lowest column of the maximum, 0 elsewhere.  A token with logit
+ * -inf has probability 0, a row of only those is all zeros; a row with a NaN, or whose maximum is +inf at a positive
+ * temperature, holds NaN.  ld / ld_out >= cols; out may be the f32 logits themselves. */
+int wkb_token_probs(const void* logits, int in_dtype, int64_t ld, const float* temperature_or_null, float* out, int64_t ld_out,
+                    int64_t rows, int64_t cols, void* stream);
+/* Verification of drafted tokens from given random numbers.  Row r of `probs` holds the target's probabilities after node r,
+ * row r of `draft` (null: none) the distribution that the children of node r were drawn from, f32 [rows, cols] with row
+ * pitches ld_p / ld_q; token[r] is the node's token, parent[r] its parent's index within the tree (below its own; the root's
+ * is not read).  The walk starts at the root.  With p, q the current node's rows, r_0 = p and Z_0 = 1, its children x_1, x_2,
+ * ... are tried in row order:
+ *   accepted (and walked to) when  u_node * q(x_k) * Z < r(x_k);   else  r <- max(r - Z * q, 0),  Z <- sum of r.
+ * Without `draft` a child is a fixed candidate: q(x_k) = 1, and a rejection takes r(x_k) out of r and from Z.  At a node with
+ * no child left the next token is drawn from r: the lowest column whose running mass exceeds u_final[t] times the whole, so
+ * that the emitted tokens follow the target's distribution.  Weights that are not positive and finite count as zero, a
+ * token outside [0, cols) has none; masses are f64; random numbers are clamped to [0, 1], NaN is 0.
+ * path [n_trees, max_path]: the accepted nodes from the root (0) on, -1 behind; n_path: how many; tokens [n_trees, max_path]:
+ * what the step emits -- the accepted drafts, then the drawn token (-1: no mass was left), -1 behind.  A walk of max_path
+ * nodes ends there.  A tree without rows gives n_path 0.  1 <= max_path <= max_nodes <= 256.  Results are run-to-run identical. */
+int wkb_tree_verify(const float* probs, int64_t ld_p, const float* draft_or_null, int64_t ld_q, const int* token, const int* parent,
+                    const int* tree_row0, int64_t rows, int64_t n_trees, int64_t max_nodes, int64_t cols, const float* u_node,
+                    const float* u_final, int* path, int* tokens, int* n_path, int64_t max_path, void* stream);
+/* Commit of a verified step: the K / V of node path[t, i], 1 <= i < n_path[t], move from position tree_ctx[t] + path[t, i] to
+ * tree_ctx[t] + i, in all layers (slabs `layer_stride` elements apart, bf16 [num_pages][kv_heads][page_tokens][head_dim]
+ * each), and new_ctx[t] (may be null, must not be tree_ctx) = tree_ctx[t] + n_path[t], the context of the next step.  A path must
+ * ascend, and no two trees of a call may share a slot.  An entry that does not ascend, or whose positions lie past the
+ * block-table row or the cache, ends that tree's moves and records 31 (wkb_gemm_status); trees that are switched off are
+ * left alone. */
+int wkb_paged_kv_commit(void* kcache, void* vcache, int64_t layers, int64_t layer_stride, int64_t num_pages, const uint32_t* block_table,
+                        const int* tree_slot, const int* tree_ctx, const int* path, const int* n_path, int64_t max_path, int64_t n_trees,
+                        int64_t kv_heads, int64_t head_dim, int64_t page_tokens, int64_t max_blocks_per_seq, int* new_ctx_or_null,
+                        void* stream);
+
 /* Page allocator (host; behaviour of paged_kv.rs:428-628): LIFO free list handing out ascending
  * pages on a fresh pool; append allocates only on a page boundary; -1 = out of pages, state unchanged. */
 void* wkb_blockmgr_new(int64_t num_blocks, int64_t block_size, int64_t num_slots, int64_t max_blocks_per_seq);

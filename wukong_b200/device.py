@@ -245,3 +245,130 @@ def paged_attn_decode_int8(q, q_row_stride, kv, layer, block_table, row_slot, ro
                                            int(out.dtype == torch.bfloat16), out.stride(0), rows, q_heads, kv.kv_heads, kv.head_dim,
                                            kv.page_tokens, mbps, max_ctx, scale, _p(scratch), _s()), "wkb_paged_attn_decode_int8")
     return out
+
+
+# ---- speculative decoding: a tree of drafted tokens is checked in one step --------------------------------------------
+
+def tree_layout(parent, row0):
+    """Host helper: for trees given as each row's parent within its tree (numpy, < the node's own index; the root's entry is
+    not read) and first rows row0 [n + 1], the attention masks (int32 [rows, words]: itself and its ancestors) and each
+    node's depth (int32 [rows]; a rotary position is ctx + depth)."""
+    parent, row0 = np.asarray(parent, np.int64), np.asarray(row0, np.int64)
+    counts = np.diff(row0)
+    if row0.ndim != 1 or row0.size < 1 or row0[0] != 0 or (counts < 0).any() or row0[-1] != parent.size:
+        raise ValueError("row0 must ascend from 0 to the number of rows")
+    words = max(1, -(-int(counts.max(initial=0)) // 32))
+    mask, depth = np.zeros((parent.size, words), np.uint32), np.zeros(parent.size, np.int32)
+    for a, count in zip(row0[:-1].tolist(), counts.tolist()):
+        for i in range(count):
+            if i:
+                p = int(parent[a + i])
+                if not 0 <= p < i:
+                    raise ValueError("a node's parent must come before it")
+                mask[a + i], depth[a + i] = mask[a + p], depth[a + p] + 1
+            mask[a + i, i // 32] |= np.uint32(1 << (i % 32))
+    return mask.view(np.int32), depth
+
+
+def _same_device(*tensors):
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != cur):
+            raise ValueError("every tensor must lie on the current CUDA device")
+
+
+def _vec(t, n, dtype, what):
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous %s tensor of %d values" % (what, dtype, n))
+
+
+def _row_pitch(t, cols, what):
+    if t.dim() != 2 or t.shape[1] < cols or t.stride(1) != 1:
+        raise ValueError("%s must be a matrix of at least %d columns with unit column stride" % (what, cols))
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def paged_attn_tree_scratch(max_nodes, q_heads, kv_heads, head_dim, device="cuda"):
+    return torch.empty(int(lib().wkb_paged_attn_tree_scratch_bytes(max_nodes, q_heads, kv_heads, head_dim)), dtype=torch.uint8, device=device)
+
+
+def paged_attn_tree(q, q_row_stride, kv, layer, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, q_heads, mbps, max_nodes, scale, scratch):
+    """Attention of the nodes of draft trees over the paged bf16 cache (wkb_paged_attn_tree): row r = node i of tree t sees
+    the tree_ctx[t] committed tokens and the nodes that its mask names.  q f32 or bf16, out f32 or bf16 [rows, q_heads * head_dim]."""
+    rows, n = out.shape[0], tree_slot.numel()
+    _same_device(q, kv.k, kv.v, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, scratch)
+    _vec(tree_slot, n, torch.int32, "tree_slot"); _vec(tree_ctx, n, torch.int32, "tree_ctx"); _vec(tree_row0, n + 1, torch.int32, "tree_row0")
+    if tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] < rows or not tree_mask.is_contiguous():
+        raise ValueError("tree_mask must be a contiguous int32 [rows, words]")
+    if q.dtype not in (torch.float32, torch.bfloat16) or out.dtype not in (torch.float32, torch.bfloat16) or kv.k.dtype != torch.bfloat16:
+        raise ValueError("q and out are f32 or bf16, the cache is bf16")
+    if out.dim() != 2 or out.shape[1] < q_heads * kv.head_dim or out.stride(1) != 1:
+        raise ValueError("out must be [rows, q_heads * head_dim] with unit column stride")
+    if rows and q.storage_offset() + (rows - 1) * q_row_stride + q_heads * kv.head_dim > q.untyped_storage().nbytes() // q.element_size():
+        raise ValueError("q does not hold %d rows of pitch %d" % (rows, q_row_stride))
+    if block_table.dtype != torch.int32 or not block_table.is_contiguous() or block_table.numel() % mbps:
+        raise ValueError("block_table must be a contiguous int32 [slots, mbps]")
+    check(lib().wkb_paged_attn_tree(_p(q), _DT[q.dtype], q_row_stride, _p(kv.k[layer]), _p(kv.v[layer]), kv.num_pages, _p(block_table), _p(tree_slot),
+                                    _p(tree_ctx), _p(tree_row0), _p(tree_mask), tree_mask.shape[1], _p(out), _DT[out.dtype], out.stride(0), rows, n,
+                                    max_nodes, q_heads, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps, scale, _p(scratch), scratch.numel(), _s()),
+          "wkb_paged_attn_tree")
+    return out
+
+
+def token_probs(logits, temperature=None, out=None):
+    """f32 probabilities softmax(logits / temperature) of vocabulary rows; a temperature of 0 gives the greedy one-hot row
+    (wkb_token_probs).  logits f32 or bf16 [rows, cols] (any row pitch), temperature f32 [rows]."""
+    rows, cols = logits.shape
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits are f32 or bf16")
+    if temperature is not None:
+        _vec(temperature, rows, torch.float32, "temperature")
+    if out is None:
+        out = torch.empty((rows, cols), dtype=torch.float32, device=logits.device)
+    if out.dtype != torch.float32 or out.shape != logits.shape:
+        raise ValueError("out must be f32 of the logits' shape")
+    _same_device(logits, temperature, out)
+    check(lib().wkb_token_probs(_p(logits), _DT[logits.dtype], _row_pitch(logits, cols, "logits"), _p(temperature), _p(out), _row_pitch(out, cols, "out"),
+                                rows, cols, _s()), "wkb_token_probs")
+    return out
+
+
+def tree_verify(probs, draft, token, parent, tree_row0, u_node, u_final, max_nodes, max_path, out=None):
+    """Accept / reject the drafted tokens of each tree and draw the token that follows (wkb_tree_verify).  probs, draft (or
+    None): f32 [rows, vocabulary].  Returns (path int32 [n, max_path], n_path int32 [n], tokens int32 [n, max_path])."""
+    rows, cols = probs.shape
+    n = tree_row0.numel() - 1
+    if probs.dtype != torch.float32 or (draft is not None and (draft.dtype != torch.float32 or draft.shape != probs.shape)):
+        raise ValueError("probs and draft must be f32 of one shape")
+    _vec(token, rows, torch.int32, "token"); _vec(parent, rows, torch.int32, "parent"); _vec(tree_row0, n + 1, torch.int32, "tree_row0")
+    _vec(u_node, rows, torch.float32, "u_node"); _vec(u_final, n, torch.float32, "u_final")
+    if out is None:
+        buf = torch.empty(n * (2 * max_path + 1), dtype=torch.int32, device=probs.device)
+        out = buf[:n * max_path].view(n, max_path), buf[2 * n * max_path:], buf[n * max_path:2 * n * max_path].view(n, max_path)
+    path, n_path, tokens = out
+    _vec(path, n * max_path, torch.int32, "path"); _vec(tokens, n * max_path, torch.int32, "tokens"); _vec(n_path, n, torch.int32, "n_path")
+    _same_device(probs, draft, token, parent, tree_row0, u_node, u_final, path, n_path, tokens)
+    check(lib().wkb_tree_verify(_p(probs), _row_pitch(probs, cols, "probs"), _p(draft), 0 if draft is None else _row_pitch(draft, cols, "draft"),
+                                _p(token), _p(parent), _p(tree_row0), rows, n, max_nodes, cols, _p(u_node), _p(u_final), _p(path), _p(tokens),
+                                _p(n_path), max_path, _s()), "wkb_tree_verify")
+    return path, n_path, tokens
+
+
+def paged_kv_commit(kv, block_table, tree_slot, tree_ctx, path, n_path, mbps, new_ctx=None):
+    """Move the accepted nodes' K / V to the positions behind the context, in every layer (wkb_paged_kv_commit); new_ctx
+    (optional int32 [n], other memory than tree_ctx) receives the context of the next step."""
+    n = tree_slot.numel()
+    _vec(tree_slot, n, torch.int32, "tree_slot"); _vec(tree_ctx, n, torch.int32, "tree_ctx"); _vec(n_path, n, torch.int32, "n_path")
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != n or not path.is_contiguous():
+        raise ValueError("path must be a contiguous int32 [n, max_path]")
+    if kv.k.dtype != torch.bfloat16 or not kv.k.is_contiguous() or not kv.v.is_contiguous():
+        raise ValueError("the cache must be contiguous bf16")
+    if block_table.dtype != torch.int32 or not block_table.is_contiguous() or block_table.numel() % mbps:
+        raise ValueError("block_table must be a contiguous int32 [slots, mbps]")
+    if new_ctx is not None:
+        _vec(new_ctx, n, torch.int32, "new_ctx")
+    _same_device(kv.k, kv.v, block_table, tree_slot, tree_ctx, path, n_path, new_ctx)
+    check(lib().wkb_paged_kv_commit(_p(kv.k), _p(kv.v), kv.layers, kv.k.stride(0), kv.num_pages, _p(block_table), _p(tree_slot), _p(tree_ctx), _p(path),
+                                    _p(n_path), path.shape[1], n, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps, _p(new_ctx), _s()),
+          "wkb_paged_kv_commit")
+    return kv
