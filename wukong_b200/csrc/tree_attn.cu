@@ -125,13 +125,15 @@ __global__ void __launch_bounds__(256) tree_attn_rows_kernel(const void* __restr
 }  // namespace tree
 }  // namespace wkb
 
+#include "tree_attn_tc.cuh"
+
 using namespace wkb;
 
 extern "C" {
 
 i64 wkb_paged_attn_tree_scratch_bytes(i64 max_nodes, i64 q_heads, i64 kv_heads, i64 head_dim) {
   if (max_nodes <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0) return 0;
-  return 256;
+  return tree::scratch_bytes(max_nodes, q_heads / kv_heads, head_dim);
 }
 
 int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void* kcache, const void* vcache, i64 num_pages, const uint32_t* block_table,
@@ -155,10 +157,21 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void
   while ((1 << page_shift) < page_tokens) ++page_shift;
   tree::Geo g{(int)rows, (int)n_trees, (int)max_nodes, (int)mask_words, (int)q_heads, (int)kv_heads, (int)page_tokens, page_shift, (int)max_blocks_per_seq,
               num_pages, q_row_stride, out_row_stride};
+  cudaStream_t st = as_stream(stream);
+  if (page_tokens >= 8) {      // a page of 8 tokens fills whole swizzle atoms of the operand
+    const i64 row_blocks = (max_nodes * group + tree::QROWS - 1) / tree::QROWS, key_blocks = (max_blocks_per_seq * page_tokens + tree::KBLK - 1) / tree::KBLK;
+    if ((double)n_trees * (double)kv_heads * (double)row_blocks * (double)key_blocks > 2147000000.0) return (int)cudaErrorInvalidValue;
+#define WKB_TREE_CASE(HD_, QS_, PS_)                                   \
+  if (head_dim == HD_ && (q_dtype == 1 ? 1 : out_dtype == 0 ? 3 : 2) == QS_ && (out_dtype == 0 ? 2 : 1) == PS_) \
+    return tree::launch_tc<HD_, QS_, PS_>(q, kcache, vcache, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, out_dtype, g, scale, scratch, st);
+    WKB_TREE_CASE(64, 1, 1) WKB_TREE_CASE(64, 1, 2) WKB_TREE_CASE(64, 2, 1) WKB_TREE_CASE(64, 3, 2)
+    WKB_TREE_CASE(128, 1, 1) WKB_TREE_CASE(128, 1, 2) WKB_TREE_CASE(128, 2, 1) WKB_TREE_CASE(128, 3, 2)
+#undef WKB_TREE_CASE
+  }
   const i64 blocks = (rows * q_heads + 7) / 8;
   const unsigned grid = (unsigned)(blocks < (i64)WKB_SM_COUNT * 64 ? blocks : (i64)WKB_SM_COUNT * 64);
   auto kern = head_dim == 64 ? tree::tree_attn_rows_kernel<64> : tree::tree_attn_rows_kernel<128>;
-  return (int)launch_pdl(kern, grid, 256, 0, as_stream(stream), q, q_dtype, (const u16*)kcache, (const u16*)vcache, block_table, tree_slot, tree_ctx,
+  return (int)launch_pdl(kern, grid, 256, 0, st, q, q_dtype, (const u16*)kcache, (const u16*)vcache, block_table, tree_slot, tree_ctx,
                          tree_row0, tree_mask, out, out_dtype, g, scale * 1.4426950408889634f);
 }
 

@@ -1,0 +1,757 @@
+// Tree attention on the 5th-generation tensor cores, for pages of 8 tokens and more.
+//
+// Work.  A unit is (tree, KV head, 128 of the tree's query rows, node-major with the heads of the group inside); its
+// keys are cut into blocks of 128.  All blocks of all units form one list that is dealt out in equal contiguous shares to
+// one CTA per SM, whatever the lengths: a share may hold several units, or a piece of one.  A unit that a single share
+// covers is written at once; the pieces of the others go to scratch as (maximum, sum, unnormalised output) and are
+// joined by tree_attn_join_kernel in key order, so results are run-to-run identical.
+//
+// A CTA has a TMA warp (K and V pages into two rings), an MMA warp and two teams of four softmax warps.  The teams take
+// alternate key blocks with tensor-memory columns of their own, so one team's exponentials run while the other's products
+// do:   S = Q K^T (128 x 128) -> P = exp2(S - m), bf16, over the same columns -> O += P V (128 x head_dim).
+// The running maximum m of a row moves only when a block exceeds it by 2^8; the accumulator is rescaled then and not at
+// every block.  f32 queries are two bf16 parts (hi + lo, two products); for f32 results
+// they are three and P is two.
+//
+// With 64 (32) query rows or fewer the operand's 128 rows hold 2 (4) copies of them, and each copy takes its own half
+// (quarter) of a block's keys, with zeros for the others': a team's warps share the exponentials of a small tree that
+// would otherwise all fall to one of them.  The copies are added up like the pieces of a unit.
+//
+// V and 0 x NaN: a probability of zero does not silence a NaN or an infinity in the product.  V elements that are not
+// finite are therefore set to zero in shared memory wherever some row of the operand does not see the key (blocks with
+// tree nodes, blocks behind the last key, and all blocks when there are copies), and added to the rows that do see them
+// when the unit's result is written.
+#pragma once
+#include "common.cuh"
+#include "tc_common.cuh"
+#include <type_traits>
+
+namespace wkb {
+int* gemm_status_word();
+
+namespace tree {
+
+constexpr int TC_THREADS = 320, KBLK = 128, QROWS = 128, SUB = 128 * 128;
+
+// Header of the scratch: where share c begins, for the join.  Then (m, l) and O of two pieces a share.
+struct ShareStart {
+  int unit_start, unit_len, share, tree, head, rowblk, total, pad;
+};
+struct Scratch {
+  ShareStart* start;
+  float2* ml;
+  float* o;
+  int rows;      // rows a piece has room for
+};
+__host__ __device__ inline int piece_rows(i64 max_nodes, i64 group) {
+  const i64 r = max_nodes * group;
+  return (int)(r < QROWS ? r : QROWS);
+}
+inline i64 scratch_bytes(i64 max_nodes, i64 group, i64 hd) {
+  const i64 rows = 2 * WKB_SM_COUNT * (i64)piece_rows(max_nodes, group);
+  return (i64)sizeof(ShareStart) * WKB_SM_COUNT + rows * 8 + rows * hd * 4;
+}
+inline Scratch carve(void* p, i64 max_nodes, i64 group) {
+  const int r = piece_rows(max_nodes, group);
+  uint8_t* b = static_cast<uint8_t*>(p);
+  Scratch s;
+  s.start = reinterpret_cast<ShareStart*>(b);
+  s.ml = reinterpret_cast<float2*>(b + sizeof(ShareStart) * WKB_SM_COUNT);
+  s.o = reinterpret_cast<float*>(b + sizeof(ShareStart) * WKB_SM_COUNT + (i64)2 * WKB_SM_COUNT * r * 8);
+  s.rows = r;
+  return s;
+}
+static_assert(sizeof(ShareStart) % 16 == 0, "the planes behind the header stay 16-byte aligned");
+
+template <int HD, int QS>
+struct TcSmem {
+  static constexpr int NSUB = HD / 64, BLK = NSUB * SUB;                 // bytes of 128 rows of an operand
+  static constexpr int HEADER = 3072;                                    // barriers, (m, l) of the teams, flags
+  static constexpr int Q_BYTES = QS * BLK < 32768 ? 32768 : QS * BLK;    // also the 256 x CW f32 of the epilogue
+  static constexpr int CW = Q_BYTES >= 65536 ? 64 : 32;
+  static constexpr int SLOTS = (232448 - HEADER - Q_BYTES) / BLK > 12 ? 12 : (232448 - HEADER - Q_BYTES) / BLK;
+  static constexpr int NK = (SLOTS + 1) / 2, NV = SLOTS / 2;
+  static constexpr int BYTES = HEADER + Q_BYTES + SLOTS * BLK;
+  static_assert(NV >= 2 && BYTES <= 232448, "at least two blocks of each operand in flight");
+};
+
+__host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_mn) {      // kind::f16: D f32, A = B = bf16, M = 128
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(QROWS >> 4) << 24);
+}
+// MN-major operand, 128-byte swizzle (the V rows as they lie in the cache): 64 dims a 128-byte row, 8 keys an atom
+__device__ __forceinline__ uint64_t sdesc_mn(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(SUB >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(id),
+               "r"(accumulate)
+               : "memory");
+}
+#define WKB_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define WKB_I8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t* r) {      // 32 columns of this thread's lane; wait with tm_ld_wait
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : WKB_R8(r, 0), WKB_R8(r, 8), WKB_R8(r, 16), WKB_R8(r, 24)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      WKB_I8(r, 0), WKB_I8(r, 8)
+      : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      WKB_I8(r, 0), WKB_I8(r, 8), WKB_I8(r, 16), WKB_I8(r, 24)
+      : "memory");
+}
+#undef WKB_R8
+#undef WKB_I8
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// non-zero when one of a word's two bf16 has an exponent of all ones
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t low_bits(i64 n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// A tree's share of the work list.
+struct TreeWork {
+  TreeRef t;
+  int keys, blocks, rowblks;
+};
+__device__ __forceinline__ TreeWork tree_work(const Geo& g, const int* slot, const int* ctx, const int* row0, int t) {
+  TreeWork w;
+  w.t = tree_ref(g, slot, ctx, row0, t);
+  const i64 keys = (i64)w.t.ctx + w.t.nodes, cover = (i64)g.mbps * g.page_tokens;
+  w.keys = (int)(keys < cover ? keys : cover);
+  w.t.ctx = min(w.t.ctx, w.keys);
+  w.blocks = (w.keys + KBLK - 1) / KBLK;
+  w.rowblks = (w.t.nodes * (g.q_heads / g.kv_heads) + QROWS - 1) / QROWS;      // 0 for a tree without rows
+  return w;
+}
+__device__ __forceinline__ int tree_items(const Geo& g, const TreeWork& w) { return w.blocks * w.rowblks * g.kv_heads; }
+
+// One piece of a unit: blocks [b0, b1) of `unit_len`.
+struct Piece {
+  TreeWork w;
+  int tree, head, rowblk, unit_start, b0, b1;
+};
+// Walks a share: item is its position in the list, tree_start that of tree `tree`.
+struct Walk {
+  int item, end, tree, tree_start;
+  __device__ __forceinline__ bool next(const Geo& g, const int* slot, const int* ctx, const int* row0, Piece& p) {
+    if (item >= end) return false;
+    for (;;) {
+      p.w = tree_work(g, slot, ctx, row0, tree);
+      const int items = tree_items(g, p.w);
+      if (item < tree_start + items) break;
+      tree_start += items;
+      if (++tree >= g.n_trees) return false;
+    }
+    const int unit = (item - tree_start) / p.w.blocks;
+    p.tree = tree;
+    p.head = unit / p.w.rowblks;
+    p.rowblk = unit % p.w.rowblks;
+    p.unit_start = tree_start + unit * p.w.blocks;
+    p.b0 = item - p.unit_start;
+    p.b1 = min(p.w.blocks, p.b0 + end - item);
+    item = p.unit_start + p.b1;
+    return true;
+  }
+};
+
+template <int HD, int QS, int PS>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const void* __restrict__ q,
+                    const u16* __restrict__ vcache, const uint32_t* __restrict__ block_table, const int* __restrict__ slot,
+                    const int* __restrict__ ctxs, const int* __restrict__ row0s, const uint32_t* __restrict__ mask, void* __restrict__ out, int out_dtype,
+                    Geo g, int box_rows, float scale, Scratch scr, int* __restrict__ status) {
+  using SM = TcSmem<HD, QS>;
+  constexpr int NK = SM::NK, NV = SM::NV, NSUB = SM::NSUB, BLK = SM::BLK;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  // header: barriers at 0, flags at 256, (m, l) at 512 .. 2560; the operands behind it on a 1024-byte boundary
+  const uint32_t q_base = (raw + 2560 + 1023u) & ~1023u, k_ring = q_base + SM::Q_BYTES, v_ring = k_ring + NK * BLK;
+  auto kfull = [&](int s) { return raw + 8u * s; };
+  auto kempty = [&](int s) { return raw + 8u * (NK + s); };
+  auto vfull = [&](int s) { return raw + 8u * (2 * NK + s); };
+  auto vempty = [&](int s) { return raw + 8u * (2 * NK + NV + s); };
+  const uint32_t more = raw + 8u * (2 * NK + 2 * NV);
+  auto s_full = [&](int t) { return more + 8u * t; };
+  auto p_full = [&](int t) { return more + 8u * (2 + t); };
+  auto o_done = [&](int t) { return more + 8u * (4 + t); };
+  const uint32_t q_full = more + 8u * 6;
+  static_assert(8 * (2 * NK + 2 * NV + 7) <= 256, "barriers fit the header");
+  volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + 256);      // 0 tensor memory, 1 failed, 2 V not finite, 3.. the share
+  float2* ml_s = reinterpret_cast<float2*>(smem_raw + 512);
+  float* stage = reinterpret_cast<float*>(smem_raw + (q_base - raw));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (q_base - raw > (uint32_t)SM::HEADER) {      // the operands would not fit behind the header: never, as the base is 1024-byte aligned
+    if (threadIdx.x == 0) atomicExch(status, WKB_STATUS_ATTN_WAIT);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NK; ++s) { mbar_init(kfull(s), 1); mbar_init(kempty(s), 1); }
+    for (int s = 0; s < NV; ++s) { mbar_init(vfull(s), 1); mbar_init(vempty(s), 1); }
+    for (int t = 0; t < 2; ++t) { mbar_init(s_full(t), 1); mbar_init(p_full(t), 4); mbar_init(o_done(t), 1); }
+    mbar_init(q_full, 8);
+    flags[1] = 0; flags[2] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(raw + 256), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+  // ---- this CTA's share: prefix sums of the trees' items over the threads, a contiguous run of trees each
+  {
+    int* sums = reinterpret_cast<int*>(ml_s);      // 10 warps
+    const int per = (g.n_trees + TC_THREADS - 1) / TC_THREADS, t0 = threadIdx.x * per, t1 = min(t0 + per, g.n_trees);
+    int mine = 0;
+    for (int t = t0; t < t1; ++t) mine += tree_items(g, tree_work(g, slot, ctxs, row0s, t));
+    int scan = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) sums[warp] = scan;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    int before = 0, total = 0;
+    for (int w = 0; w < TC_THREADS / 32; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
+    const int share = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int first = (int)blockIdx.x * share;
+    int at = before + scan - mine;
+    if (first < total && first >= at && first < at + mine) {
+      int t = t0;
+      for (;; ++t) {
+        const int n = tree_items(g, tree_work(g, slot, ctxs, row0s, t));
+        if (first < at + n) break;
+        at += n;
+      }
+      flags[3] = t; flags[4] = at;
+    }
+    if (threadIdx.x == 0) { flags[5] = min(first, total); flags[6] = min(first + share, total); flags[7] = share; flags[8] = total; }
+    __syncthreads();
+  }
+  const uint32_t tmem = (uint32_t)flags[0];
+  Walk walk{flags[5], flags[6], flags[3], flags[4]};
+  const int share = flags[7], total = flags[8];
+  const int group = g.q_heads / g.kv_heads;
+  const bool none = walk.item >= walk.end;
+  if (threadIdx.x == 0) {      // what the join has to know about the unit that this share begins in
+    ShareStart st{0, 0, share, 0, 0, 0, total, 0};
+    if (!none) {
+      Walk w = walk;
+      Piece p;
+      w.next(g, slot, ctxs, row0s, p);
+      st.unit_start = p.unit_start; st.unit_len = p.w.blocks; st.tree = p.tree; st.head = p.head; st.rowblk = p.rowblk;
+    }
+    scr.start[blockIdx.x] = st;
+  }
+  if (none) {
+    // nothing to do
+  } else if (warp == 0) {
+    // ---------------- TMA: lane i brings the i-th box (a page, or 128 tokens of a larger one) of a block ----------------
+    Piece p;
+    int n = 0, k_issued = 0, v_issued = 0;      // blocks so far, over all pieces of the share
+    bool ok = true;
+    const int boxes = KBLK / box_rows;
+    while (ok && walk.next(g, slot, ctxs, row0s, p)) {
+      const uint32_t* bt = block_table + (i64)p.w.t.slot * g.mbps;
+      const i64 oob = g.num_pages * g.kv_heads * g.page_tokens;
+      // cache row of this lane's box in block b; boxes behind the last key repeat the last page (their keys are not seen)
+      auto cache_row = [&](int b) -> int {
+        const int pos = min(b * KBLK + (lane % boxes) * box_rows, (p.w.keys - 1) / box_rows * box_rows);
+        const uint32_t page = bt[pos >> g.page_shift];
+        return page < (uint64_t)g.num_pages ? (int)(((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) : (int)oob;
+      };
+      auto load = [&](int i, bool is_v, int row) {
+        const int s = i % (is_v ? NV : NK), use = i / (is_v ? NV : NK);
+        const uint32_t fb = is_v ? vfull(s) : kfull(s), eb = is_v ? vempty(s) : kempty(s);
+        int good = 1;
+        if (lane == 0) {
+          good = mbar_wait_parked(eb, (use & 1) ^ 1) ? 1 : 0;
+          if (good) mbar_expect_tx(fb, BLK);
+        }
+        if (!__shfl_sync(0xffffffffu, good, 0)) return false;
+        __syncwarp();
+        if (lane < boxes) {
+          const uint32_t dst = (is_v ? v_ring : k_ring) + s * BLK + (uint32_t)(lane * box_rows) * 128u;
+#pragma unroll
+          for (int h = 0; h < NSUB; ++h) tma_load_2d(dst + h * SUB, is_v ? &map_v : &map_k, fb, 64 * h, row);
+        }
+        __syncwarp();
+        return true;
+      };
+      // K one block ahead of V, the order in which the MMA warp frees the slots
+      const int len = p.b1 - p.b0;
+      int row = cache_row(p.b0);
+      ok = load(n, false, row);
+      if (ok) k_issued = n + 1;
+      for (int j = 0; j < len && ok; ++j) {
+        const int ahead = j + 1 < len ? cache_row(p.b0 + j + 1) : 0;
+        if (j + 1 < len) {
+          ok = load(n + j + 1, false, ahead);
+          if (!ok) break;
+          k_issued = n + j + 2;
+        }
+        ok = load(n + j, true, row);
+        if (!ok) break;
+        v_issued = n + j + 1;
+        row = ahead;
+      }
+      n += len;
+    }
+    if (!ok && lane == 0) {
+      atomicExch(status, WKB_STATUS_ATTN_WAIT);
+      flags[1] = 1;
+      for (int i = max(0, k_issued - NK); i < k_issued; ++i) mbar_wait_parked(kfull(i % NK), (i / NK) & 1);      // copies in flight
+      for (int i = max(0, v_issued - NV); i < v_issued; ++i) mbar_wait_parked(vfull(i % NV), (i / NV) & 1);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA: S two blocks ahead, each P V as its team delivers P ----------------
+    if (lane == 0) {
+      constexpr uint32_t ID_S = tc_idesc(KBLK, false), ID_O = tc_idesc(HD, true);
+      Piece p;
+      int n = 0, pieces = 0;
+      int uses[2] = {0, 0};      // P V products of each team so far
+      bool ok = true;
+      while (ok && walk.next(g, slot, ctxs, row0s, p)) {
+        const int len = p.b1 - p.b0;
+        auto scores = [&](int j) {
+          const int i = n + j, s = i % NK;
+          if (!mbar_wait(kfull(s), (i / NK) & 1)) return false;
+          tc_fence_after();
+          const uint32_t kaddr = k_ring + s * BLK;
+#pragma unroll
+          for (int part = 0; part < QS; ++part)
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+              const uint32_t off = (uint32_t)(k >> 2) * SUB + (uint32_t)(k & 3) * 32u;
+              umma_bf16(tmem + (j & 1) * 128, make_sdesc(q_base + part * BLK + off), make_sdesc(kaddr + off), ID_S, (part > 0 || k > 0) ? 1u : 0u);
+            }
+          umma_commit(s_full(j & 1));
+          umma_commit(kempty(s));
+          return true;
+        };
+        ok = mbar_wait(q_full, pieces & 1);
+        ++pieces;
+        ok = ok && scores(0);
+        if (len > 1) ok = ok && scores(1);
+        for (int j = 0; j < len && ok; ++j) {
+          const int t = j & 1, i = n + j, s = i % NV;
+          ok = mbar_wait(p_full(t), uses[t] & 1) && mbar_wait(vfull(s), (i / NV) & 1);
+          if (!ok) break;
+          ++uses[t];
+          tc_fence_after();
+          const uint32_t vaddr = v_ring + s * BLK, o_col = tmem + 256 + t * HD;
+          // 32 keys take 32 columns of P: 16 of the hi part (two keys a column), 16 of the lo part
+#pragma unroll
+          for (int k = 0; k < KBLK / 16; ++k)
+#pragma unroll
+            for (int part = 0; part < PS; ++part)
+              mma_ts(o_col, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8, sdesc_mn(vaddr + (uint32_t)k * 2048u), ID_O,
+                     (j > 1 || k > 0 || part > 0) ? 1u : 0u);
+          umma_commit(vempty(s));
+          umma_commit(o_done(t));
+          if (j + 2 < len) ok = scores(j + 2);
+        }
+        n += len;
+      }
+      if (!ok) { atomicExch(status, WKB_STATUS_ATTN_WAIT); flags[1] = 1; }
+    }
+  } else {
+    // ---------------- softmax teams ----------------
+    const int team = (warp - 2) >> 2, quarter = warp & 3, a = quarter * 32 + lane, tid = threadIdx.x - 64;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), s_col = lane_base + team * 128, o_col = lane_base + 256 + team * HD;
+    // scores in base 2; the sign of `scale` goes into the query; never 0, which would make NaN of a hidden key's -inf
+    const float sc = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-37f);
+    const bool negate = scale < 0.0f;
+    bool ok = true;
+    int n = 0, uses = 0;      // blocks of the share, this team's blocks
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
+        ok = false;
+        if (lane == 0) { atomicExch(status, WKB_STATUS_ATTN_WAIT); flags[1] = 1; }
+      }
+    };
+    auto teams_sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };      // every softmax thread passes every one of these
+    Piece p;
+    while (walk.next(g, slot, ctxs, row0s, p)) {
+      const int len = p.b1 - p.b0;
+      const int live = min(QROWS, p.w.t.nodes * group - p.rowblk * QROWS);
+      const int copies = live <= 32 ? 4 : live <= 64 ? 2 : 1, crows = QROWS / copies;
+      const int copy = a / crows, r = a % crows;
+      // ---- the query operand: K-major, 128-byte swizzle
+      // (a row is loaded once and stored to every copy; the loads of a batch are in flight together)
+      {
+        constexpr int CH = HD / 8, BATCH = 2;      // 16-byte chunks of bf16 a row
+        for (int i0 = tid; i0 < crows * CH; i0 += 256 * BATCH) {
+          uint4 part[BATCH][QS < 2 ? 2 : QS];
+          float4 x[BATCH], y[BATCH];
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            const int idx = i0 + b * 256, qr = idx / CH, c = idx % CH;
+            x[b] = y[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            part[b][0] = make_uint4(0u, 0u, 0u, 0u);
+            if (qr >= live) continue;
+            const int ur = p.rowblk * QROWS + qr;
+            const i64 at = (i64)(p.w.t.row0 + ur / group) * g.q_row_stride + ((i64)p.head * group + ur % group) * HD + c * 8;
+            if (QS == 1) part[b][0] = *reinterpret_cast<const uint4*>(static_cast<const u16*>(q) + at);
+            else {
+              x[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
+              y[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + 4);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            const int idx = i0 + b * 256, qr = idx / CH, c = idx % CH;
+            if (idx >= crows * CH) break;
+            if (QS > 1) {
+              float f[8] = {x[b].x, x[b].y, x[b].z, x[b].w, y[b].x, y[b].y, y[b].z, y[b].w};
+#pragma unroll
+              for (int k = 0; k < QS; ++k) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  w[e] = pack_bf16(f[2 * e], f[2 * e + 1]);
+                  f[2 * e] -= u2f(w[e] << 16);
+                  f[2 * e + 1] -= u2f(w[e] & 0xffff0000u);
+                }
+                part[b][k] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+            const uint32_t flip = negate ? 0x80008000u : 0u;
+            const uint32_t dst = q_base + (uint32_t)(c >> 3) * SUB + (uint32_t)qr * 128u + (uint32_t)(((c & 7) ^ (qr & 7)) << 4);
+#pragma unroll
+            for (int k = 0; k < QS; ++k)
+              for (int cp = 0; cp < copies; ++cp)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * BLK + (uint32_t)(cp * crows) * 128u), "r"(part[b][k].x ^ flip),
+                             "r"(part[b][k].y ^ flip), "r"(part[b][k].z ^ flip), "r"(part[b][k].w ^ flip)
+                             : "memory");
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+
+      // ---- the team's key blocks
+      const int urow = p.rowblk * QROWS + min(r, live - 1);
+      const uint32_t* mrow = mask + (i64)(p.w.t.row0 + urow / group) * g.mask_words;
+      const int words = (p.w.t.nodes + 31) >> 5;
+      // which of the keys pos .. pos + 31 this row sees
+      auto visible = [&](int pos) -> uint32_t {
+        uint32_t bits = low_bits((i64)p.w.t.ctx - pos);
+        const i64 j = (i64)pos - p.w.t.ctx;
+        if (j > -32) {
+          if (j < 0) bits |= mrow[0] << (int)-j;
+          else {
+            const int w = (int)(j >> 5);
+            const uint32_t lo = w < words ? mrow[w] : 0u, hi = w + 1 < words ? mrow[w + 1] : 0u;
+            bits |= __funnelshift_r(lo, hi, (int)(j & 31));
+          }
+        }
+        return bits & low_bits((i64)p.w.keys - pos);
+      };
+      float m = -INFINITY, l = 0.0f;      // m in base 2, the maximum in use
+      auto block = [&](auto width_c, int j) {
+        constexpr int W = decltype(width_c)::value;
+        const int pos = (p.b0 + j) * KBLK + copy * W;
+        const int block_end = (p.b0 + j + 1) * KBLK;
+        float s[W];
+#pragma unroll
+        for (int c = 0; c < W / 32; ++c) tm_ld32(s_col + copy * W + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+        tm_ld_wait();
+        if (block_end > p.w.t.ctx) {
+#pragma unroll
+          for (int c = 0; c < W / 32; ++c) {
+            const uint32_t bits = visible(pos + c * 32);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[c * 32 + e] = (bits >> e) & 1u ? s[c * 32 + e] : -INFINITY;
+          }
+        }
+        float b4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < W; ++e) b4[e & 3] = fmaxf(b4[e & 3], s[e]);
+        const float top = fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3])) * sc;
+        const bool move = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
+        if (__any_sync(0xffffffffu, move)) {
+          const float next = move ? top : m;
+          const float corr = move ? ex2(m - next) : 1.0f;      // 0 when nothing had been seen
+          if (j > 1) {      // the accumulator holds this team's earlier blocks
+            wait(o_done(team), (uses - 1) & 1);
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tm_ld32(o_col + c, o);
+              tm_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = f2u(u2f(o[e]) * corr);
+              tm_st32(o_col + c, o);
+            }
+          }
+          l *= corr;
+          m = next;
+        }
+        const float m_use = m == -INFINITY ? 0.0f : m;
+        float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < W / 32; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = ex2(ffma(s[c * 32 + e], sc, -m_use)), p1 = ex2(ffma(s[c * 32 + e + 1], sc, -m_use));
+            l4[(e >> 1) & 1] += p0;
+            l4[2 + ((e >> 1) & 1)] += p1;
+            pk[e >> 1] = pack_bf16(p0, p1);
+            if (PS == 2) pk[16 + (e >> 1)] = pack_bf16(p0 - u2f(pk[e >> 1] << 16), p1 - u2f(pk[e >> 1] & 0xffff0000u));
+          }
+          if (PS == 2) tm_st32(s_col + copy * W + c * 32, pk);
+          else tm_st16(s_col + copy * W + c * 32, pk);
+        }
+        if (W < KBLK) {      // the other copies' keys
+          uint32_t zero[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) zero[e] = 0u;
+#pragma unroll
+          for (int c = 0; c < KBLK / 32; ++c)
+            if (c / (W / 32) != copy) {
+              if (PS == 2) tm_st32(s_col + c * 32, zero);
+              else tm_st16(s_col + c * 32, zero);
+            }
+        }
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+      };
+      for (int j = team; j < len; j += 2) {
+        wait(s_full(team), uses & 1);
+        tc_fence_after();
+        if (copies == 4) block(std::integral_constant<int, 32>(), j);
+        else if (copies == 2) block(std::integral_constant<int, 64>(), j);
+        else block(std::integral_constant<int, 128>(), j);
+        // V rows that some row of the operand does not see
+        if (copies > 1 || (p.b0 + j + 1) * KBLK > p.w.t.ctx) {
+          const int i = n + j, sl = i % NV, row = quarter * 32 + lane;
+          wait(vfull(sl), (i / NV) & 1);
+          const bool real = (p.b0 + j) * KBLK + row < p.w.keys;
+          const uint32_t vrow = v_ring + sl * BLK + (uint32_t)row * 128u;
+          bool hit = false;
+#pragma unroll
+          for (int h = 0; h < NSUB; ++h)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint32_t at = vrow + h * SUB + (uint32_t)((c ^ (row & 7)) << 4);
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+              if (not_finite2(w[0]) | not_finite2(w[1]) | not_finite2(w[2]) | not_finite2(w[3])) {
+                hit = true;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t bad = not_finite2(w[e]);
+                  w[e] &= ((bad & 0x8000u) ? 0u : 0xffffu) | ((bad & 0x80000000u) ? 0u : 0xffff0000u);
+                }
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+              }
+            }
+          if (hit) {
+            if (real) flags[2] = 1;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+        }
+        tm_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(team));
+        ++uses;
+      }
+      n += len;
+
+      // ---- add up the teams and the copies, CW columns at a time through the query operand's memory
+      constexpr int CW = SM::CW;
+      const bool mine = team < len;      // this team had a block
+      if (mine) { wait(o_done(team), (uses - 1) & 1); tc_fence_after(); }
+      ml_s[team * QROWS + a] = make_float2(mine ? m : -INFINITY, mine ? l : 0.0f);
+      teams_sync();
+      const int teams = min(len, 2), parts = teams * copies;      // part i of a row: ml_s[i * crows + row] (copies of team 0, then of team 1)
+      float m_all = -INFINITY, l_all = 0.0f;
+      for (int i = 0; i < parts; ++i) m_all = fmaxf(m_all, ml_s[i * crows + r].x);
+      const float m_use = m_all == -INFINITY ? 0.0f : m_all;
+      for (int i = 0; i < parts; ++i) {
+        const float2 v = ml_s[i * crows + r];
+        l_all += v.y * ex2(v.x - m_use);
+      }
+      const bool whole = len == p.w.blocks, fine = flags[1] == 0, bad_v = flags[2] != 0;
+      float w_mine = ex2(m - m_use);
+      if (whole) w_mine *= l_all != 0.0f ? 1.0f / l_all : 0.0f;      // a unit in one piece is normalised here
+      // a share's piece that begins the share is its even one; a later one that it does not finish is its odd one
+      const int piece = p.unit_start + p.b0 == (int)blockIdx.x * share ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
+      if (!whole && fine && team == 0 && copy == 0 && r < live) scr.ml[(i64)piece * scr.rows + r] = make_float2(m_all, l_all);
+#pragma unroll 1
+      for (int c0 = 0; c0 < HD; c0 += CW) {
+        if (mine) {
+#pragma unroll 1
+          for (int c1 = 0; c1 < CW; c1 += 32) {
+            uint32_t o[32];
+            tm_ld32(o_col + c0 + c1, o);
+            tm_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = f2u(u2f(o[e]) * w_mine);
+            if (bad_v && team == 0 && copy == 0 && r < live) {      // rare: the V elements that were set to zero, for the rows that see them
+              const int from = copies > 1 ? p.b0 * KBLK : max(p.b0 * KBLK, p.w.t.ctx / KBLK * KBLK);
+              for (int pos = from; pos < min(p.b1 * KBLK, p.w.keys); ++pos) {
+                if (!(visible(pos) & 1u)) continue;
+                const uint32_t page = block_table[(i64)p.w.t.slot * g.mbps + (pos >> g.page_shift)];
+                if (page >= (uint64_t)g.num_pages) continue;
+                const u16* v = vcache + (((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) * HD + c0 + c1;
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if ((v[e] & 0x7f80u) == 0x7f80u) o[e] = f2u(u2f(o[e]) + bf16_bits_to_f32(v[e]));
+              }
+            }
+            float4* d = reinterpret_cast<float4*>(stage + (team * QROWS + a) * CW + c1);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e ^ (a & 7)] = make_float4(u2f(o[4 * e]), u2f(o[4 * e + 1]), u2f(o[4 * e + 2]), u2f(o[4 * e + 3]));
+          }
+        }
+        teams_sync();
+        constexpr int C4 = CW / 4;
+        for (int idx = tid; idx < live * C4; idx += 256) {
+          const int row = idx / C4, c4 = idx % C4;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int i = 0; i < parts; ++i) {
+            const int x = i * crows + row;
+            const float4 s4 = *reinterpret_cast<const float4*>(stage + x * CW + ((c4 ^ (x & 7)) << 2));
+            v.x += s4.x; v.y += s4.y; v.z += s4.z; v.w += s4.w;
+          }
+          if (!fine) continue;
+          if (whole) {
+            const int ur = p.rowblk * QROWS + row;
+            const i64 at = (i64)(p.w.t.row0 + ur / group) * g.out_row_stride + ((i64)p.head * group + ur % group) * HD + c0 + c4 * 4;
+            if (out_dtype == 0) *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
+            else *reinterpret_cast<uint2*>(static_cast<u16*>(out) + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+          } else *reinterpret_cast<float4*>(scr.o + ((i64)piece * scr.rows + row) * HD + c0 + c4 * 4) = v;
+        }
+        teams_sync();
+      }
+      if (tid == 0) flags[2] = 0;
+      teams_sync();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// Block (c, rows): if the boundary before share c falls inside a unit, and is the first one that does, join the unit's
+// pieces (in key order) for these rows and write the result.
+template <int HD>
+__global__ void __launch_bounds__(256) tree_attn_join_kernel(const int* __restrict__ slot, const int* __restrict__ ctxs, const int* __restrict__ row0s,
+                                                             void* __restrict__ out, int out_dtype, Geo g, Scratch scr, const int* __restrict__ status) {
+  pdl_wait();
+  pdl_trigger();
+  const int c = blockIdx.x + 1;
+  const ShareStart st = scr.start[c];
+  const int x = c * st.share;
+  if (x >= st.total || x == st.unit_start || x - st.share > st.unit_start) return;
+  if (*status == WKB_STATUS_ATTN_WAIT) return;
+  const int last = (st.unit_start + st.unit_len - 1) / st.share, group = g.q_heads / g.kv_heads;
+  const TreeRef t = tree_ref(g, slot, ctxs, row0s, st.tree);
+  const int live = min(QROWS, t.nodes * group - st.rowblk * QROWS);
+  constexpr int LANES = HD / 4;
+  const int row = blockIdx.y * (256 / LANES) + threadIdx.x / LANES, col = threadIdx.x % LANES * 4;
+  if (row >= live) return;
+  auto piece = [&](int k) { return (i64)(k * st.share >= st.unit_start ? 2 * k : 2 * k + 1) * scr.rows + row; };
+  float m = -INFINITY;
+  for (int k = c - 1; k <= last; ++k) m = fmaxf(m, scr.ml[piece(k)].x);
+  const float use = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int k = c - 1; k <= last; ++k) {
+    const float2 ml = scr.ml[piece(k)];
+    const float w = ex2(ml.x - use);
+    const float4 v = *reinterpret_cast<const float4*>(scr.o + piece(k) * HD + col);
+    l += ml.y * w;
+    o.x += v.x * w; o.y += v.y * w; o.z += v.z * w; o.w += v.w * w;
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+  const int ur = st.rowblk * QROWS + row;
+  const i64 at = (i64)(t.row0 + ur / group) * g.out_row_stride + ((i64)st.head * group + ur % group) * HD + col;
+  if (out_dtype == 0) *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = o;
+  else *reinterpret_cast<uint2*>(static_cast<u16*>(out) + at) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+}
+
+// One layer's cache as a matrix [num_pages * kv_heads * page_tokens][head_dim] of bf16; box = box_rows tokens of one head
+// x 64 dims, 128-byte swizzle.  Rows past the cache read as zeros.
+inline int cache_map(CUtensorMap* map, const void* cache, i64 rows, i64 head_dim, int box_rows) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return (int)cudaErrorNotSupported;
+  cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+template <int HD, int QS, int PS>
+int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt, const int* slot, const int* ctx, const int* row0, const uint32_t* mask,
+              void* out, int out_dtype, const Geo& g, float scale, void* scratch, cudaStream_t st) {
+  const int box_rows = g.page_tokens < KBLK ? g.page_tokens : KBLK;
+  const i64 cache_rows = g.num_pages * g.kv_heads * g.page_tokens;
+  CUtensorMap mk, mv;
+  int rc = cache_map(&mk, kc, cache_rows, HD, box_rows);
+  if (rc) return rc;
+  rc = cache_map(&mv, vc, cache_rows, HD, box_rows);
+  if (rc) return rc;
+  int* status = gemm_status_word();
+  if (!status) return (int)cudaErrorMemoryAllocation;
+  auto kern = tree_attn_tc_kernel<HD, QS, PS>;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[dev & 63]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<HD, QS>::BYTES);
+    if (e != cudaSuccess) return (int)e;
+    attr_set[dev & 63] = true;
+  }
+  const int group = g.q_heads / g.kv_heads;
+  const Scratch scr = carve(scratch, g.max_nodes, group);
+  cudaError_t e = launch_pdl(kern, WKB_SM_COUNT, TC_THREADS, (size_t)TcSmem<HD, QS>::BYTES, st, mk, mv, q, (const u16*)vc, bt, slot, ctx, row0, mask, out,
+                             out_dtype, g, box_rows, scale, scr, status);
+  if (e != cudaSuccess) return (int)e;
+  const int rows_per = 256 / (HD / 4);
+  return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(WKB_SM_COUNT - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, slot, ctx, row0, out,
+                         out_dtype, g, scr, (const int*)status);
+}
+
+}  // namespace tree
+}  // namespace wkb
