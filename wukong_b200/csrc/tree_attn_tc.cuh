@@ -6,7 +6,7 @@
 // covers is written at once; the pieces of the others go to scratch as (maximum, sum, unnormalised output) and are
 // joined by tree_attn_join_kernel in key order, so results are run-to-run identical.
 //
-// A CTA has a TMA warp (K and V pages into two rings), an MMA warp and two teams of four softmax warps.  The teams take
+// A CTA has two TMA warps (pages of K and of V into a ring each), an MMA warp and two teams of four softmax warps.  The teams take
 // alternate key blocks with tensor-memory columns of their own, so one team's exponentials run while the other's products
 // do:   S = Q K^T (128 x 128) -> P = exp2(S - m), bf16, over the same columns -> O += P V (128 x head_dim).
 // The running maximum m of a row moves only when a block exceeds it by 2^8; the accumulator is rescaled then and not at
@@ -17,10 +17,10 @@
 // (quarter) of a block's keys, with zeros for the others': a team's warps share the exponentials of a small tree that
 // would otherwise all fall to one of them.  The copies are added up like the pieces of a unit.
 //
-// V and 0 x NaN: a probability of zero does not silence a NaN or an infinity in the product.  V elements that are not
-// finite are therefore set to zero in shared memory wherever some row of the operand does not see the key (blocks with
-// tree nodes, blocks behind the last key, and all blocks when there are copies), and added to the rows that do see them
-// when the unit's result is written.
+// V and 0 x NaN: a probability of zero does not silence a NaN or an infinity in the product.  In the blocks with tree
+// nodes and behind the last key, where rows see different keys, V elements that are not finite are set to zero in shared
+// memory before the product.  Where the copies' zeros meet one in the committed context, which every row sees, the result
+// is not finite, as it has to be.  Either way the elements' own sum over the keys that a row sees is its result.
 #pragma once
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -31,7 +31,7 @@ int* gemm_status_word();
 
 namespace tree {
 
-constexpr int TC_THREADS = 320, KBLK = 128, QROWS = 128, SUB = 128 * 128;
+constexpr int TC_THREADS = 384, KBLK = 128, QROWS = 128, SUB = 128 * 128;
 
 // Header of the scratch: where share c begins, for the join.  Then (m, l) and O of two pieces a share.
 struct ShareStart {
@@ -63,6 +63,25 @@ inline Scratch carve(void* p, i64 max_nodes, i64 group) {
 }
 static_assert(sizeof(ShareStart) % 16 == 0, "the planes behind the header stay 16-byte aligned");
 
+// How a key block lies in shared memory: boxes of box_rows tokens, each with its 64-dim halves behind one another, so
+// that one copy brings whole rows of a page (half as many copies as halves apart, and their issue was the limit).  With
+// 16-token boxes of two halves the 8-key groups of a block are not evenly spaced; they are taken in two sets, the first
+// and the second groups of the boxes, each with a stride of one box (the order of the keys within a block is free).
+struct Layout {
+  int box_rows, sets;
+  uint32_t box_bytes, half_bytes, group_stride;
+};
+inline Layout block_layout(int page_tokens, int hd) {
+  Layout l;
+  const int halves = hd / 64;
+  l.box_rows = halves == 1 ? (page_tokens < KBLK ? page_tokens : KBLK) : page_tokens >= KBLK ? KBLK : page_tokens >= 16 ? 16 : 8;
+  l.half_bytes = (uint32_t)l.box_rows * 128;
+  l.box_bytes = l.half_bytes * halves;
+  l.sets = halves == 2 && l.box_rows == 16 ? 2 : 1;
+  l.group_stride = halves == 1 || l.box_rows == KBLK ? 1024 : l.box_bytes;
+  return l;
+}
+
 template <int HD, int QS>
 struct TcSmem {
   static constexpr int NSUB = HD / 64, BLK = NSUB * SUB;                 // bytes of 128 rows of an operand
@@ -78,9 +97,16 @@ struct TcSmem {
 __host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_mn) {      // kind::f16: D f32, A = B = bf16, M = 128
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(QROWS >> 4) << 24);
 }
-// MN-major operand, 128-byte swizzle (the V rows as they lie in the cache): 64 dims a 128-byte row, 8 keys an atom
-__device__ __forceinline__ uint64_t sdesc_mn(uint32_t saddr) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(SUB >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory operand with 128-byte swizzle, atoms of 8 rows of 128 bytes.  K-major (Q, K): sbo = distance of 8-row
+// groups, lbo not used.  MN-major (V as it lies in the cache, 64 dims a row): sbo = distance of 8-key groups, lbo of the halves.
+__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// One box of the cache, box_rows tokens x all dims of one head, as [64-dim half][token][128 bytes].
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
+               "r"(bar), "r"(0), "r"(row), "r"(0)
+               : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(id),
@@ -125,6 +151,21 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+// Parity wait of at most about a second; each try may park the thread until the phase completes.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+    if ((it & 255u) == 255u) {
+      uint64_t t;
+      asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > 1000000000ull) return false;
+    }
+  }
 }
 // non-zero when one of a word's two bf16 has an exponent of all ones
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
@@ -181,7 +222,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const void* __restrict__ q,
                     const u16* __restrict__ vcache, const uint32_t* __restrict__ block_table, const int* __restrict__ slot,
                     const int* __restrict__ ctxs, const int* __restrict__ row0s, const uint32_t* __restrict__ mask, void* __restrict__ out, int out_dtype,
-                    Geo g, int box_rows, float scale, Scratch scr, int* __restrict__ status) {
+                    Geo g, Layout lay, float scale, Scratch scr, int* __restrict__ status) {
   using SM = TcSmem<HD, QS>;
   constexpr int NK = SM::NK, NV = SM::NV, NSUB = SM::NSUB, BLK = SM::BLK;
   extern __shared__ uint8_t smem_raw[];
@@ -272,68 +313,57 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   }
   if (none) {
     // nothing to do
-  } else if (warp == 0) {
-    // ---------------- TMA: lane i brings the i-th box (a page, or 128 tokens of a larger one) of a block ----------------
+  } else if (warp == 0 || warp == TC_THREADS / 32 - 1) {
+    // ---------------- TMA: one warp for K, one for V; lane i brings the i-th box of a block ----------------
+    const bool is_v = warp != 0;
+    const uint32_t ring = is_v ? v_ring : k_ring;
+    const CUtensorMap* map = is_v ? &map_v : &map_k;
+    const int slots = is_v ? NV : NK, boxes = KBLK / lay.box_rows, per = 32 / boxes;
     Piece p;
-    int n = 0, k_issued = 0, v_issued = 0;      // blocks so far, over all pieces of the share
+    int n = 0;      // blocks so far, over all pieces of the share
     bool ok = true;
-    const int boxes = KBLK / box_rows;
     while (ok && walk.next(g, slot, ctxs, row0s, p)) {
       const uint32_t* bt = block_table + (i64)p.w.t.slot * g.mbps;
       const i64 oob = g.num_pages * g.kv_heads * g.page_tokens;
-      // cache row of this lane's box in block b; boxes behind the last key repeat the last page (their keys are not seen)
-      auto cache_row = [&](int b) -> int {
-        const int pos = min(b * KBLK + (lane % boxes) * box_rows, (p.w.keys - 1) / box_rows * box_rows);
+      // The warp holds the cache rows of 32 boxes (32 / boxes blocks), lane by lane, and the next 32 are on their way: a
+      // look-up a block, used at once, cost more than the copies.  Boxes behind the last key repeat the last page (their
+      // keys are not seen).
+      const int len = p.b1 - p.b0;
+      auto cache_rows = [&](int batch) -> int {
+        const i64 at = (i64)(p.b0 + batch * per) * KBLK + (i64)lane * lay.box_rows;
+        const int last = (p.w.keys - 1) / lay.box_rows * lay.box_rows, pos = at < last ? (int)at : last;
         const uint32_t page = bt[pos >> g.page_shift];
         return page < (uint64_t)g.num_pages ? (int)(((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) : (int)oob;
       };
-      auto load = [&](int i, bool is_v, int row) {
-        const int s = i % (is_v ? NV : NK), use = i / (is_v ? NV : NK);
+      int rows_now = cache_rows(0), rows_next = per < len ? cache_rows(1) : 0, in_batch = 0, batch = 0;
+      for (int j = 0; j < len; ++j) {
+        if (in_batch == per) {
+          in_batch = 0;
+          ++batch;
+          rows_now = rows_next;
+          if ((batch + 1) * per < len) rows_next = cache_rows(batch + 1);
+        }
+        const int row = __shfl_sync(0xffffffffu, rows_now, in_batch * boxes + (lane & (boxes - 1)));
+        ++in_batch;
+        const int s = n % slots;
         const uint32_t fb = is_v ? vfull(s) : kfull(s), eb = is_v ? vempty(s) : kempty(s);
-        int good = 1;
-        if (lane == 0) {
-          good = mbar_wait_parked(eb, (use & 1) ^ 1) ? 1 : 0;
-          if (good) mbar_expect_tx(fb, BLK);
-        }
-        if (!__shfl_sync(0xffffffffu, good, 0)) return false;
+        if (!__all_sync(0xffffffffu, bar_wait(eb, ((n / slots) & 1) ^ 1))) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(fb, BLK);
         __syncwarp();
-        if (lane < boxes) {
-          const uint32_t dst = (is_v ? v_ring : k_ring) + s * BLK + (uint32_t)(lane * box_rows) * 128u;
-#pragma unroll
-          for (int h = 0; h < NSUB; ++h) tma_load_2d(dst + h * SUB, is_v ? &map_v : &map_k, fb, 64 * h, row);
-        }
-        __syncwarp();
-        return true;
-      };
-      // K one block ahead of V, the order in which the MMA warp frees the slots
-      const int len = p.b1 - p.b0;
-      int row = cache_row(p.b0);
-      ok = load(n, false, row);
-      if (ok) k_issued = n + 1;
-      for (int j = 0; j < len && ok; ++j) {
-        const int ahead = j + 1 < len ? cache_row(p.b0 + j + 1) : 0;
-        if (j + 1 < len) {
-          ok = load(n + j + 1, false, ahead);
-          if (!ok) break;
-          k_issued = n + j + 2;
-        }
-        ok = load(n + j, true, row);
-        if (!ok) break;
-        v_issued = n + j + 1;
-        row = ahead;
+        if (lane < boxes) tma_box(ring + s * BLK + (uint32_t)lane * lay.box_bytes, map, fb, row);
+        ++n;
       }
-      n += len;
     }
     if (!ok && lane == 0) {
       atomicExch(status, WKB_STATUS_ATTN_WAIT);
       flags[1] = 1;
-      for (int i = max(0, k_issued - NK); i < k_issued; ++i) mbar_wait_parked(kfull(i % NK), (i / NK) & 1);      // copies in flight
-      for (int i = max(0, v_issued - NV); i < v_issued; ++i) mbar_wait_parked(vfull(i % NV), (i / NV) & 1);
+      for (int i = max(0, n - slots); i < n; ++i) bar_wait(is_v ? vfull(i % slots) : kfull(i % slots), (i / slots) & 1);      // copies in flight
     }
   } else if (warp == 1) {
     // ---------------- MMA: S two blocks ahead, each P V as its team delivers P ----------------
     if (lane == 0) {
-      constexpr uint32_t ID_S = tc_idesc(KBLK, false), ID_O = tc_idesc(HD, true);
+      const uint32_t id_s = lay.sets == 2 ? tc_idesc(KBLK / 2, false) : tc_idesc(KBLK, false);
+      constexpr uint32_t ID_O = tc_idesc(HD, true);
       Piece p;
       int n = 0, pieces = 0;
       int uses[2] = {0, 0};      // P V products of each team so far
@@ -342,27 +372,28 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const int len = p.b1 - p.b0;
         auto scores = [&](int j) {
           const int i = n + j, s = i % NK;
-          if (!mbar_wait(kfull(s), (i / NK) & 1)) return false;
+          if (!bar_wait(kfull(s), (i / NK) & 1)) return false;
           tc_fence_after();
           const uint32_t kaddr = k_ring + s * BLK;
+          for (int set = 0; set < lay.sets; ++set)
 #pragma unroll
-          for (int part = 0; part < QS; ++part)
+            for (int part = 0; part < QS; ++part)
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-              const uint32_t off = (uint32_t)(k >> 2) * SUB + (uint32_t)(k & 3) * 32u;
-              umma_bf16(tmem + (j & 1) * 128, make_sdesc(q_base + part * BLK + off), make_sdesc(kaddr + off), ID_S, (part > 0 || k > 0) ? 1u : 0u);
-            }
+              for (int k = 0; k < HD / 16; ++k)
+                umma_bf16(tmem + (j & 1) * 128 + set * (KBLK / 2), sdesc(q_base + part * BLK + (uint32_t)(k >> 2) * SUB + (uint32_t)(k & 3) * 32u, 16, 1024),
+                          sdesc(kaddr + set * 1024 + (uint32_t)(k >> 2) * lay.half_bytes + (uint32_t)(k & 3) * 32u, 16, lay.group_stride), id_s,
+                          (part > 0 || k > 0) ? 1u : 0u);
           umma_commit(s_full(j & 1));
           umma_commit(kempty(s));
           return true;
         };
-        ok = mbar_wait(q_full, pieces & 1);
+        ok = bar_wait(q_full, pieces & 1);
         ++pieces;
         ok = ok && scores(0);
         if (len > 1) ok = ok && scores(1);
         for (int j = 0; j < len && ok; ++j) {
           const int t = j & 1, i = n + j, s = i % NV;
-          ok = mbar_wait(p_full(t), uses[t] & 1) && mbar_wait(vfull(s), (i / NV) & 1);
+          ok = bar_wait(p_full(t), uses[t] & 1) && bar_wait(vfull(s), (i / NV) & 1);
           if (!ok) break;
           ++uses[t];
           tc_fence_after();
@@ -372,8 +403,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           for (int k = 0; k < KBLK / 16; ++k)
 #pragma unroll
             for (int part = 0; part < PS; ++part)
-              mma_ts(o_col, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8, sdesc_mn(vaddr + (uint32_t)k * 2048u), ID_O,
-                     (j > 1 || k > 0 || part > 0) ? 1u : 0u);
+              mma_ts(o_col, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8,
+                     sdesc(lay.sets == 2 ? vaddr + (uint32_t)(k >> 2) * 1024u + (uint32_t)(k & 3) * 2u * lay.group_stride : vaddr + (uint32_t)k * 2u * lay.group_stride,
+                           lay.half_bytes, lay.group_stride),
+                     ID_O, (j > 1 || k > 0 || part > 0) ? 1u : 0u);
           umma_commit(vempty(s));
           umma_commit(o_done(t));
           if (j + 2 < len) ok = scores(j + 2);
@@ -382,7 +415,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       if (!ok) { atomicExch(status, WKB_STATUS_ATTN_WAIT); flags[1] = 1; }
     }
-  } else {
+  } else if (warp < 10) {      // (warp 10 has no part: it makes the V warp the third of another scheduler)
     // ---------------- softmax teams ----------------
     const int team = (warp - 2) >> 2, quarter = warp & 3, a = quarter * 32 + lane, tid = threadIdx.x - 64;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), s_col = lane_base + team * 128, o_col = lane_base + 256 + team * HD;
@@ -392,7 +425,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     bool ok = true;
     int n = 0, uses = 0;      // blocks of the share, this team's blocks
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
+      if (ok && !__all_sync(0xffffffffu, bar_wait(bar, parity))) {
         ok = false;
         if (lane == 0) { atomicExch(status, WKB_STATUS_ATTN_WAIT); flags[1] = 1; }
       }
@@ -459,11 +492,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (lane == 0) mbar_arrive(q_full);
 
       // ---- the team's key blocks
-      const int urow = p.rowblk * QROWS + min(r, live - 1);
-      const uint32_t* mrow = mask + (i64)(p.w.t.row0 + urow / group) * g.mask_words;
+      auto mask_of = [&](int row) { return mask + (i64)(p.w.t.row0 + (p.rowblk * QROWS + row) / group) * g.mask_words; };
+      const uint32_t* own_mask = mask_of(min(r, live - 1));
       const int words = (p.w.t.nodes + 31) >> 5;
-      // which of the keys pos .. pos + 31 this row sees
-      auto visible = [&](int pos) -> uint32_t {
+      // which of the keys pos .. pos + 31 the row with this mask sees
+      auto visible = [&](const uint32_t* mrow, int pos) -> uint32_t {
         uint32_t bits = low_bits((i64)p.w.t.ctx - pos);
         const i64 j = (i64)pos - p.w.t.ctx;
         if (j > -32) {
@@ -488,7 +521,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (block_end > p.w.t.ctx) {
 #pragma unroll
           for (int c = 0; c < W / 32; ++c) {
-            const uint32_t bits = visible(pos + c * 32);
+            uint32_t bits;
+            if (lay.sets == 2) {      // 32 columns are the first (second) 8 keys of four boxes of 16
+              const int col = copy * W + c * 32, at = (p.b0 + j) * KBLK + (col & 32) * 2 + (col >> 6) * 8;
+              const uint32_t a2 = visible(own_mask, at), b2 = visible(own_mask, at + 32);
+              bits = (a2 & 0xffu) | (a2 >> 8 & 0xff00u) | (b2 & 0xffu) << 16 | (b2 << 8 & 0xff000000u);
+            } else bits = visible(own_mask, pos + c * 32);
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[c * 32 + e] = (bits >> e) & 1u ? s[c * 32 + e] : -INFINITY;
           }
@@ -552,32 +590,36 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (copies == 4) block(std::integral_constant<int, 32>(), j);
         else if (copies == 2) block(std::integral_constant<int, 64>(), j);
         else block(std::integral_constant<int, 128>(), j);
-        // V rows that some row of the operand does not see
-        if (copies > 1 || (p.b0 + j + 1) * KBLK > p.w.t.ctx) {
+        // V of keys that some row does not see
+        if ((p.b0 + j + 1) * KBLK > p.w.t.ctx) {
           const int i = n + j, sl = i % NV, row = quarter * 32 + lane;
           wait(vfull(sl), (i / NV) & 1);
-          const bool real = (p.b0 + j) * KBLK + row < p.w.keys;
-          const uint32_t vrow = v_ring + sl * BLK + (uint32_t)row * 128u;
+          const uint32_t vrow = v_ring + sl * BLK + (uint32_t)(row / lay.box_rows) * lay.box_bytes + (uint32_t)(row & (lay.box_rows - 1)) * 128u;
           bool hit = false;
 #pragma unroll
-          for (int h = 0; h < NSUB; ++h)
+          for (int h = 0; h < 2 * NSUB; ++h) {
+            uint32_t w[4][4];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const uint32_t at = vrow + h * SUB + (uint32_t)((c ^ (row & 7)) << 4);
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-              if (not_finite2(w[0]) | not_finite2(w[1]) | not_finite2(w[2]) | not_finite2(w[3])) {
+            for (int c = 0; c < 4; ++c)
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3])
+                           : "r"(vrow + (h >> 1) * lay.half_bytes + (uint32_t)((((h & 1) * 4 + c) ^ (row & 7)) << 4)));
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (not_finite2(w[c][0]) | not_finite2(w[c][1]) | not_finite2(w[c][2]) | not_finite2(w[c][3])) {
                 hit = true;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  const uint32_t bad = not_finite2(w[e]);
-                  w[e] &= ((bad & 0x8000u) ? 0u : 0xffffu) | ((bad & 0x80000000u) ? 0u : 0xffff0000u);
+                  const uint32_t bad = not_finite2(w[c][e]);
+                  w[c][e] &= ((bad & 0x8000u) ? 0u : 0xffffu) | ((bad & 0x80000000u) ? 0u : 0xffff0000u);
                 }
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(vrow + (h >> 1) * lay.half_bytes + (uint32_t)((((h & 1) * 4 + c) ^ (row & 7)) << 4)),
+                             "r"(w[c][0]), "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3])
+                             : "memory");
               }
-            }
+          }
           if (hit) {
-            if (real) flags[2] = 1;
+            if ((p.b0 + j) * KBLK + row < p.w.keys) flags[2] = 1;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
         }
@@ -619,18 +661,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             tm_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = f2u(u2f(o[e]) * w_mine);
-            if (bad_v && team == 0 && copy == 0 && r < live) {      // rare: the V elements that were set to zero, for the rows that see them
-              const int from = copies > 1 ? p.b0 * KBLK : max(p.b0 * KBLK, p.w.t.ctx / KBLK * KBLK);
-              for (int pos = from; pos < min(p.b1 * KBLK, p.w.keys); ++pos) {
-                if (!(visible(pos) & 1u)) continue;
-                const uint32_t page = block_table[(i64)p.w.t.slot * g.mbps + (pos >> g.page_shift)];
-                if (page >= (uint64_t)g.num_pages) continue;
-                const u16* v = vcache + (((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) * HD + c0 + c1;
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if ((v[e] & 0x7f80u) == 0x7f80u) o[e] = f2u(u2f(o[e]) + bf16_bits_to_f32(v[e]));
-              }
-            }
             float4* d = reinterpret_cast<float4*>(stage + (team * QROWS + a) * CW + c1);
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[e ^ (a & 7)] = make_float4(u2f(o[4 * e]), u2f(o[4 * e + 1]), u2f(o[4 * e + 2]), u2f(o[4 * e + 3]));
@@ -647,6 +677,23 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             v.x += s4.x; v.y += s4.y; v.z += s4.z; v.w += s4.w;
           }
           if (!fine) continue;
+          // rare: V holds a NaN or an infinity that this row may see.  Its sum over those elements is then the result
+          if (bad_v || (copies > 1 && !(fabsf(v.x) <= 3.402823466e+38f && fabsf(v.y) <= 3.402823466e+38f && fabsf(v.z) <= 3.402823466e+38f &&
+                                        fabsf(v.w) <= 3.402823466e+38f))) {
+            const uint32_t* mrow = mask_of(row);
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int pos = p.b0 * KBLK; pos < min(p.b1 * KBLK, p.w.keys); ++pos) {
+              if (!(visible(mrow, pos) & 1u)) continue;
+              const uint32_t page = block_table[(i64)p.w.t.slot * g.mbps + (pos >> g.page_shift)];
+              if (page >= (uint64_t)g.num_pages) continue;
+              const u16* vp = vcache + (((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) * HD + c0 + c4 * 4;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if ((vp[e] & 0x7f80u) == 0x7f80u) x[e] += bf16_bits_to_f32(vp[e]);
+            }
+            v.x = x[0] != 0.0f ? x[0] : v.x; v.y = x[1] != 0.0f ? x[1] : v.y;      // untouched where there was none
+            v.z = x[2] != 0.0f ? x[2] : v.z; v.w = x[3] != 0.0f ? x[3] : v.w;
+          }
           if (whole) {
             const int ur = p.rowblk * QROWS + row;
             const i64 at = (i64)(p.w.t.row0 + ur / group) * g.out_row_stride + ((i64)p.head * group + ur % group) * HD + c0 + c4 * 4;
@@ -708,29 +755,29 @@ __global__ void __launch_bounds__(256) tree_attn_join_kernel(const int* __restri
   else *reinterpret_cast<uint2*>(static_cast<u16*>(out) + at) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
 }
 
-// One layer's cache as a matrix [num_pages * kv_heads * page_tokens][head_dim] of bf16; box = box_rows tokens of one head
-// x 64 dims, 128-byte swizzle.  Rows past the cache read as zeros.
+// One layer's cache as [64-dim half][num_pages * kv_heads * page_tokens][64] of bf16; box = all halves of box_rows tokens
+// of one head, 128-byte swizzle.  Rows past the cache read as zeros.
 inline int cache_map(CUtensorMap* map, const void* cache, i64 rows, i64 head_dim, int box_rows) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return (int)cudaErrorNotSupported;
-  cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)(head_dim / 64)};
+  cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, 128};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, (cuuint32_t)(head_dim / 64)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
 template <int HD, int QS, int PS>
 int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt, const int* slot, const int* ctx, const int* row0, const uint32_t* mask,
               void* out, int out_dtype, const Geo& g, float scale, void* scratch, cudaStream_t st) {
-  const int box_rows = g.page_tokens < KBLK ? g.page_tokens : KBLK;
+  const Layout lay = block_layout(g.page_tokens, HD);
   const i64 cache_rows = g.num_pages * g.kv_heads * g.page_tokens;
   CUtensorMap mk, mv;
-  int rc = cache_map(&mk, kc, cache_rows, HD, box_rows);
+  int rc = cache_map(&mk, kc, cache_rows, HD, lay.box_rows);
   if (rc) return rc;
-  rc = cache_map(&mv, vc, cache_rows, HD, box_rows);
+  rc = cache_map(&mv, vc, cache_rows, HD, lay.box_rows);
   if (rc) return rc;
   int* status = gemm_status_word();
   if (!status) return (int)cudaErrorMemoryAllocation;
@@ -746,7 +793,7 @@ int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt,
   const int group = g.q_heads / g.kv_heads;
   const Scratch scr = carve(scratch, g.max_nodes, group);
   cudaError_t e = launch_pdl(kern, WKB_SM_COUNT, TC_THREADS, (size_t)TcSmem<HD, QS>::BYTES, st, mk, mv, q, (const u16*)vc, bt, slot, ctx, row0, mask, out,
-                             out_dtype, g, box_rows, scale, scr, status);
+                             out_dtype, g, lay, scale, scr, status);
   if (e != cudaSuccess) return (int)e;
   const int rows_per = 256 / (HD / 4);
   return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(WKB_SM_COUNT - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, slot, ctx, row0, out,
