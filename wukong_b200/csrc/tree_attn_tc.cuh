@@ -63,24 +63,15 @@ inline Scratch carve(void* p, i64 max_nodes, i64 group) {
 }
 static_assert(sizeof(ShareStart) % 16 == 0, "the planes behind the header stay 16-byte aligned");
 
-// How a key block lies in shared memory: boxes of box_rows tokens, each with its 64-dim halves behind one another, so
-// that one copy brings whole rows of a page (half as many copies as halves apart, and their issue was the limit).  With
-// 16-token boxes of two halves the 8-key groups of a block are not evenly spaced; they are taken in two sets, the first
-// and the second groups of the boxes, each with a stride of one box (the order of the keys within a block is free).
+// How a key block lies in shared memory: boxes of whole rows of a page, the 64-dim halves of a box behind one another (one
+// copy a box; copies of half rows were twice as many, and their issue was the limit).  With two halves a box is 8 tokens,
+// so that the block's 8-key groups are evenly spaced and one instruction multiplies all 128 keys; boxes of 16 tokens need
+// two of 64 keys each, and reading the query operand twice cost more (1.53 against 1.41 us a block) than it saved.
+template <int HD>
 struct Layout {
-  int box_rows, sets;
-  uint32_t box_bytes, half_bytes, group_stride;
+  static constexpr int HALVES = HD / 64, GROUP = 1024 * HALVES, HALF = 1024;      // distance of the 8-key groups, of the halves
+  static __host__ __device__ int box_rows(int page_tokens) { return HALVES == 2 ? 8 : page_tokens < KBLK ? page_tokens : KBLK; }
 };
-inline Layout block_layout(int page_tokens, int hd) {
-  Layout l;
-  const int halves = hd / 64;
-  l.box_rows = halves == 1 ? (page_tokens < KBLK ? page_tokens : KBLK) : page_tokens >= KBLK ? KBLK : page_tokens >= 16 ? 16 : 8;
-  l.half_bytes = (uint32_t)l.box_rows * 128;
-  l.box_bytes = l.half_bytes * halves;
-  l.sets = halves == 2 && l.box_rows == 16 ? 2 : 1;
-  l.group_stride = halves == 1 || l.box_rows == KBLK ? 1024 : l.box_bytes;
-  return l;
-}
 
 template <int HD, int QS>
 struct TcSmem {
@@ -222,7 +213,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const void* __restrict__ q,
                     const u16* __restrict__ vcache, const uint32_t* __restrict__ block_table, const int* __restrict__ slot,
                     const int* __restrict__ ctxs, const int* __restrict__ row0s, const uint32_t* __restrict__ mask, void* __restrict__ out, int out_dtype,
-                    Geo g, Layout lay, float scale, Scratch scr, int* __restrict__ status) {
+                    Geo g, float scale, Scratch scr, int* __restrict__ status) {
   using SM = TcSmem<HD, QS>;
   constexpr int NK = SM::NK, NV = SM::NV, NSUB = SM::NSUB, BLK = SM::BLK;
   extern __shared__ uint8_t smem_raw[];
@@ -299,7 +290,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const uint32_t tmem = (uint32_t)flags[0];
   Walk walk{flags[5], flags[6], flags[3], flags[4]};
   const int share = flags[7], total = flags[8];
-  const int group = g.q_heads / g.kv_heads;
+  const int group = g.q_heads / g.kv_heads, gshift = 31 - __clz(group);      // a power of two
   const bool none = walk.item >= walk.end;
   if (threadIdx.x == 0) {      // what the join has to know about the unit that this share begins in
     ShareStart st{0, 0, share, 0, 0, 0, total, 0};
@@ -318,7 +309,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const bool is_v = warp != 0;
     const uint32_t ring = is_v ? v_ring : k_ring;
     const CUtensorMap* map = is_v ? &map_v : &map_k;
-    const int slots = is_v ? NV : NK, boxes = KBLK / lay.box_rows, per = 32 / boxes;
+    const int slots = is_v ? NV : NK, box_rows = Layout<HD>::box_rows(g.page_tokens), boxes = KBLK / box_rows, per = 32 / boxes;
+    const uint32_t box_bytes = (uint32_t)box_rows * HD * 2;
     Piece p;
     int n = 0;      // blocks so far, over all pieces of the share
     bool ok = true;
@@ -330,8 +322,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       // keys are not seen).
       const int len = p.b1 - p.b0;
       auto cache_rows = [&](int batch) -> int {
-        const i64 at = (i64)(p.b0 + batch * per) * KBLK + (i64)lane * lay.box_rows;
-        const int last = (p.w.keys - 1) / lay.box_rows * lay.box_rows, pos = at < last ? (int)at : last;
+        const i64 at = (i64)(p.b0 + batch * per) * KBLK + (i64)lane * box_rows;
+        const int last = (p.w.keys - 1) / box_rows * box_rows, pos = at < last ? (int)at : last;
         const uint32_t page = bt[pos >> g.page_shift];
         return page < (uint64_t)g.num_pages ? (int)(((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) : (int)oob;
       };
@@ -350,7 +342,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (!__all_sync(0xffffffffu, bar_wait(eb, ((n / slots) & 1) ^ 1))) { ok = false; break; }
         if (lane == 0) mbar_expect_tx(fb, BLK);
         __syncwarp();
-        if (lane < boxes) tma_box(ring + s * BLK + (uint32_t)lane * lay.box_bytes, map, fb, row);
+        if (lane < boxes) tma_box(ring + s * BLK + (uint32_t)lane * box_bytes, map, fb, row);
         ++n;
       }
     }
@@ -362,8 +354,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   } else if (warp == 1) {
     // ---------------- MMA: S two blocks ahead, each P V as its team delivers P ----------------
     if (lane == 0) {
-      const uint32_t id_s = lay.sets == 2 ? tc_idesc(KBLK / 2, false) : tc_idesc(KBLK, false);
-      constexpr uint32_t ID_O = tc_idesc(HD, true);
+      constexpr uint32_t ID_S = tc_idesc(KBLK, false), ID_O = tc_idesc(HD, true);
+      using LY = Layout<HD>;
       Piece p;
       int n = 0, pieces = 0;
       int uses[2] = {0, 0};      // P V products of each team so far
@@ -375,14 +367,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (!bar_wait(kfull(s), (i / NK) & 1)) return false;
           tc_fence_after();
           const uint32_t kaddr = k_ring + s * BLK;
-          for (int set = 0; set < lay.sets; ++set)
 #pragma unroll
-            for (int part = 0; part < QS; ++part)
+          for (int part = 0; part < QS; ++part)
 #pragma unroll
-              for (int k = 0; k < HD / 16; ++k)
-                umma_bf16(tmem + (j & 1) * 128 + set * (KBLK / 2), sdesc(q_base + part * BLK + (uint32_t)(k >> 2) * SUB + (uint32_t)(k & 3) * 32u, 16, 1024),
-                          sdesc(kaddr + set * 1024 + (uint32_t)(k >> 2) * lay.half_bytes + (uint32_t)(k & 3) * 32u, 16, lay.group_stride), id_s,
-                          (part > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < HD / 16; ++k)
+              umma_bf16(tmem + (j & 1) * 128, sdesc(q_base + part * BLK + (uint32_t)(k >> 2) * SUB + (uint32_t)(k & 3) * 32u, 16, 1024),
+                        sdesc(kaddr + (uint32_t)(k >> 2) * LY::HALF + (uint32_t)(k & 3) * 32u, 16, LY::GROUP), ID_S, (part > 0 || k > 0) ? 1u : 0u);
           umma_commit(s_full(j & 1));
           umma_commit(kempty(s));
           return true;
@@ -403,10 +393,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           for (int k = 0; k < KBLK / 16; ++k)
 #pragma unroll
             for (int part = 0; part < PS; ++part)
-              mma_ts(o_col, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8,
-                     sdesc(lay.sets == 2 ? vaddr + (uint32_t)(k >> 2) * 1024u + (uint32_t)(k & 3) * 2u * lay.group_stride : vaddr + (uint32_t)k * 2u * lay.group_stride,
-                           lay.half_bytes, lay.group_stride),
-                     ID_O, (j > 1 || k > 0 || part > 0) ? 1u : 0u);
+              mma_ts(o_col, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8, sdesc(vaddr + (uint32_t)k * 2u * LY::GROUP, LY::HALF, LY::GROUP), ID_O,
+                     (j > 1 || k > 0 || part > 0) ? 1u : 0u);
           umma_commit(vempty(s));
           umma_commit(o_done(t));
           if (j + 2 < len) ok = scores(j + 2);
@@ -440,7 +428,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       // ---- the query operand: K-major, 128-byte swizzle
       // (a row is loaded once and stored to every copy; the loads of a batch are in flight together)
       {
-        constexpr int CH = HD / 8, BATCH = 2;      // 16-byte chunks of bf16 a row
+        constexpr int CH = HD / 8, BATCH = 4;      // 16-byte chunks of bf16 a row
         for (int i0 = tid; i0 < crows * CH; i0 += 256 * BATCH) {
           uint4 part[BATCH][QS < 2 ? 2 : QS];
           float4 x[BATCH], y[BATCH];
@@ -451,7 +439,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             part[b][0] = make_uint4(0u, 0u, 0u, 0u);
             if (qr >= live) continue;
             const int ur = p.rowblk * QROWS + qr;
-            const i64 at = (i64)(p.w.t.row0 + ur / group) * g.q_row_stride + ((i64)p.head * group + ur % group) * HD + c * 8;
+            const i64 at = (i64)(p.w.t.row0 + (ur >> gshift)) * g.q_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD + c * 8;
             if (QS == 1) part[b][0] = *reinterpret_cast<const uint4*>(static_cast<const u16*>(q) + at);
             else {
               x[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
@@ -492,7 +480,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (lane == 0) mbar_arrive(q_full);
 
       // ---- the team's key blocks
-      auto mask_of = [&](int row) { return mask + (i64)(p.w.t.row0 + (p.rowblk * QROWS + row) / group) * g.mask_words; };
+      auto mask_of = [&](int row) { return mask + (i64)(p.w.t.row0 + ((p.rowblk * QROWS + row) >> gshift)) * g.mask_words; };
       const uint32_t* own_mask = mask_of(min(r, live - 1));
       const int words = (p.w.t.nodes + 31) >> 5;
       // which of the keys pos .. pos + 31 the row with this mask sees
@@ -521,12 +509,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (block_end > p.w.t.ctx) {
 #pragma unroll
           for (int c = 0; c < W / 32; ++c) {
-            uint32_t bits;
-            if (lay.sets == 2) {      // 32 columns are the first (second) 8 keys of four boxes of 16
-              const int col = copy * W + c * 32, at = (p.b0 + j) * KBLK + (col & 32) * 2 + (col >> 6) * 8;
-              const uint32_t a2 = visible(own_mask, at), b2 = visible(own_mask, at + 32);
-              bits = (a2 & 0xffu) | (a2 >> 8 & 0xff00u) | (b2 & 0xffu) << 16 | (b2 << 8 & 0xff000000u);
-            } else bits = visible(own_mask, pos + c * 32);
+            const uint32_t bits = visible(own_mask, pos + c * 32);
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[c * 32 + e] = (bits >> e) & 1u ? s[c * 32 + e] : -INFINITY;
           }
@@ -594,7 +577,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if ((p.b0 + j + 1) * KBLK > p.w.t.ctx) {
           const int i = n + j, sl = i % NV, row = quarter * 32 + lane;
           wait(vfull(sl), (i / NV) & 1);
-          const uint32_t vrow = v_ring + sl * BLK + (uint32_t)(row / lay.box_rows) * lay.box_bytes + (uint32_t)(row & (lay.box_rows - 1)) * 128u;
+          const uint32_t vrow = v_ring + sl * BLK + (uint32_t)(row >> 3) * Layout<HD>::GROUP + (uint32_t)(row & 7) * 128u;
           bool hit = false;
 #pragma unroll
           for (int h = 0; h < 2 * NSUB; ++h) {
@@ -603,7 +586,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             for (int c = 0; c < 4; ++c)
               asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                            : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3])
-                           : "r"(vrow + (h >> 1) * lay.half_bytes + (uint32_t)((((h & 1) * 4 + c) ^ (row & 7)) << 4)));
+                           : "r"(vrow + (h >> 1) * Layout<HD>::HALF + (uint32_t)((((h & 1) * 4 + c) ^ (row & 7)) << 4)));
 #pragma unroll
             for (int c = 0; c < 4; ++c)
               if (not_finite2(w[c][0]) | not_finite2(w[c][1]) | not_finite2(w[c][2]) | not_finite2(w[c][3])) {
@@ -613,7 +596,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                   const uint32_t bad = not_finite2(w[c][e]);
                   w[c][e] &= ((bad & 0x8000u) ? 0u : 0xffffu) | ((bad & 0x80000000u) ? 0u : 0xffff0000u);
                 }
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(vrow + (h >> 1) * lay.half_bytes + (uint32_t)((((h & 1) * 4 + c) ^ (row & 7)) << 4)),
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(vrow + (h >> 1) * Layout<HD>::HALF + (uint32_t)((((h & 1) * 4 + c) ^ (row & 7)) << 4)),
                              "r"(w[c][0]), "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3])
                              : "memory");
               }
@@ -696,7 +679,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
           if (whole) {
             const int ur = p.rowblk * QROWS + row;
-            const i64 at = (i64)(p.w.t.row0 + ur / group) * g.out_row_stride + ((i64)p.head * group + ur % group) * HD + c0 + c4 * 4;
+            const i64 at = (i64)(p.w.t.row0 + (ur >> gshift)) * g.out_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD + c0 + c4 * 4;
             if (out_dtype == 0) *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
             else *reinterpret_cast<uint2*>(static_cast<u16*>(out) + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
           } else *reinterpret_cast<float4*>(scr.o + ((i64)piece * scr.rows + row) * HD + c0 + c4 * 4) = v;
@@ -772,12 +755,12 @@ inline int cache_map(CUtensorMap* map, const void* cache, i64 rows, i64 head_dim
 template <int HD, int QS, int PS>
 int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt, const int* slot, const int* ctx, const int* row0, const uint32_t* mask,
               void* out, int out_dtype, const Geo& g, float scale, void* scratch, cudaStream_t st) {
-  const Layout lay = block_layout(g.page_tokens, HD);
+  const int box_rows = Layout<HD>::box_rows(g.page_tokens);
   const i64 cache_rows = g.num_pages * g.kv_heads * g.page_tokens;
   CUtensorMap mk, mv;
-  int rc = cache_map(&mk, kc, cache_rows, HD, lay.box_rows);
+  int rc = cache_map(&mk, kc, cache_rows, HD, box_rows);
   if (rc) return rc;
-  rc = cache_map(&mv, vc, cache_rows, HD, lay.box_rows);
+  rc = cache_map(&mv, vc, cache_rows, HD, box_rows);
   if (rc) return rc;
   int* status = gemm_status_word();
   if (!status) return (int)cudaErrorMemoryAllocation;
@@ -793,7 +776,7 @@ int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt,
   const int group = g.q_heads / g.kv_heads;
   const Scratch scr = carve(scratch, g.max_nodes, group);
   cudaError_t e = launch_pdl(kern, WKB_SM_COUNT, TC_THREADS, (size_t)TcSmem<HD, QS>::BYTES, st, mk, mv, q, (const u16*)vc, bt, slot, ctx, row0, mask, out,
-                             out_dtype, g, lay, scale, scr, status);
+                             out_dtype, g, scale, scr, status);
   if (e != cudaSuccess) return (int)e;
   const int rows_per = 256 / (HD / 4);
   return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(WKB_SM_COUNT - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, slot, ctx, row0, out,
