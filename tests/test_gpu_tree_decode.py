@@ -555,6 +555,43 @@ def test_kv_commit_refuses_bad_paths(dev):
     assert dev.gemm_status() == 31 and torch.equal(kv.k, before)
 
 
+# ---- refusals of the wrappers ---------------------------------------------------------------------------------------
+
+def test_wrappers_refuse_wrong_tensors(dev):
+    import torch
+    z = lambda *s, dt=torch.int32: torch.zeros(s, dtype=dt, device="cuda")
+    f, h = torch.float32, torch.float16
+    kv = dev.PagedKV(2, 4, 2, 64)
+    ok = dict(q=z(3, 256, dt=f), q_row_stride=256, kv=kv, layer=1, block_table=z(1, 4), tree_slot=z(1), tree_ctx=z(1), tree_row0=z(2), tree_mask=z(3, 1),
+              out=z(3, 256, dt=f), q_heads=4, mbps=4, max_nodes=3, scale=1.0, scratch=dev.paged_attn_tree_scratch(3, 4, 2, 64))
+    dev.paged_attn_tree(**ok)
+    for bad in [dict(q=z(3, 256, dt=h)), dict(out=z(3, 256, dt=h)), dict(q=z(2, 256, dt=f)), dict(q=z(3, 256, dt=f).cpu()), dict(layer=2), dict(layer=-1), dict(tree_ctx=z(2)),
+                dict(tree_row0=z(3)), dict(tree_slot=z(1, dt=torch.int64)), dict(tree_mask=z(2, 1)), dict(tree_mask=z(3)), dict(out=z(3, 128, dt=f)), dict(out=z(256, 3, dt=f).t()),
+                dict(mbps=3), dict(mbps=0), dict(block_table=z(1, 4, dt=torch.int64)), dict(scratch=z(64)), dict(kv=dev.PagedKVInt8(2, 4, 2, 64))]:
+        with pytest.raises(ValueError):
+            dev.paged_attn_tree(**{**ok, **bad})
+    from wukong_b200._lib import WukongB200Error
+    for bad in [dict(max_nodes=0), dict(max_nodes=33), dict(q_heads=3), dict(scratch=z(64, dt=torch.uint8))]:
+        with pytest.raises(WukongB200Error):
+            dev.paged_attn_tree(**{**ok, **bad})
+    for bad in [(z(2, 8, dt=h), None), (z(2, 8, dt=f), z(3, dt=f)), (z(2, 8, dt=f), z(2, dt=h)), (z(8, 2, dt=f).t(), None)]:
+        with pytest.raises(ValueError):
+            dev.token_probs(*bad)
+    with pytest.raises(ValueError):
+        dev.token_probs(z(2, 8, dt=f), out=z(2, 9, dt=f))
+    ok = dict(probs=z(4, 8, dt=f), draft=z(4, 8, dt=f), token=z(4), parent=z(4), tree_row0=z(2), u_node=z(4, dt=f), u_final=z(1, dt=f), max_nodes=4, max_path=4)
+    dev.tree_verify(**ok)
+    for bad in [dict(draft=z(4, 9, dt=f)), dict(probs=z(4, 8, dt=h)), dict(token=z(5)), dict(parent=z(3)), dict(u_node=z(3, dt=f)), dict(u_final=z(2, dt=f)),
+                dict(tree_row0=z(2, dt=torch.int64)), dict(out=(z(1, 3), z(1), z(1, 4)))]:
+        with pytest.raises(ValueError):
+            dev.tree_verify(**{**ok, **bad})
+    ok = dict(kv=kv, block_table=z(1, 4), tree_slot=z(1), tree_ctx=z(1), path=z(1, 3), n_path=z(1), mbps=4)
+    dev.paged_kv_commit(**ok)
+    for bad in [dict(path=z(2, 3)), dict(path=z(3)), dict(n_path=z(2)), dict(new_ctx=z(2)), dict(kv=dev.PagedKVInt8(2, 4, 2, 64)), dict(mbps=5)]:
+        with pytest.raises(ValueError):
+            dev.paged_kv_commit(**{**ok, **bad})
+
+
 # ---- together -------------------------------------------------------------------------------------------------------
 
 def test_speculative_generation_equals_plain_greedy(dev):

@@ -24,7 +24,6 @@
 #pragma once
 #include "common.cuh"
 #include "tc_common.cuh"
-#include <type_traits>
 
 namespace wkb {
 int* gemm_status_word();
@@ -77,8 +76,7 @@ template <int HD, int QS>
 struct TcSmem {
   static constexpr int NSUB = HD / 64, BLK = NSUB * SUB;                 // bytes of 128 rows of an operand
   static constexpr int HEADER = 3072;                                    // barriers, (m, l) of the teams, flags
-  static constexpr int Q_BYTES = QS * BLK < 32768 ? 32768 : QS * BLK;    // also the 256 x CW f32 of the epilogue
-  static constexpr int CW = Q_BYTES >= 65536 ? 64 : 32;
+  static constexpr int Q_BYTES = QS * BLK < 32768 ? 32768 : QS * BLK;    // also the 128 x 64 f32 of the epilogue
   static constexpr int SLOTS = (232448 - HEADER - Q_BYTES) / BLK > 12 ? 12 : (232448 - HEADER - Q_BYTES) / BLK;
   static constexpr int NK = (SLOTS + 1) / 2, NV = SLOTS / 2;
   static constexpr int BYTES = HEADER + Q_BYTES + SLOTS * BLK;
@@ -292,7 +290,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const int share = flags[7], total = flags[8];
   const int group = g.q_heads / g.kv_heads, gshift = 31 - __clz(group);      // a power of two
   const bool none = walk.item >= walk.end;
-  if (threadIdx.x == 0) {      // what the join has to know about the unit that this share begins in
+  if (threadIdx.x == 320) {      // (of the warp without a part) what the join has to know about the unit that this share begins in
     ShareStart st{0, 0, share, 0, 0, 0, total, 0};
     if (!none) {
       Walk w = walk;
@@ -498,26 +496,32 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         return bits & low_bits((i64)p.w.keys - pos);
       };
       float m = -INFINITY, l = 0.0f;      // m in base 2, the maximum in use
-      auto block = [&](auto width_c, int j) {
-        constexpr int W = decltype(width_c)::value;
-        const int pos = (p.b0 + j) * KBLK + copy * W;
-        const int block_end = (p.b0 + j + 1) * KBLK;
-        float s[W];
+      // One block, 32 columns at a time in rolled loops: the kernel is short enough that first executions of unrolled code
+      // (instruction fetches) took longer than the work.  The last columns of the first pass stay in registers.
+      const int chunks = 4 / copies, col0 = copy * chunks * 32;
+      auto block = [&](int j) {
+        const int pos0 = (p.b0 + j) * KBLK + col0;
+        const bool masked = (p.b0 + j + 1) * KBLK > p.w.t.ctx;
+        float s[32];
+        auto load = [&](int c) {
+          tm_ld32(s_col + col0 + c * 32, reinterpret_cast<uint32_t*>(s));
+          tm_ld_wait();
+          if (masked) {
+            const uint32_t bits = visible(own_mask, pos0 + c * 32);
 #pragma unroll
-        for (int c = 0; c < W / 32; ++c) tm_ld32(s_col + copy * W + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
-        tm_ld_wait();
-        if (block_end > p.w.t.ctx) {
-#pragma unroll
-          for (int c = 0; c < W / 32; ++c) {
-            const uint32_t bits = visible(own_mask, pos + c * 32);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) s[c * 32 + e] = (bits >> e) & 1u ? s[c * 32 + e] : -INFINITY;
+            for (int e = 0; e < 32; ++e) s[e] = (bits >> e) & 1u ? s[e] : -INFINITY;
           }
-        }
-        float b4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        };
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < chunks; ++c) {
+          load(c);
+          float b4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int e = 0; e < W; ++e) b4[e & 3] = fmaxf(b4[e & 3], s[e]);
-        const float top = fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3])) * sc;
+          for (int e = 4; e < 32; ++e) b4[e & 3] = fmaxf(b4[e & 3], s[e]);
+          top = fmaxf(top, fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3])));
+        }
+        top *= sc;
         const bool move = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
         if (__any_sync(0xffffffffu, move)) {
           const float next = move ? top : m;
@@ -539,69 +543,66 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           m = next;
         }
         const float m_use = m == -INFINITY ? 0.0f : m;
-        float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int c = 0; c < W / 32; ++c) {
+#pragma unroll 1
+        for (int c = chunks - 1;; ) {
+          float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float p0 = ex2(ffma(s[c * 32 + e], sc, -m_use)), p1 = ex2(ffma(s[c * 32 + e + 1], sc, -m_use));
+            const float p0 = ex2(ffma(s[e], sc, -m_use)), p1 = ex2(ffma(s[e + 1], sc, -m_use));
             l4[(e >> 1) & 1] += p0;
             l4[2 + ((e >> 1) & 1)] += p1;
             pk[e >> 1] = pack_bf16(p0, p1);
             if (PS == 2) pk[16 + (e >> 1)] = pack_bf16(p0 - u2f(pk[e >> 1] << 16), p1 - u2f(pk[e >> 1] & 0xffff0000u));
           }
-          if (PS == 2) tm_st32(s_col + copy * W + c * 32, pk);
-          else tm_st16(s_col + copy * W + c * 32, pk);
+          if (PS == 2) tm_st32(s_col + col0 + c * 32, pk);
+          else tm_st16(s_col + col0 + c * 32, pk);
+          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          if (--c < 0) break;
+          load(c);
         }
-        if (W < KBLK) {      // the other copies' keys
+        if (copies > 1) {      // zeros for the other copies' keys
           uint32_t zero[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) zero[e] = 0u;
-#pragma unroll
-          for (int c = 0; c < KBLK / 32; ++c)
-            if (c / (W / 32) != copy) {
-              if (PS == 2) tm_st32(s_col + c * 32, zero);
-              else tm_st16(s_col + c * 32, zero);
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32)
+            if (c < col0 || c >= col0 + chunks * 32) {
+              if (PS == 2) tm_st32(s_col + c, zero);
+              else tm_st16(s_col + c, zero);
             }
         }
-        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
       };
       for (int j = team; j < len; j += 2) {
         wait(s_full(team), uses & 1);
         tc_fence_after();
-        if (copies == 4) block(std::integral_constant<int, 32>(), j);
-        else if (copies == 2) block(std::integral_constant<int, 64>(), j);
-        else block(std::integral_constant<int, 128>(), j);
+        block(j);
         // V of keys that some row does not see
         if ((p.b0 + j + 1) * KBLK > p.w.t.ctx) {
           const int i = n + j, sl = i % NV, row = quarter * 32 + lane;
           wait(vfull(sl), (i / NV) & 1);
           const uint32_t vrow = v_ring + sl * BLK + (uint32_t)(row >> 3) * Layout<HD>::GROUP + (uint32_t)(row & 7) * 128u;
-          bool hit = false;
+          auto piece_at = [&](int k) { return vrow + (uint32_t)(k >> 3) * Layout<HD>::HALF + (uint32_t)(((k & 7) ^ (row & 7)) << 4); };
+          uint32_t bad = 0u;
+#pragma unroll 1
+          for (int k = 0; k < 8 * NSUB; k += 8) {
+            uint32_t w[8][4];
 #pragma unroll
-          for (int h = 0; h < 2 * NSUB; ++h) {
-            uint32_t w[4][4];
+            for (int c = 0; c < 8; ++c)
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3]) : "r"(piece_at(k + c)));
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3])
-                           : "r"(vrow + (h >> 1) * Layout<HD>::HALF + (uint32_t)((((h & 1) * 4 + c) ^ (row & 7)) << 4)));
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (not_finite2(w[c][0]) | not_finite2(w[c][1]) | not_finite2(w[c][2]) | not_finite2(w[c][3])) {
-                hit = true;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const uint32_t bad = not_finite2(w[c][e]);
-                  w[c][e] &= ((bad & 0x8000u) ? 0u : 0xffffu) | ((bad & 0x80000000u) ? 0u : 0xffff0000u);
-                }
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(vrow + (h >> 1) * Layout<HD>::HALF + (uint32_t)((((h & 1) * 4 + c) ^ (row & 7)) << 4)),
-                             "r"(w[c][0]), "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3])
-                             : "memory");
-              }
+            for (int c = 0; c < 8; ++c) bad |= not_finite2(w[c][0]) | not_finite2(w[c][1]) | not_finite2(w[c][2]) | not_finite2(w[c][3]);
           }
-          if (hit) {
+          if (bad) {
+#pragma unroll 1
+            for (int k = 0; k < 32 * NSUB; ++k) {
+              const uint32_t at = piece_at(k >> 2) + (uint32_t)(k & 3) * 4u;
+              uint32_t w;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+              const uint32_t b = not_finite2(w);
+              w &= ((b & 0x8000u) ? 0u : 0xffffu) | ((b & 0x80000000u) ? 0u : 0xffff0000u);
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+            }
             if ((p.b0 + j) * KBLK + row < p.w.keys) flags[2] = 1;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
@@ -614,80 +615,115 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       n += len;
 
-      // ---- add up the teams and the copies, CW columns at a time through the query operand's memory
-      constexpr int CW = SM::CW;
-      const bool mine = team < len;      // this team had a block
-      if (mine) { wait(o_done(team), (uses - 1) & 1); tc_fence_after(); }
-      ml_s[team * QROWS + a] = make_float2(mine ? m : -INFINITY, mine ? l : 0.0f);
+      // ---- the result: the teams' accumulators lie in the same lanes and are added in registers; the copies lie in other
+      // lanes and are added through the query operand's memory, 64 columns at a time
+      if (team < len) wait(o_done(team), (uses - 1) & 1);
+      ml_s[team * QROWS + a] = make_float2(team < len ? m : -INFINITY, team < len ? l : 0.0f);
+      tc_fence_before();
       teams_sync();
-      const int teams = min(len, 2), parts = teams * copies;      // part i of a row: ml_s[i * crows + row] (copies of team 0, then of team 1)
+      tc_fence_after();
+      const bool both = len > 1;      // team 1 had a block
       float m_all = -INFINITY, l_all = 0.0f;
-      for (int i = 0; i < parts; ++i) m_all = fmaxf(m_all, ml_s[i * crows + r].x);
+#pragma unroll 1
+      for (int i = r; i < (both ? 2 : 1) * QROWS; i += crows) m_all = fmaxf(m_all, ml_s[i].x);      // copies of team 0, then of team 1
       const float m_use = m_all == -INFINITY ? 0.0f : m_all;
-      for (int i = 0; i < parts; ++i) {
-        const float2 v = ml_s[i * crows + r];
+#pragma unroll 1
+      for (int i = r; i < (both ? 2 : 1) * QROWS; i += crows) {
+        const float2 v = ml_s[i];
         l_all += v.y * ex2(v.x - m_use);
       }
       const bool whole = len == p.w.blocks, fine = flags[1] == 0, bad_v = flags[2] != 0;
-      float w_mine = ex2(m - m_use);
-      if (whole) w_mine *= l_all != 0.0f ? 1.0f / l_all : 0.0f;      // a unit in one piece is normalised here
+      const float inv = !whole ? 1.0f : l_all != 0.0f ? 1.0f / l_all : 0.0f;      // a unit in one piece is normalised here
+      const float w0 = ex2(ml_s[a].x - m_use) * inv, w1 = both ? ex2(ml_s[QROWS + a].x - m_use) * inv : 0.0f;
       // a share's piece that begins the share is its even one; a later one that it does not finish is its odd one
       const int piece = p.unit_start + p.b0 == (int)blockIdx.x * share ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
       if (!whole && fine && team == 0 && copy == 0 && r < live) scr.ml[(i64)piece * scr.rows + r] = make_float2(m_all, l_all);
+      // rare: V holds a NaN or an infinity that this row may see.  Its sum over those elements is then the result
+      auto bad_columns = [&](int row, int col, float4& v) {
+        const uint32_t* mrow = mask_of(row);
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-      for (int c0 = 0; c0 < HD; c0 += CW) {
-        if (mine) {
+        for (int pos = p.b0 * KBLK; pos < min(p.b1 * KBLK, p.w.keys); ++pos) {
+          if (!(visible(mrow, pos) & 1u)) continue;
+          const uint32_t page = block_table[(i64)p.w.t.slot * g.mbps + (pos >> g.page_shift)];
+          if (page >= (uint64_t)g.num_pages) continue;
+          const u16* vp = vcache + (((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) * HD + col;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((vp[e] & 0x7f80u) == 0x7f80u) x[e] += bf16_bits_to_f32(vp[e]);
+        }
+        v.x = x[0] != 0.0f ? x[0] : v.x; v.y = x[1] != 0.0f ? x[1] : v.y;      // untouched where there was none
+        v.z = x[2] != 0.0f ? x[2] : v.z; v.w = x[3] != 0.0f ? x[3] : v.w;
+      };
+      const bool staged = copies > 1 || bad_v;
+      auto out_at = [&](int row) {      // of column 0
+        const int ur = p.rowblk * QROWS + row;
+        return whole ? (i64)(p.w.t.row0 + (ur >> gshift)) * g.out_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD
+                     : ((i64)piece * scr.rows + row) * HD;
+      };
+      auto put = [&](i64 at, const float4& v) {
+        if (!whole) *reinterpret_cast<float4*>(scr.o + at) = v;
+        else if (out_dtype == 0) *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
+        else *reinterpret_cast<uint2*>(static_cast<u16*>(out) + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+      };
 #pragma unroll 1
-          for (int c1 = 0; c1 < CW; c1 += 32) {
-            uint32_t o[32];
-            tm_ld32(o_col + c0 + c1, o);
+      for (int c0 = 0; c0 < HD; c0 += 64) {
+        {
+          const int col = c0 + team * 32;
+          uint32_t o[32];
+          tm_ld32(lane_base + 256 + col, o);
+          if (both) {
+            uint32_t o1[32];
+            tm_ld32(lane_base + 256 + HD + col, o1);
             tm_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = f2u(u2f(o[e]) * w_mine);
-            float4* d = reinterpret_cast<float4*>(stage + (team * QROWS + a) * CW + c1);
+            for (int e = 0; e < 32; ++e) o[e] = f2u(ffma(u2f(o1[e]), w1, u2f(o[e]) * w0));
+          } else {
+            tm_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = f2u(u2f(o[e]) * w0);
+          }
+          if (staged) {
+            float4* d = reinterpret_cast<float4*>(stage + a * 64 + team * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[e ^ (a & 7)] = make_float4(u2f(o[4 * e]), u2f(o[4 * e + 1]), u2f(o[4 * e + 2]), u2f(o[4 * e + 3]));
-          }
-        }
-        teams_sync();
-        constexpr int C4 = CW / 4;
-        for (int idx = tid; idx < live * C4; idx += 256) {
-          const int row = idx / C4, c4 = idx % C4;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int i = 0; i < parts; ++i) {
-            const int x = i * crows + row;
-            const float4 s4 = *reinterpret_cast<const float4*>(stage + x * CW + ((c4 ^ (x & 7)) << 2));
-            v.x += s4.x; v.y += s4.y; v.z += s4.z; v.w += s4.w;
-          }
-          if (!fine) continue;
-          // rare: V holds a NaN or an infinity that this row may see.  Its sum over those elements is then the result
-          if (bad_v || (copies > 1 && !(fabsf(v.x) <= 3.402823466e+38f && fabsf(v.y) <= 3.402823466e+38f && fabsf(v.z) <= 3.402823466e+38f &&
-                                        fabsf(v.w) <= 3.402823466e+38f))) {
-            const uint32_t* mrow = mask_of(row);
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int pos = p.b0 * KBLK; pos < min(p.b1 * KBLK, p.w.keys); ++pos) {
-              if (!(visible(mrow, pos) & 1u)) continue;
-              const uint32_t page = block_table[(i64)p.w.t.slot * g.mbps + (pos >> g.page_shift)];
-              if (page >= (uint64_t)g.num_pages) continue;
-              const u16* vp = vcache + (((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) * HD + c0 + c4 * 4;
+          } else if (r < live && fine) {
+            const i64 at = out_at(r) + col;
+            if (whole && out_dtype == 1) {
+              uint4* d = reinterpret_cast<uint4*>(static_cast<u16*>(out) + at);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if ((vp[e] & 0x7f80u) == 0x7f80u) x[e] += bf16_bits_to_f32(vp[e]);
+                d[e] = make_uint4(pack_bf16(u2f(o[8 * e]), u2f(o[8 * e + 1])), pack_bf16(u2f(o[8 * e + 2]), u2f(o[8 * e + 3])),
+                                  pack_bf16(u2f(o[8 * e + 4]), u2f(o[8 * e + 5])), pack_bf16(u2f(o[8 * e + 6]), u2f(o[8 * e + 7])));
+            } else {
+              float4* d = reinterpret_cast<float4*>((whole ? static_cast<float*>(out) : scr.o) + at);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) d[e] = make_float4(u2f(o[4 * e]), u2f(o[4 * e + 1]), u2f(o[4 * e + 2]), u2f(o[4 * e + 3]));
             }
-            v.x = x[0] != 0.0f ? x[0] : v.x; v.y = x[1] != 0.0f ? x[1] : v.y;      // untouched where there was none
-            v.z = x[2] != 0.0f ? x[2] : v.z; v.w = x[3] != 0.0f ? x[3] : v.w;
           }
-          if (whole) {
-            const int ur = p.rowblk * QROWS + row;
-            const i64 at = (i64)(p.w.t.row0 + (ur >> gshift)) * g.out_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD + c0 + c4 * 4;
-            if (out_dtype == 0) *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
-            else *reinterpret_cast<uint2*>(static_cast<u16*>(out) + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-          } else *reinterpret_cast<float4*>(scr.o + ((i64)piece * scr.rows + row) * HD + c0 + c4 * 4) = v;
+        }
+        if (!staged) continue;
+        teams_sync();
+        const int c4 = tid & 15;
+#pragma unroll 1
+        for (int row = tid >> 4; row < live; row += 16) {
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+          for (int x = row; x < QROWS; x += crows) {
+            const float4 s4 = *reinterpret_cast<const float4*>(stage + x * 64 + ((c4 ^ (x & 7)) << 2));
+            v.x += s4.x; v.y += s4.y; v.z += s4.z; v.w += s4.w;
+          }
+          if (bad_v || !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) <= 3.402823466e+38f)) bad_columns(row, c0 + c4 * 4, v);
+          if (fine) put(out_at(row) + c0 + c4 * 4, v);
         }
         teams_sync();
       }
-      if (tid == 0) flags[2] = 0;
-      teams_sync();
+      if (bad_v) {
+        teams_sync();
+        if (tid == 0) flags[2] = 0;
+      }
+      tc_fence_before();
+      teams_sync();      // the accumulators, the operand's memory and ml_s are free
     }
   }
   tc_fence_before();

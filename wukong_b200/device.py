@@ -249,6 +249,14 @@ def paged_attn_decode_int8(q, q_row_stride, kv, layer, block_table, row_slot, ro
 
 # ---- speculative decoding: a tree of drafted tokens is checked in one step --------------------------------------------
 
+_TREE_DT = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _raw_stream(dev):
+    """The current stream of device `dev` as an address, without building a torch.cuda.Stream."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 def tree_layout(parent, row0):
     """Host helper: for trees given as each row's parent within its tree (numpy, < the node's own index; the root's entry is
     not read) and first rows row0 [n + 1], the attention masks (int32 [rows, words]: itself and its ancestors) and each
@@ -270,22 +278,44 @@ def tree_layout(parent, row0):
     return mask.view(np.int32), depth
 
 
-def _same_device(*tensors):
-    cur = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != cur):
-            raise ValueError("every tensor must lie on the current CUDA device")
+# A decode step makes these calls once a layer or once a step, often eagerly, so the checks are kept to what a wrong call
+# would otherwise turn into a fault: types, extents, strides and the device.
+
+def _here(t):
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise ValueError("every tensor must lie on the current CUDA device")
+    return dev
 
 
-def _vec(t, n, dtype, what):
-    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
-        raise ValueError("%s must be a contiguous %s tensor of %d values" % (what, dtype, n))
+def _on(dev, t, n, dtype, what):
+    """A contiguous tensor of n values on device `dev`."""
+    if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous %s tensor of %d values on the current CUDA device" % (what, dtype, n))
+    return t.data_ptr()
 
 
-def _row_pitch(t, cols, what):
-    if t.dim() != 2 or t.shape[1] < cols or t.stride(1) != 1:
-        raise ValueError("%s must be a matrix of at least %d columns with unit column stride" % (what, cols))
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _matrix(dev, t, cols, what):
+    """(address, row pitch) of a matrix on device `dev` whose rows hold `cols` values."""
+    if t.dim() != 2 or t.shape[1] < cols or t.stride(1) != 1 or t.get_device() != dev:
+        raise ValueError("%s must be a matrix of at least %d columns with unit column stride on the current CUDA device" % (what, cols))
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _table(dev, t, mbps):
+    if t.dtype is not torch.int32 or mbps < 1 or t.numel() % mbps or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError("block_table must be a contiguous int32 [slots, mbps] on the current CUDA device")
+    return t.data_ptr()
+
+
+def _slabs(dev, kv):
+    k, v = kv.k, kv.v
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.get_device() != dev or v.get_device() != dev or \
+            not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError("the cache must be contiguous bf16 on the current CUDA device")
+    if k.shape != (kv.layers, kv.num_pages, kv.kv_heads, kv.page_tokens, kv.head_dim) or v.shape != k.shape:
+        raise ValueError("the cache must be [layers, pages, kv_heads, page_tokens, head_dim]")
+    return k.data_ptr(), v.data_ptr(), k.stride(0)
 
 
 def paged_attn_tree_scratch(max_nodes, q_heads, kv_heads, head_dim, device="cuda"):
@@ -295,80 +325,80 @@ def paged_attn_tree_scratch(max_nodes, q_heads, kv_heads, head_dim, device="cuda
 def paged_attn_tree(q, q_row_stride, kv, layer, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, q_heads, mbps, max_nodes, scale, scratch):
     """Attention of the nodes of draft trees over the paged bf16 cache (wkb_paged_attn_tree): row r = node i of tree t sees
     the tree_ctx[t] committed tokens and the nodes that its mask names.  q f32 or bf16, out f32 or bf16 [rows, q_heads * head_dim]."""
-    rows, n = out.shape[0], tree_slot.numel()
-    _same_device(q, kv.k, kv.v, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, scratch)
-    _vec(tree_slot, n, torch.int32, "tree_slot"); _vec(tree_ctx, n, torch.int32, "tree_ctx"); _vec(tree_row0, n + 1, torch.int32, "tree_row0")
-    if tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] < rows or not tree_mask.is_contiguous():
-        raise ValueError("tree_mask must be a contiguous int32 [rows, words]")
-    if q.dtype not in (torch.float32, torch.bfloat16) or out.dtype not in (torch.float32, torch.bfloat16) or kv.k.dtype != torch.bfloat16:
-        raise ValueError("q and out are f32 or bf16, the cache is bf16")
-    if out.dim() != 2 or out.shape[1] < q_heads * kv.head_dim or out.stride(1) != 1:
-        raise ValueError("out must be [rows, q_heads * head_dim] with unit column stride")
-    if rows and q.storage_offset() + (rows - 1) * q_row_stride + q_heads * kv.head_dim > q.untyped_storage().nbytes() // q.element_size():
-        raise ValueError("q does not hold %d rows of pitch %d" % (rows, q_row_stride))
-    if block_table.dtype != torch.int32 or not block_table.is_contiguous() or block_table.numel() % mbps:
-        raise ValueError("block_table must be a contiguous int32 [slots, mbps]")
-    check(lib().wkb_paged_attn_tree(_p(q), _DT[q.dtype], q_row_stride, _p(kv.k[layer]), _p(kv.v[layer]), kv.num_pages, _p(block_table), _p(tree_slot),
-                                    _p(tree_ctx), _p(tree_row0), _p(tree_mask), tree_mask.shape[1], _p(out), _DT[out.dtype], out.stride(0), rows, n,
-                                    max_nodes, q_heads, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps, scale, _p(scratch), scratch.numel(), _s()),
-          "wkb_paged_attn_tree")
+    dev, n, rows, width = _here(out), tree_slot.numel(), out.shape[0], q_heads * kv.head_dim
+    tq, to = _TREE_DT.get(q.dtype), _TREE_DT.get(out.dtype)
+    if tq is None or to is None:
+        raise ValueError("q and out are f32 or bf16")
+    k, v, layer_stride = _slabs(dev, kv)
+    if not 0 <= layer < kv.layers:
+        raise ValueError("no such layer")
+    if q.get_device() != dev or (rows and (q.storage_offset() + (rows - 1) * q_row_stride + width) * q.element_size() > q.untyped_storage().nbytes()):
+        raise ValueError("q must hold %d rows of pitch %d on the current CUDA device" % (rows, q_row_stride))
+    words = tree_mask.shape[1] if tree_mask.dim() == 2 else 0
+    if tree_mask.shape[0] < rows:
+        raise ValueError("tree_mask must have a row for each row of out")
+    po, ldo = _matrix(dev, out, width, "out")
+    at = layer * layer_stride * 2
+    check(lib().wkb_paged_attn_tree(q.data_ptr(), tq, q_row_stride, k + at, v + at, kv.num_pages, _table(dev, block_table, mbps),
+                                    _on(dev, tree_slot, n, torch.int32, "tree_slot"), _on(dev, tree_ctx, n, torch.int32, "tree_ctx"),
+                                    _on(dev, tree_row0, n + 1, torch.int32, "tree_row0"),
+                                    _on(dev, tree_mask, tree_mask.shape[0] * words, torch.int32, "tree_mask"), words, po, to, ldo, rows, n, max_nodes,
+                                    q_heads, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps, scale,
+                                    _on(dev, scratch, scratch.numel(), torch.uint8, "scratch"), scratch.numel(), _raw_stream(dev)), "wkb_paged_attn_tree")
     return out
 
 
 def token_probs(logits, temperature=None, out=None):
     """f32 probabilities softmax(logits / temperature) of vocabulary rows; a temperature of 0 gives the greedy one-hot row
     (wkb_token_probs).  logits f32 or bf16 [rows, cols] (any row pitch), temperature f32 [rows]."""
+    dev = _here(logits)
     rows, cols = logits.shape
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    dt = _TREE_DT.get(logits.dtype)
+    if dt is None:
         raise ValueError("logits are f32 or bf16")
-    if temperature is not None:
-        _vec(temperature, rows, torch.float32, "temperature")
+    px, ld = _matrix(dev, logits, cols, "logits")
     if out is None:
         out = torch.empty((rows, cols), dtype=torch.float32, device=logits.device)
-    if out.dtype != torch.float32 or out.shape != logits.shape:
+    if out.dtype is not torch.float32 or out.shape != logits.shape:
         raise ValueError("out must be f32 of the logits' shape")
-    _same_device(logits, temperature, out)
-    check(lib().wkb_token_probs(_p(logits), _DT[logits.dtype], _row_pitch(logits, cols, "logits"), _p(temperature), _p(out), _row_pitch(out, cols, "out"),
-                                rows, cols, _s()), "wkb_token_probs")
+    po, ldo = _matrix(dev, out, cols, "out")
+    check(lib().wkb_token_probs(px, dt, ld, None if temperature is None else _on(dev, temperature, rows, torch.float32, "temperature"), po, ldo, rows, cols,
+                                _raw_stream(dev)), "wkb_token_probs")
     return out
 
 
 def tree_verify(probs, draft, token, parent, tree_row0, u_node, u_final, max_nodes, max_path, out=None):
     """Accept / reject the drafted tokens of each tree and draw the token that follows (wkb_tree_verify).  probs, draft (or
     None): f32 [rows, vocabulary].  Returns (path int32 [n, max_path], n_path int32 [n], tokens int32 [n, max_path])."""
+    dev = _here(probs)
     rows, cols = probs.shape
     n = tree_row0.numel() - 1
-    if probs.dtype != torch.float32 or (draft is not None and (draft.dtype != torch.float32 or draft.shape != probs.shape)):
+    if probs.dtype is not torch.float32 or (draft is not None and (draft.dtype is not torch.float32 or draft.shape != probs.shape)):
         raise ValueError("probs and draft must be f32 of one shape")
-    _vec(token, rows, torch.int32, "token"); _vec(parent, rows, torch.int32, "parent"); _vec(tree_row0, n + 1, torch.int32, "tree_row0")
-    _vec(u_node, rows, torch.float32, "u_node"); _vec(u_final, n, torch.float32, "u_final")
+    pp, ldp = _matrix(dev, probs, cols, "probs")
+    pd, ldq = (None, 0) if draft is None else _matrix(dev, draft, cols, "draft")
     if out is None:
         buf = torch.empty(n * (2 * max_path + 1), dtype=torch.int32, device=probs.device)
         out = buf[:n * max_path].view(n, max_path), buf[2 * n * max_path:], buf[n * max_path:2 * n * max_path].view(n, max_path)
     path, n_path, tokens = out
-    _vec(path, n * max_path, torch.int32, "path"); _vec(tokens, n * max_path, torch.int32, "tokens"); _vec(n_path, n, torch.int32, "n_path")
-    _same_device(probs, draft, token, parent, tree_row0, u_node, u_final, path, n_path, tokens)
-    check(lib().wkb_tree_verify(_p(probs), _row_pitch(probs, cols, "probs"), _p(draft), 0 if draft is None else _row_pitch(draft, cols, "draft"),
-                                _p(token), _p(parent), _p(tree_row0), rows, n, max_nodes, cols, _p(u_node), _p(u_final), _p(path), _p(tokens),
-                                _p(n_path), max_path, _s()), "wkb_tree_verify")
+    i32, f32 = torch.int32, torch.float32
+    check(lib().wkb_tree_verify(pp, ldp, pd, ldq, _on(dev, token, rows, i32, "token"), _on(dev, parent, rows, i32, "parent"),
+                                _on(dev, tree_row0, n + 1, i32, "tree_row0"), rows, n, max_nodes, cols, _on(dev, u_node, rows, f32, "u_node"),
+                                _on(dev, u_final, n, f32, "u_final"), _on(dev, path, n * max_path, i32, "path"),
+                                _on(dev, tokens, n * max_path, i32, "tokens"), _on(dev, n_path, n, i32, "n_path"), max_path, _raw_stream(dev)),
+          "wkb_tree_verify")
     return path, n_path, tokens
 
 
 def paged_kv_commit(kv, block_table, tree_slot, tree_ctx, path, n_path, mbps, new_ctx=None):
     """Move the accepted nodes' K / V to the positions behind the context, in every layer (wkb_paged_kv_commit); new_ctx
     (optional int32 [n], other memory than tree_ctx) receives the context of the next step."""
-    n = tree_slot.numel()
-    _vec(tree_slot, n, torch.int32, "tree_slot"); _vec(tree_ctx, n, torch.int32, "tree_ctx"); _vec(n_path, n, torch.int32, "n_path")
-    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != n or not path.is_contiguous():
-        raise ValueError("path must be a contiguous int32 [n, max_path]")
-    if kv.k.dtype != torch.bfloat16 or not kv.k.is_contiguous() or not kv.v.is_contiguous():
-        raise ValueError("the cache must be contiguous bf16")
-    if block_table.dtype != torch.int32 or not block_table.is_contiguous() or block_table.numel() % mbps:
-        raise ValueError("block_table must be a contiguous int32 [slots, mbps]")
-    if new_ctx is not None:
-        _vec(new_ctx, n, torch.int32, "new_ctx")
-    _same_device(kv.k, kv.v, block_table, tree_slot, tree_ctx, path, n_path, new_ctx)
-    check(lib().wkb_paged_kv_commit(_p(kv.k), _p(kv.v), kv.layers, kv.k.stride(0), kv.num_pages, _p(block_table), _p(tree_slot), _p(tree_ctx), _p(path),
-                                    _p(n_path), path.shape[1], n, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps, _p(new_ctx), _s()),
-          "wkb_paged_kv_commit")
+    dev, n, i32 = _here(tree_slot), tree_slot.numel(), torch.int32
+    k, v, layer_stride = _slabs(dev, kv)
+    if path.dim() != 2 or path.shape[0] != n:
+        raise ValueError("path must be int32 [n, max_path]")
+    check(lib().wkb_paged_kv_commit(k, v, kv.layers, layer_stride, kv.num_pages, _table(dev, block_table, mbps), _on(dev, tree_slot, n, i32, "tree_slot"),
+                                    _on(dev, tree_ctx, n, i32, "tree_ctx"), _on(dev, path, n * path.shape[1], i32, "path"),
+                                    _on(dev, n_path, n, i32, "n_path"), path.shape[1], n, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps,
+                                    None if new_ctx is None else _on(dev, new_ctx, n, i32, "new_ctx"), _raw_stream(dev)), "wkb_paged_kv_commit")
     return kv
