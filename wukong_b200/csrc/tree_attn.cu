@@ -159,13 +159,13 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void
               num_pages, q_row_stride, out_row_stride};
   cudaStream_t st = as_stream(stream);
   if (page_tokens >= 8) {      // a page of 8 tokens fills whole swizzle atoms of the operand
-    const i64 row_blocks = (max_nodes * group + tree::QROWS - 1) / tree::QROWS, key_blocks = (max_blocks_per_seq * page_tokens + tree::KBLK - 1) / tree::KBLK;
+    const i64 row_blocks = (max_nodes * group + tree::QROWS - 1) / tree::QROWS, key_blocks = (max_blocks_per_seq * page_tokens + tree::KBLK - 1) / tree::KBLK + tree::UNIT_COST;
     if ((double)n_trees * (double)kv_heads * (double)row_blocks * (double)key_blocks > 2147000000.0) return (int)cudaErrorInvalidValue;
 #define WKB_TREE_CASE(HD_, QS_, PS_)                                   \
-  if (head_dim == HD_ && (q_dtype == 1 ? 1 : out_dtype == 0 ? 3 : 2) == QS_ && (out_dtype == 0 ? 2 : 1) == PS_) \
+  if (head_dim == HD_ && (q_dtype == 0 ? 2 : 1) == QS_ && (out_dtype == 0 ? 2 : 1) == PS_) \
     return tree::launch_tc<HD_, QS_, PS_>(q, kcache, vcache, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, out_dtype, g, scale, scratch, st);
-    WKB_TREE_CASE(64, 1, 1) WKB_TREE_CASE(64, 1, 2) WKB_TREE_CASE(64, 2, 1) WKB_TREE_CASE(64, 3, 2)
-    WKB_TREE_CASE(128, 1, 1) WKB_TREE_CASE(128, 1, 2) WKB_TREE_CASE(128, 2, 1) WKB_TREE_CASE(128, 3, 2)
+    WKB_TREE_CASE(64, 1, 1) WKB_TREE_CASE(64, 1, 2) WKB_TREE_CASE(64, 2, 1) WKB_TREE_CASE(64, 2, 2)
+    WKB_TREE_CASE(128, 1, 1) WKB_TREE_CASE(128, 1, 2) WKB_TREE_CASE(128, 2, 1) WKB_TREE_CASE(128, 2, 2)
 #undef WKB_TREE_CASE
   }
   const i64 blocks = (rows * q_heads + 7) / 8;

@@ -10,8 +10,8 @@
 // alternate key blocks with tensor-memory columns of their own, so one team's exponentials run while the other's products
 // do:   S = Q K^T (128 x 128) -> P = exp2(S - m), bf16, over the same columns -> O += P V (128 x head_dim).
 // The running maximum m of a row moves only when a block exceeds it by 2^8; the accumulator is rescaled then and not at
-// every block.  f32 queries are two bf16 parts (hi + lo, two products); for f32 results
-// they are three and P is two.
+// every block.  f32 queries are two bf16 parts (hi + lo, two products); for f32 results P
+// is two parts as well (5e-6 of the result over 8192 keys, of which the products' accumulation is the larger share).
 //
 // With 64 (32) query rows or fewer the operand's 128 rows hold 2 (4) copies of them, and each copy takes its own half
 // (quarter) of a block's keys, with zeros for the others': a team's warps share the exponentials of a small tree that
@@ -76,10 +76,10 @@ template <int HD, int QS>
 struct TcSmem {
   static constexpr int NSUB = HD / 64, BLK = NSUB * SUB;                 // bytes of 128 rows of an operand
   static constexpr int HEADER = 3072;                                    // barriers, (m, l) of the teams, flags
-  static constexpr int Q_BYTES = QS * BLK < 32768 ? 32768 : QS * BLK;    // also the 128 x 64 f32 of the epilogue
-  static constexpr int SLOTS = (232448 - HEADER - Q_BYTES) / BLK > 12 ? 12 : (232448 - HEADER - Q_BYTES) / BLK;
+  static constexpr int Q_BYTES = QS * BLK, STAGE_BYTES = QROWS * 64 * 4;
+  static constexpr int ROOM = (232448 - HEADER - Q_BYTES - STAGE_BYTES) / BLK, SLOTS = ROOM > 12 ? 12 : ROOM;
   static constexpr int NK = (SLOTS + 1) / 2, NV = SLOTS / 2;
-  static constexpr int BYTES = HEADER + Q_BYTES + SLOTS * BLK;
+  static constexpr int BYTES = HEADER + Q_BYTES + STAGE_BYTES + SLOTS * BLK;
   static_assert(NV >= 2 && BYTES <= 232448, "at least two blocks of each operand in flight");
 };
 
@@ -175,7 +175,9 @@ __device__ __forceinline__ TreeWork tree_work(const Geo& g, const int* slot, con
   w.rowblks = (w.t.nodes * (g.q_heads / g.kv_heads) + QROWS - 1) / QROWS;      // 0 for a tree without rows
   return w;
 }
-__device__ __forceinline__ int tree_items(const Geo& g, const TreeWork& w) { return w.blocks * w.rowblks * g.kv_heads; }
+// A unit counts as its blocks and UNIT_COST more: what beginning and ending one takes, in blocks.
+constexpr int UNIT_COST = 5;
+__device__ __forceinline__ int tree_items(const Geo& g, const TreeWork& w) { return (w.blocks + UNIT_COST) * w.rowblks * g.kv_heads; }
 
 // One piece of a unit: blocks [b0, b1) of `unit_len`.
 struct Piece {
@@ -186,23 +188,25 @@ struct Piece {
 struct Walk {
   int item, end, tree, tree_start;
   __device__ __forceinline__ bool next(const Geo& g, const int* slot, const int* ctx, const int* row0, Piece& p) {
-    if (item >= end) return false;
-    for (;;) {
-      p.w = tree_work(g, slot, ctx, row0, tree);
-      const int items = tree_items(g, p.w);
-      if (item < tree_start + items) break;
-      tree_start += items;
-      if (++tree >= g.n_trees) return false;
+    while (item < end) {
+      for (;;) {
+        p.w = tree_work(g, slot, ctx, row0, tree);
+        const int items = tree_items(g, p.w);
+        if (item < tree_start + items) break;
+        tree_start += items;
+        if (++tree >= g.n_trees) return false;
+      }
+      const int size = p.w.blocks + UNIT_COST, unit = (item - tree_start) / size;
+      p.tree = tree;
+      p.head = unit / p.w.rowblks;
+      p.rowblk = unit - p.head * p.w.rowblks;
+      p.unit_start = tree_start + unit * size;
+      p.b0 = item - p.unit_start;
+      p.b1 = min(p.w.blocks, p.b0 + end - item);
+      item = p.unit_start + size;
+      if (p.b0 < p.b1) return true;      // else the share begins behind the unit's last block
     }
-    const int unit = (item - tree_start) / p.w.blocks;
-    p.tree = tree;
-    p.head = unit / p.w.rowblks;
-    p.rowblk = unit % p.w.rowblks;
-    p.unit_start = tree_start + unit * p.w.blocks;
-    p.b0 = item - p.unit_start;
-    p.b1 = min(p.w.blocks, p.b0 + end - item);
-    item = p.unit_start + p.b1;
-    return true;
+    return false;
   }
 };
 
@@ -217,7 +221,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   // header: barriers at 0, flags at 256, (m, l) at 512 .. 2560; the operands behind it on a 1024-byte boundary
-  const uint32_t q_base = (raw + 2560 + 1023u) & ~1023u, k_ring = q_base + SM::Q_BYTES, v_ring = k_ring + NK * BLK;
+  const uint32_t q_base = (raw + 2560 + 1023u) & ~1023u, stage_base = q_base + SM::Q_BYTES, k_ring = stage_base + SM::STAGE_BYTES, v_ring = k_ring + NK * BLK;
   auto kfull = [&](int s) { return raw + 8u * s; };
   auto kempty = [&](int s) { return raw + 8u * (NK + s); };
   auto vfull = [&](int s) { return raw + 8u * (2 * NK + s); };
@@ -230,7 +234,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   static_assert(8 * (2 * NK + 2 * NV + 7) <= 256, "barriers fit the header");
   volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + 256);      // 0 tensor memory, 1 failed, 2 V not finite, 3.. the share
   float2* ml_s = reinterpret_cast<float2*>(smem_raw + 512);
-  float* stage = reinterpret_cast<float*>(smem_raw + (q_base - raw));
+  float* stage = reinterpret_cast<float*>(smem_raw + (stage_base - raw));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (q_base - raw > (uint32_t)SM::HEADER) {      // the operands would not fit behind the header: never, as the base is 1024-byte aligned
@@ -295,8 +299,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (!none) {
       Walk w = walk;
       Piece p;
-      w.next(g, slot, ctxs, row0s, p);
-      st.unit_start = p.unit_start; st.unit_len = p.w.blocks; st.tree = p.tree; st.head = p.head; st.rowblk = p.rowblk;
+      if (w.next(g, slot, ctxs, row0s, p)) { st.unit_start = p.unit_start; st.unit_len = p.w.blocks; st.tree = p.tree; st.head = p.head; st.rowblk = p.rowblk; }
     }
     scr.start[blockIdx.x] = st;
   }
@@ -409,7 +412,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const float sc = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-37f);
     const bool negate = scale < 0.0f;
     bool ok = true;
-    int n = 0, uses = 0;      // blocks of the share, this team's blocks
+    int n = 0, uses = 0, done[2] = {0, 0};      // blocks of the share, this team's blocks, either team's
     auto wait = [&](uint32_t bar, uint32_t parity) {
       if (ok && !__all_sync(0xffffffffu, bar_wait(bar, parity))) {
         ok = false;
@@ -417,66 +420,77 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
     };
     auto teams_sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };      // every softmax thread passes every one of these
-    Piece p;
-    while (walk.next(g, slot, ctxs, row0s, p)) {
-      const int len = p.b1 - p.b0;
-      const int live = min(QROWS, p.w.t.nodes * group - p.rowblk * QROWS);
-      const int copies = live <= 32 ? 4 : live <= 64 ? 2 : 1, crows = QROWS / copies;
-      const int copy = a / crows, r = a % crows;
-      // ---- the query operand: K-major, 128-byte swizzle
-      // (a row is loaded once and stored to every copy; the loads of a batch are in flight together)
-      {
-        constexpr int CH = HD / 8, BATCH = 4;      // 16-byte chunks of bf16 a row
-        for (int i0 = tid; i0 < crows * CH; i0 += 256 * BATCH) {
-          uint4 part[BATCH][QS < 2 ? 2 : QS];
-          float4 x[BATCH], y[BATCH];
+    // The query operand (K-major, 128-byte swizzle) of a piece: rows are fetched to registers, BATCH chunks a thread, and
+    // stored to every copy.
+    constexpr int CH = HD / 8, BATCH = 4;      // 16-byte chunks of bf16 a row
+    float4 qx[BATCH], qy[QS == 1 ? 1 : BATCH];
+    auto live_of = [&](const Piece& p) { return min(QROWS, p.w.t.nodes * group - p.rowblk * QROWS); };
+    auto copies_of = [&](int live) { return live <= 32 ? 4 : live <= 64 ? 2 : 1; };
+    auto q_fetch = [&](const Piece& p, int i0) {
+      const int live = live_of(p);
 #pragma unroll
-          for (int b = 0; b < BATCH; ++b) {
-            const int idx = i0 + b * 256, qr = idx / CH, c = idx % CH;
-            x[b] = y[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            part[b][0] = make_uint4(0u, 0u, 0u, 0u);
-            if (qr >= live) continue;
-            const int ur = p.rowblk * QROWS + qr;
-            const i64 at = (i64)(p.w.t.row0 + (ur >> gshift)) * g.q_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD + c * 8;
-            if (QS == 1) part[b][0] = *reinterpret_cast<const uint4*>(static_cast<const u16*>(q) + at);
-            else {
-              x[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
-              y[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + 4);
-            }
-          }
+      for (int b = 0; b < BATCH; ++b) {
+        const int idx = i0 + b * 256, qr = idx / CH, c = idx % CH, ur = p.rowblk * QROWS + qr;
+        qx[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (QS > 1) qy[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (qr >= live) continue;
+        const i64 at = (i64)(p.w.t.row0 + (ur >> gshift)) * g.q_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD + c * 8;
+        if (QS == 1) qx[b] = *reinterpret_cast<const float4*>(static_cast<const u16*>(q) + at);
+        else {
+          qx[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
+          qy[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + 4);
+        }
+      }
+    };
+    auto q_put = [&](const Piece& p) {
+      const int copies = copies_of(live_of(p)), crows = QROWS / copies;
+      const uint32_t flip = negate ? 0x80008000u : 0u;
+#pragma unroll 1
+      for (int i0 = tid;;) {
 #pragma unroll
-          for (int b = 0; b < BATCH; ++b) {
-            const int idx = i0 + b * 256, qr = idx / CH, c = idx % CH;
-            if (idx >= crows * CH) break;
-            if (QS > 1) {
-              float f[8] = {x[b].x, x[b].y, x[b].z, x[b].w, y[b].x, y[b].y, y[b].z, y[b].w};
-#pragma unroll
-              for (int k = 0; k < QS; ++k) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  w[e] = pack_bf16(f[2 * e], f[2 * e + 1]);
-                  f[2 * e] -= u2f(w[e] << 16);
-                  f[2 * e + 1] -= u2f(w[e] & 0xffff0000u);
-                }
-                part[b][k] = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            }
-            const uint32_t flip = negate ? 0x80008000u : 0u;
-            const uint32_t dst = q_base + (uint32_t)(c >> 3) * SUB + (uint32_t)qr * 128u + (uint32_t)(((c & 7) ^ (qr & 7)) << 4);
+        for (int b = 0; b < BATCH; ++b) {
+          const int idx = i0 + b * 256, qr = idx / CH, c = idx % CH;
+          if (idx >= crows * CH) break;
+          uint32_t w[QS][4];
+          if (QS == 1) { w[0][0] = f2u(qx[b].x); w[0][1] = f2u(qx[b].y); w[0][2] = f2u(qx[b].z); w[0][3] = f2u(qx[b].w); }
+          else {
+            const float4 y = qy[QS == 1 ? 0 : b];
+            float f[8] = {qx[b].x, qx[b].y, qx[b].z, qx[b].w, y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int k = 0; k < QS; ++k)
-              for (int cp = 0; cp < copies; ++cp)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * BLK + (uint32_t)(cp * crows) * 128u), "r"(part[b][k].x ^ flip),
-                             "r"(part[b][k].y ^ flip), "r"(part[b][k].z ^ flip), "r"(part[b][k].w ^ flip)
-                             : "memory");
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                w[k][e] = pack_bf16(f[2 * e], f[2 * e + 1]);
+                f[2 * e] -= u2f(w[k][e] << 16);
+                f[2 * e + 1] -= u2f(w[k][e] & 0xffff0000u);
+              }
           }
+          const uint32_t dst = q_base + (uint32_t)(c >> 3) * SUB + (uint32_t)qr * 128u + (uint32_t)(((c & 7) ^ (qr & 7)) << 4);
+#pragma unroll 1
+          for (int cp = 0; cp < copies; ++cp)
+#pragma unroll
+            for (int k = 0; k < QS; ++k)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * BLK + (uint32_t)(cp * crows) * 128u), "r"(w[k][0] ^ flip),
+                           "r"(w[k][1] ^ flip), "r"(w[k][2] ^ flip), "r"(w[k][3] ^ flip)
+                           : "memory");
         }
+        i0 += 256 * BATCH;
+        if (i0 >= crows * CH) break;
+        q_fetch(p, i0);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
-
+    };
+    Piece p, following;
+    bool more = walk.next(g, slot, ctxs, row0s, following);
+    if (more) { q_fetch(following, tid); q_put(following); }
+    while (more) {
+      p = following;
+      more = walk.next(g, slot, ctxs, row0s, following);
+      const int len = p.b1 - p.b0;
+      const int live = live_of(p), copies = copies_of(live), crows = QROWS / copies;
+      const int copy = a / crows, r = a % crows;
       // ---- the team's key blocks
       auto mask_of = [&](int row) { return mask + (i64)(p.w.t.row0 + ((p.rowblk * QROWS + row) >> gshift)) * g.mask_words; };
       const uint32_t* own_mask = mask_of(min(r, live - 1));
@@ -616,13 +630,17 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       n += len;
 
       // ---- the result: the teams' accumulators lie in the same lanes and are added in registers; the copies lie in other
-      // lanes and are added through the query operand's memory, 64 columns at a time
-      if (team < len) wait(o_done(team), (uses - 1) & 1);
+      // lanes and are added through shared memory, 64 columns at a time
+      if (more) q_fetch(following, tid);
       ml_s[team * QROWS + a] = make_float2(team < len ? m : -INFINITY, team < len ? l : 0.0f);
-      tc_fence_before();
-      teams_sync();
-      tc_fence_after();
+      teams_sync();      // every product with this piece's query is done: the next one's can start while the result is written
+      if (more) q_put(following);
       const bool both = len > 1;      // team 1 had a block
+      done[0] += (len + 1) >> 1;
+      done[1] += len >> 1;
+      wait(o_done(0), (done[0] - 1) & 1);
+      if (both) wait(o_done(1), (done[1] - 1) & 1);
+      tc_fence_after();
       float m_all = -INFINITY, l_all = 0.0f;
 #pragma unroll 1
       for (int i = r; i < (both ? 2 : 1) * QROWS; i += crows) m_all = fmaxf(m_all, ml_s[i].x);      // copies of team 0, then of team 1
@@ -723,7 +741,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (tid == 0) flags[2] = 0;
       }
       tc_fence_before();
-      teams_sync();      // the accumulators, the operand's memory and ml_s are free
+      teams_sync();      // the accumulators and ml_s are free
     }
   }
   tc_fence_before();
@@ -745,7 +763,7 @@ __global__ void __launch_bounds__(256) tree_attn_join_kernel(const int* __restri
   const int c = blockIdx.x + 1;
   const ShareStart st = scr.start[c];
   const int x = c * st.share;
-  if (x >= st.total || x == st.unit_start || x - st.share > st.unit_start) return;
+  if (x >= st.total || st.unit_len == 0 || x <= st.unit_start || x - st.share > st.unit_start) return;
   if (*status == WKB_STATUS_ATTN_WAIT) return;
   const int last = (st.unit_start + st.unit_len - 1) / st.share, group = g.q_heads / g.kv_heads;
   const TreeRef t = tree_ref(g, slot, ctxs, row0s, st.tree);

@@ -379,7 +379,8 @@ def tree_verify(probs, draft, token, parent, tree_row0, u_node, u_final, max_nod
     pd, ldq = (None, 0) if draft is None else _matrix(dev, draft, cols, "draft")
     if out is None:
         buf = torch.empty(n * (2 * max_path + 1), dtype=torch.int32, device=probs.device)
-        out = buf[:n * max_path].view(n, max_path), buf[2 * n * max_path:], buf[n * max_path:2 * n * max_path].view(n, max_path)
+        shape, pitch, part = (n, max_path), (max_path, 1), n * max_path
+        out = buf.as_strided(shape, pitch, 0), buf.as_strided((n,), (1,), 2 * part), buf.as_strided(shape, pitch, part)
     path, n_path, tokens = out
     i32, f32 = torch.int32, torch.float32
     check(lib().wkb_tree_verify(pp, ldp, pd, ldq, _on(dev, token, rows, i32, "token"), _on(dev, parent, rows, i32, "parent"),
