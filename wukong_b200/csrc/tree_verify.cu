@@ -11,12 +11,15 @@ namespace verify {
 constexpr int MAX_NODES = 256;
 
 // ---- temperature softmax --------------------------------------------------------------------------------------------
-__device__ __forceinline__ float load_logit(const void* x, int dtype, i64 at) {
-  return dtype == 0 ? static_cast<const float*>(x)[at] : bf16_bits_to_f32(static_cast<const u16*>(x)[at]);
-}
-// One CTA per row: maximum (and its lowest column), sum, write.
-__global__ void __launch_bounds__(512) token_probs_kernel(const void* __restrict__ x, int dtype, i64 ld, const float* __restrict__ temperature,
-                                                          float* __restrict__ out, i64 ld_out, i64 cols) {
+__device__ __forceinline__ float logit(const float* x, int i) { return x[i]; }
+__device__ __forceinline__ float logit(const __nv_bfloat16* x, int i) { return bf16_bits_to_f32(reinterpret_cast<const u16*>(x)[i]); }
+// log2(e) / t, finite and not 0, so that the maximum keeps weight 1 and a token that is ruled out weight 0
+__device__ __forceinline__ float exponent_scale(float t) { return fmaxf(fminf(1.4426950408889634f / t, 3.402823466e+38f), 1e-37f); }
+
+// Rows wider than a cluster's registers: one CTA per row, three passes (the second and third mostly from L2).
+template <typename T>
+__global__ void __launch_bounds__(512) token_probs_wide_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature, float* __restrict__ out,
+                                                               i64 ld_out, int cols) {
   pdl_wait();
   pdl_trigger();
   __shared__ float red_v[16];
@@ -26,11 +29,11 @@ __global__ void __launch_bounds__(512) token_probs_kernel(const void* __restrict
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float best = -INFINITY;
   int at = 0x7fffffff;
-  bool nan = false;
-  for (i64 i = threadIdx.x; i < cols; i += 512) {
-    const float v = load_logit(x, dtype, row * ld + i);
+  bool nan = temp != temp;
+  for (int i = threadIdx.x; i < cols; i += 512) {
+    const float v = logit(x + row * ld, i);
     nan |= v != v;
-    if (v > best || (v == best && (int)i < at)) { best = v; at = (int)i; }
+    if (v > best) { best = v; at = i; }
   }
   for (int o = 16; o > 0; o >>= 1) {
     const float v = __shfl_xor_sync(0xffffffffu, best, o);
@@ -39,154 +42,372 @@ __global__ void __launch_bounds__(512) token_probs_kernel(const void* __restrict
   }
   if (lane == 0) { red_v[warp] = best; red_i[warp] = at; }
   nan = __syncthreads_or(nan);
-  best = red_v[0]; at = red_i[0];
-  for (int w = 1; w < 16; ++w)
+  for (int w = 0; w < 16; ++w)
     if (red_v[w] > best || (red_v[w] == best && red_i[w] < at)) { best = red_v[w]; at = red_i[w]; }
   __syncthreads();
-  const float scale = fminf(1.4426950408889634f / temp, 3.402823466e+38f);      // finite, so that the maximum keeps weight 1
+  const float scale = exponent_scale(temp);
   float sum = 0.0f;
   if (temp > 0.0f) {
-    for (i64 i = threadIdx.x; i < cols; i += 512) sum += exp2f((load_logit(x, dtype, row * ld + i) - best) * scale);
+    for (int i = threadIdx.x; i < cols; i += 512) sum += exp2f((logit(x + row * ld, i) - best) * scale);
     sum = warp_sum(sum);
     if (lane == 0) red_v[warp] = sum;
     __syncthreads();
     sum = 0.0f;
     for (int w = 0; w < 16; ++w) sum += red_v[w];
   }
-  for (i64 i = threadIdx.x; i < cols; i += 512) {
+  for (int i = threadIdx.x; i < cols; i += 512) {
     float p;
-    if (nan || temp != temp) p = NAN;
+    if (nan) p = NAN;
     else if (best == -INFINITY) p = 0.0f;                 // every token is ruled out
-    else if (temp > 0.0f) p = exp2f((load_logit(x, dtype, row * ld + i) - best) * scale) / sum;
-    else p = (int)i == at ? 1.0f : 0.0f;
+    else if (temp > 0.0f) p = exp2f((logit(x + row * ld, i) - best) * scale) / sum;
+    else p = i == at ? 1.0f : 0.0f;
     out[row * ld_out + i] = p;
   }
+}
+
+// Two floats per CTA travel through the cluster: `mine` is published, `all` collects every CTA's.
+__device__ __forceinline__ float2 cluster_get(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+constexpr int PT = 512;      // threads of a CTA
+
+// A row is a cluster's: each CTA keeps its E * 512 columns in registers, so the logits are read once and the probabilities
+// written once (HBM is the bound).  The CTAs trade (maximum, sum relative to it) through shared memory.  Element loads are
+// 4 (2) bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no more than that.
+template <typename T, int E>
+__global__ void __launch_bounds__(PT) token_probs_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature, float* __restrict__ out,
+                                                         i64 ld_out, int cols) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float red[PT / 32];
+  __shared__ float2 mine[2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  const i64 row = blockIdx.x / size;
+  const int first = (int)rank * E * PT + threadIdx.x;
+  const T* xr = x + row * ld;
+  const float temp = temperature ? temperature[row] : 1.0f;
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = first + e * PT;
+    v[e] = i < cols ? logit(xr, i) : -INFINITY;
+  }
+  float m = -INFINITY;
+  bool nan = temp != temp;
+#pragma unroll
+  for (int e = 0; e < E; ++e) { m = fmaxf(m, v[e]); nan |= v[e] != v[e]; }
+  m = warp_max(m);
+  if (lane == 0) red[warp] = m;
+  nan = __syncthreads_or(nan);
+#pragma unroll
+  for (int w = 0; w < PT / 32; ++w) m = fmaxf(m, red[w]);
+  if (temp <= 0.0f) {      // (a branch that all CTAs of the row take alike)
+    // greedy: the lowest column of the row's maximum
+    if (threadIdx.x == 0) mine[0] = make_float2(m, nan ? 1.0f : 0.0f);
+    cluster_sync();
+    for (uint32_t k = 0; k < size; ++k) {
+      const float2 o = cluster_get(smem_addr(&mine[0]), k);
+      m = fmaxf(m, o.x);
+      nan |= o.y != 0.0f;
+    }
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int e = E - 1; e >= 0; --e)
+      if (v[e] == m && first + e * PT < cols) at = first + e * PT;
+    for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+    __syncthreads();
+    if (lane == 0) red[warp] = __int_as_float(at);
+    __syncthreads();
+    for (int w = 0; w < PT / 32; ++w) at = min(at, __float_as_int(red[w]));
+    if (threadIdx.x == 0) mine[1] = make_float2(__int_as_float(at), 0.0f);
+    cluster_sync();
+    for (uint32_t k = 0; k < size; ++k) at = min(at, __float_as_int(cluster_get(smem_addr(&mine[1]), k).x));
+    if (m == -INFINITY) at = -1;      // every token is ruled out
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = first + e * PT;
+      if (i < cols) out[row * ld_out + i] = nan ? NAN : i == at ? 1.0f : 0.0f;
+    }
+    cluster_sync();      // no CTA leaves while another may read its numbers
+    return;
+  }
+  const float scale = exponent_scale(temp);
+  const float base = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    v[e] = exp2f((v[e] - base) * scale);
+    sum += v[e];
+  }
+  sum = warp_sum(sum);
+  __syncthreads();
+  if (lane == 0) red[warp] = sum;
+  __syncthreads();
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < PT / 32; ++w) sum += red[w];
+  if (threadIdx.x == 0) mine[0] = make_float2(nan ? NAN : m, sum);      // a NaN spoils the row
+  cluster_sync();
+  float m_all = -INFINITY, l = 0.0f;
+  for (uint32_t k = 0; k < size; ++k) {
+    const float2 o = cluster_get(smem_addr(&mine[0]), k);
+    nan |= o.x != o.x;
+    m_all = fmaxf(m_all, o.x);
+  }
+  for (uint32_t k = 0; k < size; ++k) {
+    const float2 o = cluster_get(smem_addr(&mine[0]), k);
+    if (o.x != -INFINITY) l += o.y * exp2f((o.x - m_all) * scale);
+  }
+  const float f = nan ? NAN : m == -INFINITY ? 0.0f : exp2f((m - m_all) * scale) / l;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = first + e * PT;
+    if (i < cols) out[row * ld_out + i] = v[e] * f;
+  }
+  cluster_sync();
 }
 
 // ---- verification ---------------------------------------------------------------------------------------------------
 __device__ __forceinline__ double weight(float v) { return v > 0.0f && v <= 3.402823466e+38f ? (double)v : 0.0; }
 
-// One CTA per tree.  Thread 0 walks the tree; a pass over the vocabulary sums the mass that is left.
-__global__ void __launch_bounds__(512) tree_verify_kernel(const float* __restrict__ probs, i64 ld_p, const float* __restrict__ draft, i64 ld_q,
-                                                          const int* __restrict__ token, const int* __restrict__ parent, const int* __restrict__ row0,
-                                                          int rows, int cols, int max_nodes, const float* __restrict__ u_node,
-                                                          const float* __restrict__ u_final, int* __restrict__ path, int* __restrict__ tokens,
-                                                          int* __restrict__ n_path, int max_path) {
+// What the leader asks of its cluster: the masses that are left of node `row` after `tries` rejections.
+struct Ask {
+  int row, tries, last;
+};
+// One cluster per tree.  The walk needs two numbers of each node, p and q of its token in its parent's rows: the leading
+// CTA gathers them for all nodes at once, and its first warp walks in shared memory.  Only the mass that is left after a
+// rejection (before the next sibling is tried) and the final draw need a pass over the vocabulary, a contiguous run of
+// columns per warp of the cluster; the row is read from HBM once and the run that holds the draw a second time, from L2.
+// The leader alone decides, so every CTA takes the same steps.  Sums are in a fixed order.  Bound: the latency of the four
+// dependent trips to memory for a few trees, the rows' bytes for many.
+template <bool DRAFT>
+__global__ void __launch_bounds__(PT) tree_verify_kernel(const float* __restrict__ probs, i64 ld_p, const float* __restrict__ draft, i64 ld_q,
+                                                         const int* __restrict__ token, const int* __restrict__ parent, const int* __restrict__ row0,
+                                                         int rows, int cols, int max_nodes, const float* __restrict__ u_node,
+                                                         const float* __restrict__ u_final, int* __restrict__ path, int* __restrict__ tokens,
+                                                         int* __restrict__ n_path, int max_path) {
   pdl_wait();
   pdl_trigger();
-  __shared__ int tok_s[MAX_NODES], par_s[MAX_NODES], tried[MAX_NODES], path_s[MAX_NODES];
-  __shared__ double z_s[MAX_NODES + 1], part[16];
-  __shared__ int cur, tries, len, more;
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ int tok_s[MAX_NODES], par_s[MAX_NODES], tried_s[MAX_NODES], path_s[MAX_NODES];
+  __shared__ float p_s[MAX_NODES], q_s[MAX_NODES], u_s[MAX_NODES];
+  __shared__ double z_s[MAX_NODES + 1], part_s[8 * PT / 32];
+  __shared__ Ask ask;
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  const int t = blockIdx.x / size, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)size * (PT / 32);
   const int a = min(max(row0[t], 0), rows), nodes = min(min(max(row0[t + 1], a), rows) - a, max_nodes);
-  for (int i = threadIdx.x; i < max_path; i += 512) { path[(i64)t * max_path + i] = -1; tokens[(i64)t * max_path + i] = -1; }
-  if (nodes <= 0) {
-    if (threadIdx.x == 0) n_path[t] = 0;
+  int* const my_path = path + (i64)t * max_path;
+  int* const my_tokens = tokens + (i64)t * max_path;
+  if (nodes <= 0) {      // (uniform over the cluster: nobody meets)
+    if (rank == 0) {
+      for (int i = threadIdx.x; i < max_path; i += PT) { my_path[i] = -1; my_tokens[i] = -1; }
+      if (threadIdx.x == 0) n_path[t] = 0;
+    }
     return;
   }
-  for (int i = threadIdx.x; i < nodes; i += 512) { tok_s[i] = token[a + i]; par_s[i] = parent[a + i]; }
-  if (threadIdx.x == 0) { cur = 0; tries = 0; len = 1; path_s[0] = 0; z_s[0] = 1.0; }
-  __syncthreads();
-  // what is left of column i's weight after the `tries` rejections below node cur
-  auto left = [&](int i) -> double {
-    double r = weight(probs[(i64)(a + cur) * ld_p + i]);
-    if (draft) {
-      const double q = tries ? weight(draft[(i64)(a + cur) * ld_q + i]) : 0.0;
-      for (int k = 0; k < tries; ++k) r = fmax(r - z_s[k] * q, 0.0);
+  if (rank == 0) {
+    for (int i = threadIdx.x; i < nodes; i += PT) {
+      const int x = token[a + i], par = parent[a + i];
+      const bool known = i > 0 && par >= 0 && par < nodes && x >= 0 && x < cols;
+      const float u = u_node[a + i];
+      tok_s[i] = x;
+      par_s[i] = i > 0 ? par : -1;
+      u_s[i] = u != u ? 0.0f : fminf(1.0f, fmaxf(0.0f, u));
+      p_s[i] = known ? probs[(i64)(a + par) * ld_p + x] : 0.0f;
+      q_s[i] = DRAFT && known ? draft[(i64)(a + par) * ld_q + x] : 0.0f;
+    }
+    __syncthreads();
+  }
+  const int run = ((cols + warps - 1) / warps + 31) / 32 * 32;      // columns of a warp
+  // what is left of column i's weight p (q the draft's) after the rejections
+  auto left = [&](int i, float p, float q, int tries) -> double {
+    double r = weight(p);
+    if (DRAFT) {
+      const double w = weight(q);
+      for (int k = 0; k < tries; ++k) r = fmax(r - z_s[k] * w, 0.0);
     } else {
       for (int k = 0; k < tries; ++k)
-        if (tried[k] == i) r = 0.0;
+        if (tried_s[k] == i) r = 0.0;
     }
     return r;
   };
-  const int seg = ((cols + 15) / 16 + 31) / 32 * 32;      // a warp's columns
-  auto sums = [&]() {
-    double s = 0.0;
-    for (int i = warp * seg + lane; i < min(cols, (warp + 1) * seg); i += 32) s += left(i);
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) part[warp] = s;
-    __syncthreads();
+  auto remote = [&](const void* p, uint32_t of) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(of));
+    return r;
   };
-  int next = 1;
+  constexpr int BATCH = 8;      // loads in flight per thread
+  int cur = 0, tries = 0, len = 1, next = 1;      // the walk, of the leader's first warp
   bool summed = false;
+  if (rank == 0 && warp == 0 && lane == 0) { path_s[0] = 0; z_s[0] = 1.0; }
   for (;;) {
-    if (threadIdx.x == 0) {
-      more = 0;
-      while (len < max_path) {
-        while (next < nodes && par_s[next] != cur) ++next;
-        if (next >= nodes) break;
-        if (draft && tries && !summed) { more = 1; break; }      // the mass that is left is needed first
-        const int x = tok_s[next];
+    if (rank == 0 && warp == 0) {
+      bool wait = false;
+      __syncwarp();
+      while (len < max_path && !wait) {
+        int c = -1;      // the next node from `next` on whose parent is `cur`
+        for (int b = next & ~31; b < nodes && c < 0; b += 32) {
+          const unsigned hit = __ballot_sync(0xffffffffu, b + lane < nodes && b + lane >= next && par_s[b + lane] == cur);
+          if (hit) c = b + __ffs(hit) - 1;
+        }
+        if (c < 0) break;
+        if (DRAFT && tries && !summed) { wait = true; break; }      // the mass that is left is needed first
+        const int x = tok_s[c];
         const bool in = x >= 0 && x < cols;
-        const double q = !draft ? 1.0 : in ? weight(draft[(i64)(a + cur) * ld_q + x]) : 0.0;
-        const double r = in ? left(x) : 0.0;
-        float u = u_node[a + next];
-        u = u != u ? 0.0f : fminf(1.0f, fmaxf(0.0f, u));
-        if ((double)u * q * z_s[tries] < r) {
-          path_s[len++] = next;
-          cur = next;
+        const double q = !DRAFT ? 1.0 : in ? weight(q_s[c]) : 0.0, r = in ? left(x, p_s[c], q_s[c], tries) : 0.0;
+        __syncwarp();
+        if ((double)u_s[c] * q * z_s[tries] < r) {
+          if (lane == 0) path_s[len] = c;
+          ++len;
+          cur = c;
           tries = 0;
         } else {
-          if (!draft) z_s[tries + 1] = z_s[tries] - r;
-          tried[tries++] = x;
+          if (lane == 0) {
+            if (!DRAFT) z_s[tries + 1] = z_s[tries] - r;
+            tried_s[tries] = x;
+          }
+          ++tries;
           summed = false;
         }
-        ++next;
+        __syncwarp();
+        next = c + 1;
       }
+      if (lane == 0) { ask.row = a + cur; ask.tries = tries; ask.last = wait ? 0 : 1; }
     }
-    __syncthreads();
-    if (!more) break;
-    sums();
-    if (threadIdx.x == 0) {
+    cluster_sync();
+    Ask now;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(now.row) : "r"(remote(&ask.row, 0)) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(now.tries) : "r"(remote(&ask.tries, 0)) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(now.last) : "r"(remote(&ask.last, 0)) : "memory");
+    if (rank != 0) {
+      for (int k = threadIdx.x; k < now.tries; k += PT) {
+        if (DRAFT) asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(z_s[k]) : "r"(remote(&z_s[k], 0)) : "memory");
+        else asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(tried_s[k]) : "r"(remote(&tried_s[k], 0)) : "memory");
+      }
+      __syncthreads();
+    }
+    const float* pr = probs + (i64)now.row * ld_p;
+    const float* qr = DRAFT ? draft + (i64)now.row * ld_q : nullptr;
+    {
+      const int g = (int)rank * (PT / 32) + warp, end = min((i64)cols, (i64)(g + 1) * run);
+      double s = 0.0;
+      for (i64 i0 = (i64)g * run + lane; i0 - lane < end; i0 += 32 * BATCH) {
+        float p[BATCH], q[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const bool in = i0 + k * 32 < end;
+          p[k] = in ? pr[i0 + k * 32] : 0.0f;
+          q[k] = DRAFT && now.tries && in ? qr[i0 + k * 32] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) s += left((int)i0 + k * 32, p[k], q[k], now.tries);
+      }
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote(&part_s[g], 0)), "d"(s) : "memory");
+    }
+    cluster_sync();
+    if (now.last) break;
+    if (rank == 0 && warp == 0) {
       double z = 0.0;
-      for (int w = 0; w < 16; ++w) z += part[w];
-      z_s[tries] = z;
+      for (int w = lane; w < warps; w += 32) z += part_s[w];
+      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      if (lane == 0) z_s[tries] = z;
       summed = true;
+      __syncwarp();
     }
-    __syncthreads();
   }
-  sums();
+  if (rank != 0 || warp != 0) return;
   // inverse CDF over what is left: the lowest column whose running mass exceeds u * mass, the last one with a weight otherwise
-  if (warp == 0) {
-    double total = 0.0;
-    for (int w = 0; w < 16; ++w) total += part[w];
-    int pick = -1;
-    if (total > 0.0) {
-      float u = u_final[t];
-      u = u != u ? 0.0f : fminf(1.0f, fmaxf(0.0f, u));
-      const double target = (double)u * total;
-      double base = 0.0;
-      int w = 0, last = 0;
-      for (; w < 16; ++w) {
-        if (part[w] > 0.0) last = w;
-        if (base + part[w] > target) break;
-        base += part[w];
+  const float* pr = probs + (i64)(a + cur) * ld_p;
+  const float* qr = DRAFT ? draft + (i64)(a + cur) * ld_q : nullptr;
+  // exclusive prefix of the runs' masses; the same additions give the whole and find the run
+  auto prefix = [&](int k, double before, double& v, double& up_to) {
+    v = k + lane < warps ? part_s[k + lane] : 0.0;
+    double s = v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const double n = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += n;
+    }
+    up_to = before + s;
+    return __shfl_sync(0xffffffffu, up_to, 31);
+  };
+  double total = 0.0, base = 0.0, v, up_to;
+  int w0 = -1, last = -1;      // the run that holds the draw, the last run with a weight
+  for (int k = 0; k < warps; k += 32) total = prefix(k, total, v, up_to);
+  int pick = -1;
+  if (total > 0.0) {
+    float u = u_final[t];
+    u = u != u ? 0.0f : fminf(1.0f, fmaxf(0.0f, u));
+    double target = (double)u * total, before = 0.0;
+    for (int k = 0; k < warps && w0 < 0; k += 32) {
+      const double next_before = prefix(k, before, v, up_to);
+      const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && up_to > target), some = __ballot_sync(0xffffffffu, v > 0.0);
+      if (over | some) {
+        const int l = over ? __ffs(over) - 1 : 31 - __clz(some);
+        (over ? w0 : last) = k + l;
+        base = __shfl_sync(0xffffffffu, up_to - v, l);
       }
-      if (w == 16) { w = last; base = 0.0; for (int k = 0; k < last; ++k) base += part[k]; }
-      for (int i0 = w * seg; i0 < min(cols, (w + 1) * seg); i0 += 32) {
-        const double r = i0 + lane < min(cols, (w + 1) * seg) ? left(i0 + lane) : 0.0;
+      before = next_before;
+    }
+    if (w0 < 0) { w0 = last; target = INFINITY; }      // nothing exceeds it: the last weight of all
+    const i64 end = min((i64)cols, (i64)(w0 + 1) * run);
+    bool found = false;
+    for (i64 i0 = (i64)w0 * run + lane; i0 - lane < end && !found; i0 += 32 * BATCH) {
+      float p[BATCH], q[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const bool in = i0 + k * 32 < end;
+        p[k] = in ? pr[i0 + k * 32] : 0.0f;
+        q[k] = DRAFT && tries && in ? qr[i0 + k * 32] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const double r = left((int)i0 + k * 32, p[k], q[k], tries);
         double s = r;
         for (int o = 1; o < 32; o <<= 1) {
-          const double v = __shfl_up_sync(0xffffffffu, s, o);
-          if (lane >= o) s += v;
+          const double n = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += n;
         }
         const unsigned over = __ballot_sync(0xffffffffu, r > 0.0 && base + s > target), some = __ballot_sync(0xffffffffu, r > 0.0);
-        if (over) { pick = i0 + __ffs(over) - 1; break; }
-        if (some) pick = i0 + 31 - __clz(some);
+        if (!found) {
+          const int at = (int)(i0 - lane) + k * 32;
+          if (over) { pick = at + __ffs(over) - 1; found = true; }
+          else if (some) pick = at + 31 - __clz(some);
+        }
         base += __shfl_sync(0xffffffffu, s, 31);
       }
     }
-    for (int i = lane; i < len; i += 32) {
-      path[(i64)t * max_path + i] = path_s[i];
-      tokens[(i64)t * max_path + i] = i + 1 < len ? tok_s[path_s[i + 1]] : pick;
-    }
-    if (lane == 0) n_path[t] = len;
   }
+  for (int i = lane; i < max_path; i += 32) {
+    my_path[i] = i < len ? path_s[i] : -1;
+    my_tokens[i] = i + 1 < len ? tok_s[path_s[i + 1]] : i + 1 == len ? pick : -1;
+  }
+  if (lane == 0) n_path[t] = len;
 }
 
 // ---- commit ---------------------------------------------------------------------------------------------------------
-// The K / V rows of node path[i] (i >= 1) move from position ctx + path[i] to ctx + i, 16 bytes a thread, in the order of
-// the path.  A path ascends, so path[i] >= i and no row is overwritten before it has been read.
+// The K / V rows of node path[i] (i >= 1) move from position ctx + path[i] to ctx + i, 16 bytes a thread, eight nodes at a
+// time: their look-ups, then their loads, then their stores.  A path ascends, so path[j] > i for j > i: a row that is
+// written was read before, in this round or an earlier one.  Bound: HBM for many sequences, two dependent trips for one.
 __global__ void __launch_bounds__(256) kv_commit_kernel(uint4* __restrict__ kc, uint4* __restrict__ vc, i64 layer_stride, i64 num_pages,
                                                         const uint32_t* __restrict__ block_table, const int* __restrict__ slots,
                                                         const int* __restrict__ ctxs, const int* __restrict__ path, const int* __restrict__ n_path,
@@ -194,34 +415,94 @@ __global__ void __launch_bounds__(256) kv_commit_kernel(uint4* __restrict__ kc, 
                                                         int* __restrict__ new_ctx, int* __restrict__ status) {
   pdl_wait();
   pdl_trigger();
-  const int t = blockIdx.y, slot = slots[t], ctx = ctxs[t];
+  const int t = blockIdx.y, slot = slots[t], ctx = ctxs[t], n = min(n_path[t], max_path);
   if (slot < 0 || ctx < 0) return;
-  const int n = min(n_path[t], max_path);
-  const i64 per = (i64)layers * kv_heads * chunks;
-  const i64 at = (i64)blockIdx.x * 256 + threadIdx.x;
+  const int per = layers * kv_heads * chunks;
+  const int at = (int)blockIdx.x * 256 + threadIdx.x;
   if (at == 0 && new_ctx) new_ctx[t] = ctx + max(n, 0);
   if (at >= 2 * per) return;
-  const i64 e = at % per;
-  uint4* cache = (at < per ? kc : vc) + e / ((i64)kv_heads * chunks) * layer_stride;
-  const int head = (int)(e / chunks % kv_heads), c = (int)(e % chunks);
+  const int e = at < per ? at : at - per, lh = e / chunks, c = e - lh * chunks, layer = lh / kv_heads, head = lh - layer * kv_heads;
+  uint4* cache = (at < per ? kc : vc) + layer * layer_stride + (i64)head * page_tokens * chunks + c;
+  const i64 page_stride = (i64)kv_heads * page_tokens * chunks;
+  const uint32_t* bt = block_table + (i64)slot * mbps;
+  const i64 cover = (i64)mbps * page_tokens;
+  constexpr int BATCH = 8;
   int before = 0;
-  for (int i = 1; i < n; ++i) {
-    const int node = path[(i64)t * max_path + i];
-    const i64 src = (i64)ctx + node, dst = (i64)ctx + i;
-    const bool ok = node > before && src < (i64)mbps * page_tokens;
-    uint32_t ps = 0, pd = 0;
-    if (ok) { ps = block_table[(i64)slot * mbps + src / page_tokens]; pd = block_table[(i64)slot * mbps + dst / page_tokens]; }
-    if (!ok || ps >= (uint64_t)num_pages || pd >= (uint64_t)num_pages) {      // not a path, or past the table or the cache: stop here
+  for (int i0 = 1; i0 < n; i0 += BATCH) {
+    int node[BATCH];
+    i64 from[BATCH], to[BATCH];
+    uint4 v[BATCH];
+    int good = 0;      // entries of this round that belong to a path
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) node[k] = i0 + k < n ? path[(i64)t * max_path + i0 + k] : -1;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const i64 src = (i64)ctx + node[k], dst = (i64)ctx + i0 + k;
+      const bool in = node[k] >= i0 + k && src < cover;
+      const uint32_t s32 = in ? (uint32_t)src : 0u, d32 = in ? (uint32_t)dst : 0u, pt = (uint32_t)page_tokens;
+      const uint32_t ps = in ? bt[s32 / pt] : 0xffffffffu, pd = in ? bt[d32 / pt] : 0xffffffffu;
+      const bool ok = ps < (uint64_t)num_pages && pd < (uint64_t)num_pages && node[k] > (k ? node[k ? k - 1 : 0] : before);
+      from[k] = ok ? ps * page_stride + (i64)(s32 % pt) * chunks : -1;
+      to[k] = ok ? pd * page_stride + (i64)(d32 % pt) * chunks : -1;
+      if (ok && good == k) good = k + 1;
+    }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (k < good) v[k] = cache[from[k]];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (k < good && from[k] != to[k]) cache[to[k]] = v[k];
+    if (good < min(BATCH, n - i0)) {      // not a path, or past the table or the cache: the moves end here
       if (e == 0 && status) atomicExch(status, WKB_STATUS_KV_POS_RANGE);
       return;
     }
-    before = node;
-    if (node != i) {
-      const i64 from = (((i64)ps * kv_heads + head) * page_tokens + src % page_tokens) * chunks + c;
-      const i64 to = (((i64)pd * kv_heads + head) * page_tokens + dst % page_tokens) * chunks + c;
-      cache[to] = cache[from];
-    }
+    before = node[BATCH - 1];
   }
+}
+
+// A launch whose blocks form clusters of `ctas`, as a programmatic dependent like launch_pdl's.
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned block, int ctas, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// A row's columns over the CTAs of a cluster and the registers of their threads: clusters grow until two CTAs per SM are
+// at work (small batches) and a thread holds at most 32 columns (large vocabularies), or at 8.
+constexpr i64 PROBS_MAX = 8 * 64 * (i64)PT;
+struct ProbsShape {
+  int ctas, regs;
+};
+static ProbsShape probs_shape(i64 rows, i64 cols) {
+  ProbsShape s{1, 4};
+  while (s.ctas < 8 && (cols > (i64)s.ctas * 32 * PT || (rows * s.ctas < 2 * WKB_SM_COUNT && cols > (i64)s.ctas * 4 * PT))) s.ctas *= 2;
+  while (s.regs < 64 && (i64)s.ctas * s.regs * PT < cols) s.regs *= 2;
+  return s;
+}
+template <typename T>
+static int launch_probs(const ProbsShape& s, const T* x, i64 ld, const float* temperature, float* out, i64 ld_out, i64 rows, i64 cols, cudaStream_t st) {
+  if (cols > PROBS_MAX) return (int)launch_pdl(token_probs_wide_kernel<T>, (unsigned)rows, 512, 0, st, x, ld, temperature, out, ld_out, (int)cols);
+  auto kern = s.regs == 4 ? token_probs_kernel<T, 4> : s.regs == 8 ? token_probs_kernel<T, 8> : s.regs == 16 ? token_probs_kernel<T, 16>
+            : s.regs == 32 ? token_probs_kernel<T, 32> : token_probs_kernel<T, 64>;
+  return (int)launch_cluster(kern, (unsigned)(rows * s.ctas), PT, s.ctas, st, x, ld, temperature, out, ld_out, (int)cols);
+}
+// CTAs of a tree's cluster: as many as keep two per SM at work, each with 2048 columns at least.
+static int verify_ctas(i64 n_trees, i64 cols) {
+  int c = 1;
+  while (c < 8 && n_trees * c < 2 * WKB_SM_COUNT && cols > (i64)c * 2048) c *= 2;
+  return c;
 }
 
 }  // namespace verify
@@ -235,8 +516,10 @@ extern "C" {
 
 int wkb_token_probs(const void* logits, int in_dtype, i64 ld, const float* temperature_or_null, float* out, i64 ld_out, i64 rows, i64 cols, void* stream) {
   if (rows <= 0 || cols <= 0) return 0;
-  if ((in_dtype != 0 && in_dtype != 1) || ld < cols || ld_out < cols || cols > 0x7fffff00 || rows > 0x7fffffff) return (int)cudaErrorInvalidValue;
-  return (int)launch_pdl(verify::token_probs_kernel, (unsigned)rows, 512, 0, as_stream(stream), logits, in_dtype, ld, temperature_or_null, out, ld_out, cols);
+  if ((in_dtype != 0 && in_dtype != 1) || ld < cols || ld_out < cols || cols > 0x7fffff00 || rows > 0x7fffffff / 8) return (int)cudaErrorInvalidValue;
+  const verify::ProbsShape s = verify::probs_shape(rows, cols);
+  if (in_dtype == 0) return verify::launch_probs<float>(s, static_cast<const float*>(logits), ld, temperature_or_null, out, ld_out, rows, cols, as_stream(stream));
+  return verify::launch_probs<__nv_bfloat16>(s, static_cast<const __nv_bfloat16*>(logits), ld, temperature_or_null, out, ld_out, rows, cols, as_stream(stream));
 }
 
 int wkb_tree_verify(const float* probs, i64 ld_p, const float* draft_or_null, i64 ld_q, const int* token, const int* parent, const int* tree_row0,
@@ -245,8 +528,11 @@ int wkb_tree_verify(const float* probs, i64 ld_p, const float* draft_or_null, i6
   if (n_trees <= 0) return 0;
   if (rows < 0 || rows > 0x7fffffff || n_trees > 0x7fffffff || cols <= 0 || cols > 0x7fffff00 || ld_p < cols || (draft_or_null && ld_q < cols)) return (int)cudaErrorInvalidValue;
   if (max_nodes < 1 || max_nodes > verify::MAX_NODES || max_path < 1 || max_path > max_nodes) return (int)cudaErrorInvalidValue;
-  return (int)launch_pdl(verify::tree_verify_kernel, (unsigned)n_trees, 512, 0, as_stream(stream), probs, ld_p, draft_or_null, ld_q, token, parent, tree_row0,
-                         (int)rows, (int)cols, (int)max_nodes, u_node, u_final, path, tokens, n_path, (int)max_path);
+  const int ctas = verify::verify_ctas(n_trees, cols);
+  if (n_trees > 0x7fffffff / ctas) return (int)cudaErrorInvalidValue;
+  auto kern = draft_or_null ? verify::tree_verify_kernel<true> : verify::tree_verify_kernel<false>;
+  return (int)verify::launch_cluster(kern, (unsigned)(n_trees * ctas), verify::PT, ctas, as_stream(stream), probs, ld_p, draft_or_null, ld_q, token, parent,
+                                     tree_row0, (int)rows, (int)cols, (int)max_nodes, u_node, u_final, path, tokens, n_path, (int)max_path);
 }
 
 int wkb_paged_kv_commit(void* kcache, void* vcache, i64 layers, i64 layer_stride, i64 num_pages, const uint32_t* block_table, const int* tree_slot,
@@ -260,7 +546,7 @@ int wkb_paged_kv_commit(void* kcache, void* vcache, i64 layers, i64 layer_stride
   if (layers > 1 && layer_stride < num_pages * kv_heads * page_tokens * head_dim) return (int)cudaErrorInvalidValue;
   if (((((uintptr_t)kcache) | ((uintptr_t)vcache)) & 15) != 0 || layer_stride % 8 != 0) return (int)cudaErrorMisalignedAddress;
   const i64 threads = 2 * layers * kv_heads * (head_dim / 8), blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffff) return (int)cudaErrorInvalidValue;
+  if (layers > 0x7fffffff / 2 / (head_dim / 8) / kv_heads) return (int)cudaErrorInvalidValue;
   int* status = gemm_status_word();
   if (!status) return (int)cudaErrorMemoryAllocation;
   return (int)launch_pdl(verify::kv_commit_kernel, dim3((unsigned)blocks, (unsigned)n_trees), 256, 0, as_stream(stream), (uint4*)kcache, (uint4*)vcache,
