@@ -14,7 +14,7 @@ constexpr int MAX_NODES = 256;
 __device__ __forceinline__ float logit(const float* x, int i) { return x[i]; }
 __device__ __forceinline__ float logit(const __nv_bfloat16* x, int i) { return bf16_bits_to_f32(reinterpret_cast<const u16*>(x)[i]); }
 // log2(e) / t, finite and not 0, so that the maximum keeps weight 1 and a token that is ruled out weight 0
-__device__ __forceinline__ float exponent_scale(float t) { return fmaxf(fminf(1.4426950408889634f / t, 3.402823466e+38f), 1e-37f); }
+__device__ __forceinline__ float exponent_scale(float t) { return t != t ? t : fmaxf(fminf(1.4426950408889634f / t, 3.402823466e+38f), 1e-37f); }
 
 // Rows wider than a cluster's registers: one CTA per row, three passes (the second and third mostly from L2).
 template <typename T>
@@ -65,14 +65,6 @@ __global__ void __launch_bounds__(512) token_probs_wide_kernel(const T* __restri
   }
 }
 
-// Two floats per CTA travel through the cluster: `mine` is published, `all` collects every CTA's.
-__device__ __forceinline__ float2 cluster_get(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  float2 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote) : "memory");
-  return v;
-}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -91,100 +83,104 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)
 constexpr int PT = 512;      // threads of a CTA
 
 // A row is a cluster's: each CTA keeps its E * 512 columns in registers, so the logits are read once and the probabilities
-// written once (HBM is the bound).  The CTAs trade (maximum, sum relative to it) through shared memory.  Element loads are
-// 4 (2) bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no more than that.
+// written once (HBM is the bound).  Every warp reduces its columns to (maximum, sum relative to it) and puts the pair into
+// every CTA's table; one cluster barrier later each warp adds up the whole table, so that nothing else is waited for
+// between the last load and the first store (block-wide reductions and a second barrier cost 65 us instead of 55 for
+// 1024 x 32000).  Element loads are 4 (2) bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no
+// more than that.
 template <typename T, int E>
-__global__ void __launch_bounds__(PT) token_probs_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature, float* __restrict__ out,
-                                                         i64 ld_out, int cols) {
+__global__ void __launch_bounds__(PT, E > 32 ? 1 : 2) token_probs_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature,
+                                                                         float* __restrict__ out, i64 ld_out, int cols) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float red[PT / 32];
-  __shared__ float2 mine[2];
+  __shared__ float2 table[8 * PT / 32];
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // awaited before the first store to another CTA: it has begun
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const i64 row = blockIdx.x / size;
-  const int first = (int)rank * E * PT + threadIdx.x;
-  const T* xr = x + row * ld;
-  const float temp = temperature ? temperature[row] : 1.0f;
+  const int first = (int)rank * E * PT + threadIdx.x, mine = cols - first;      // column e * PT behind `first` exists below `mine`
+  const T* xr = x + row * ld + first;
+  float* const o = out + row * ld_out + first;
   float v[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = first + e * PT;
-    v[e] = i < cols ? logit(xr, i) : -INFINITY;
-  }
-  float m = -INFINITY;
-  bool nan = temp != temp;
+  for (int e = 0; e < E; ++e) v[e] = e * PT < mine ? logit(xr, e * PT) : -INFINITY;
+  const float temp = temperature ? temperature[row] : 1.0f;
+  const bool cold = temp <= 0.0f;      // alike in all CTAs of the row
+  const float scale = exponent_scale(temp);
+  float m = -INFINITY, second;         // second: the sum, or the column of the maximum
 #pragma unroll
-  for (int e = 0; e < E; ++e) { m = fmaxf(m, v[e]); nan |= v[e] != v[e]; }
-  m = warp_max(m);
-  if (lane == 0) red[warp] = m;
-  nan = __syncthreads_or(nan);
-#pragma unroll
-  for (int w = 0; w < PT / 32; ++w) m = fmaxf(m, red[w]);
-  if (temp <= 0.0f) {      // (a branch that all CTAs of the row take alike)
-    // greedy: the lowest column of the row's maximum
-    if (threadIdx.x == 0) mine[0] = make_float2(m, nan ? 1.0f : 0.0f);
-    cluster_sync();
-    for (uint32_t k = 0; k < size; ++k) {
-      const float2 o = cluster_get(smem_addr(&mine[0]), k);
-      m = fmaxf(m, o.x);
-      nan |= o.y != 0.0f;
-    }
+  for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+  float base;
+  if (cold) {
     int at = 0x7fffffff;
+    bool nan = false;
 #pragma unroll
-    for (int e = E - 1; e >= 0; --e)
-      if (v[e] == m && first + e * PT < cols) at = first + e * PT;
-    for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-    __syncthreads();
-    if (lane == 0) red[warp] = __int_as_float(at);
-    __syncthreads();
-    for (int w = 0; w < PT / 32; ++w) at = min(at, __float_as_int(red[w]));
-    if (threadIdx.x == 0) mine[1] = make_float2(__int_as_float(at), 0.0f);
-    cluster_sync();
-    for (uint32_t k = 0; k < size; ++k) at = min(at, __float_as_int(cluster_get(smem_addr(&mine[1]), k).x));
-    if (m == -INFINITY) at = -1;      // every token is ruled out
+    for (int e = E - 1; e >= 0; --e) {
+      if (v[e] == m && e * PT < mine) at = first + e * PT;
+      nan |= v[e] != v[e];
+    }
+    for (int k = 16; k > 0; k >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, m, k);
+      const int oa = __shfl_xor_sync(0xffffffffu, at, k);
+      if (om > m || (om == m && oa < at)) { m = om; at = oa; }
+    }
+    if (__any_sync(0xffffffffu, nan)) m = NAN;
+    base = 0.0f;
+    second = __int_as_float(at);
+  } else {
+    base = m == -INFINITY ? 0.0f : m;
+    second = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int i = first + e * PT;
-      if (i < cols) out[row * ld_out + i] = nan ? NAN : i == at ? 1.0f : 0.0f;
+      v[e] = exp2f((v[e] - base) * scale);      // a NaN spoils the sum and with it the row
+      second += v[e];
     }
-    cluster_sync();      // no CTA leaves while another may read its numbers
+    const float mw = warp_max(m);
+    second = warp_sum(m == -INFINITY ? second : second * exp2f((m - mw) * scale));
+    m = mw;
+  }
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (lane < (int)size) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(&table[rank * (PT / 32) + warp])), "r"(lane));
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(m), "f"(second) : "memory");
+  }
+  cluster_sync();
+  const int entries = (int)size * (PT / 32);
+  if (cold) {
+    bool nan = false;
+    float top = -INFINITY;
+    int at = 0x7fffffff;
+    for (int k = lane; k < entries; k += 32) {
+      const float2 p = table[k];
+      nan |= p.x != p.x;
+      if (p.x > top || (p.x == top && __float_as_int(p.y) < at)) { top = p.x; at = __float_as_int(p.y); }
+    }
+    for (int k = 16; k > 0; k >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, top, k);
+      const int oa = __shfl_xor_sync(0xffffffffu, at, k);
+      if (om > top || (om == top && oa < at)) { top = om; at = oa; }
+    }
+    if (top == -INFINITY) at = -1;      // every token is ruled out
+    nan = __any_sync(0xffffffffu, nan);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e * PT < mine) o[e * PT] = nan ? NAN : first + e * PT == at ? 1.0f : 0.0f;
     return;
   }
-  const float scale = exponent_scale(temp);
-  const float base = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f;
+  float top = -INFINITY, l = 0.0f;
+  for (int k = lane; k < entries; k += 32) top = fmaxf(top, table[k].x);
+  top = warp_max(top);
+  for (int k = lane; k < entries; k += 32) {
+    const float2 p = table[k];
+    l += p.x == -INFINITY ? p.y : p.y * exp2f((p.x - top) * scale);
+  }
+  l = warp_sum(l);
+  const float own = (base - top) * scale;      // this thread's exponentials are relative to its own maximum
+  const float f = top == -INFINITY ? (l == l ? 0.0f : NAN) : (mine > 0 && base <= top ? exp2f(own) : 1.0f) / l;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    v[e] = exp2f((v[e] - base) * scale);
-    sum += v[e];
-  }
-  sum = warp_sum(sum);
-  __syncthreads();
-  if (lane == 0) red[warp] = sum;
-  __syncthreads();
-  sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < PT / 32; ++w) sum += red[w];
-  if (threadIdx.x == 0) mine[0] = make_float2(nan ? NAN : m, sum);      // a NaN spoils the row
-  cluster_sync();
-  float m_all = -INFINITY, l = 0.0f;
-  for (uint32_t k = 0; k < size; ++k) {
-    const float2 o = cluster_get(smem_addr(&mine[0]), k);
-    nan |= o.x != o.x;
-    m_all = fmaxf(m_all, o.x);
-  }
-  for (uint32_t k = 0; k < size; ++k) {
-    const float2 o = cluster_get(smem_addr(&mine[0]), k);
-    if (o.x != -INFINITY) l += o.y * exp2f((o.x - m_all) * scale);
-  }
-  const float f = nan ? NAN : m == -INFINITY ? 0.0f : exp2f((m - m_all) * scale) / l;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = first + e * PT;
-    if (i < cols) out[row * ld_out + i] = v[e] * f;
-  }
-  cluster_sync();
+  for (int e = 0; e < E; ++e)
+    if (e * PT < mine) o[e * PT] = v[e] * f;
 }
 
 // ---- verification ---------------------------------------------------------------------------------------------------
