@@ -186,9 +186,13 @@ __global__ void __launch_bounds__(PT, E > 32 ? 1 : 2) token_probs_kernel(const T
 // ---- verification ---------------------------------------------------------------------------------------------------
 __device__ __forceinline__ double weight(float v) { return v > 0.0f && v <= 3.402823466e+38f ? (double)v : 0.0; }
 
+// 4 bytes of global memory into this thread's cell, or 0 where `have` is 0; complete after cp.async.wait_all
+__device__ __forceinline__ void fetch4(float* cell, const float* src, uint32_t have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(cell)), "l"(src), "r"(have) : "memory");
+}
 // What the leader asks of its cluster: the masses that are left of node `row` after `tries` rejections.
-struct Ask {
-  int row, tries, last;
+struct alignas(16) Ask {
+  int row, tries, last, pad;
 };
 // One cluster per tree.  The walk needs two numbers of each node, p and q of its token in its parent's rows: the leading
 // CTA gathers them for all nodes at once, and its first warp walks in shared memory.  Only the mass that is left after a
@@ -196,8 +200,9 @@ struct Ask {
 // columns per warp of the cluster; the row is read from HBM once and the run that holds the draw a second time, from L2.
 // The leader alone decides, so every CTA takes the same steps.  Sums are in a fixed order.  Bound: the latency of the four
 // dependent trips to memory for a few trees, the rows' bytes for many.
+constexpr int HOLD = 16;
 template <bool DRAFT>
-__global__ void __launch_bounds__(PT) tree_verify_kernel(const float* __restrict__ probs, i64 ld_p, const float* __restrict__ draft, i64 ld_q,
+__global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restrict__ probs, i64 ld_p, const float* __restrict__ draft, i64 ld_q,
                                                          const int* __restrict__ token, const int* __restrict__ parent, const int* __restrict__ row0,
                                                          int rows, int cols, int max_nodes, const float* __restrict__ u_node,
                                                          const float* __restrict__ u_final, int* __restrict__ path, int* __restrict__ tokens,
@@ -208,6 +213,8 @@ __global__ void __launch_bounds__(PT) tree_verify_kernel(const float* __restrict
   __shared__ float p_s[MAX_NODES], q_s[MAX_NODES], u_s[MAX_NODES];
   __shared__ double z_s[MAX_NODES + 1], part_s[8 * PT / 32];
   __shared__ Ask ask;
+  extern __shared__ float cells[];      // [p, q][HOLD][PT]
+  __shared__ int walk_s[3], pick_s[2];
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int t = blockIdx.x / size, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)size * (PT / 32);
   const int a = min(max(row0[t], 0), rows), nodes = min(min(max(row0[t + 1], a), rows) - a, max_nodes);
@@ -251,7 +258,12 @@ __global__ void __launch_bounds__(PT) tree_verify_kernel(const float* __restrict
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(of));
     return r;
   };
-  constexpr int BATCH = 8;      // loads in flight per thread
+  // A thread's columns go through its own cells of shared memory, HOLD at a time: all copies in flight together, and
+  // rolled loops (unrolled, fetching the instructions took longer than fetching the columns), and a run of no more
+  // than that stays there, so that the passes after a node's first read nothing.
+  const bool holds = run <= 32 * HOLD;
+  float* const cell = cells + threadIdx.x;
+  int held = -1;
   int cur = 0, tries = 0, len = 1, next = 1;      // the walk, of the leader's first warp
   bool summed = false;
   if (rank == 0 && warp == 0 && lane == 0) { path_s[0] = 0; z_s[0] = 1.0; }
@@ -291,9 +303,7 @@ __global__ void __launch_bounds__(PT) tree_verify_kernel(const float* __restrict
     }
     cluster_sync();
     Ask now;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(now.row) : "r"(remote(&ask.row, 0)) : "memory");
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(now.tries) : "r"(remote(&ask.tries, 0)) : "memory");
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(now.last) : "r"(remote(&ask.last, 0)) : "memory");
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(now.row), "=r"(now.tries), "=r"(now.last), "=r"(now.pad) : "r"(remote(&ask, 0)) : "memory");
     if (rank != 0) {
       for (int k = threadIdx.x; k < now.tries; k += PT) {
         if (DRAFT) asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(z_s[k]) : "r"(remote(&z_s[k], 0)) : "memory");
@@ -304,21 +314,53 @@ __global__ void __launch_bounds__(PT) tree_verify_kernel(const float* __restrict
     const float* pr = probs + (i64)now.row * ld_p;
     const float* qr = DRAFT ? draft + (i64)now.row * ld_q : nullptr;
     {
-      const int g = (int)rank * (PT / 32) + warp, end = min((i64)cols, (i64)(g + 1) * run);
-      double s = 0.0;
-      for (i64 i0 = (i64)g * run + lane; i0 - lane < end; i0 += 32 * BATCH) {
-        float p[BATCH], q[BATCH];
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          const bool in = i0 + k * 32 < end;
-          p[k] = in ? pr[i0 + k * 32] : 0.0f;
-          q[k] = DRAFT && now.tries && in ? qr[i0 + k * 32] : 0.0f;
+      const int g = (int)rank * (PT / 32) + warp, end = (int)min((i64)cols, (i64)(g + 1) * run);
+      double s[4] = {0.0, 0.0, 0.0, 0.0};
+      for (i64 i0 = (i64)g * run + lane; i0 - lane < end; i0 += 32 * HOLD) {
+        if (!holds || held != now.row) {
+#pragma unroll 4
+          for (int k = 0; k < HOLD; ++k) {
+            const i64 i = i0 + k * 32;
+            const uint32_t have = i < end ? 4u : 0u;      // the cell of a column behind the run is filled with 0
+            fetch4(cell + k * PT, pr + (have ? i : 0), have);
+            if (DRAFT) fetch4(cell + (HOLD + k) * PT, qr + (have ? i : 0), have);
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
         }
+        const int n = min(HOLD, (int)((end - (i0 - lane) + 31) >> 5));
+        // four sums: an f64 operation's latency is what a column costs
+#pragma unroll 1
+        for (int k = 0; k < n; k += 4) {
+          double r[4];
 #pragma unroll
-        for (int k = 0; k < BATCH; ++k) s += left((int)i0 + k * 32, p[k], q[k], now.tries);
+          for (int e = 0; e < 4; ++e) r[e] = weight(cell[(k + e) * PT]);
+          if (DRAFT) {
+            double w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = weight(cell[(HOLD + k + e) * PT]);
+#pragma unroll 1
+            for (int j = 0; j < now.tries; ++j) {
+              const double z = z_s[j];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) r[e] = fmax(r[e] - z * w[e], 0.0);
+            }
+          } else {
+#pragma unroll 1
+            for (int j = 0; j < now.tries; ++j) {
+              const int at = tried_s[j] - (int)i0 - k * 32;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (at == e * 32) r[e] = 0.0;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[e] += r[e];
+        }
       }
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote(&part_s[g], 0)), "d"(s) : "memory");
+      held = now.row;
+      double sum = (s[0] + s[1]) + (s[2] + s[3]);
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote(&part_s[g], 0)), "d"(sum) : "memory");
     }
     cluster_sync();
     if (now.last) break;
@@ -331,68 +373,75 @@ __global__ void __launch_bounds__(PT) tree_verify_kernel(const float* __restrict
       __syncwarp();
     }
   }
-  if (rank != 0 || warp != 0) return;
+  if (rank != 0) return;
+  if (threadIdx.x == 0) { walk_s[0] = cur; walk_s[1] = tries; walk_s[2] = len; pick_s[0] = 0x7fffffff; pick_s[1] = -1; }
+  __syncthreads();
+  cur = walk_s[0]; tries = walk_s[1]; len = walk_s[2];
   // inverse CDF over what is left: the lowest column whose running mass exceeds u * mass, the last one with a weight otherwise
   const float* pr = probs + (i64)(a + cur) * ld_p;
   const float* qr = DRAFT ? draft + (i64)(a + cur) * ld_q : nullptr;
-  // exclusive prefix of the runs' masses; the same additions give the whole and find the run
-  auto prefix = [&](int k, double before, double& v, double& up_to) {
-    v = k + lane < warps ? part_s[k + lane] : 0.0;
-    double s = v;
-    for (int o = 1; o < 32; o <<= 1) {
-      const double n = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += n;
-    }
-    up_to = before + s;
-    return __shfl_sync(0xffffffffu, up_to, 31);
-  };
-  double total = 0.0, base = 0.0, v, up_to;
-  int w0 = -1, last = -1;      // the run that holds the draw, the last run with a weight
-  for (int k = 0; k < warps; k += 32) total = prefix(k, total, v, up_to);
+  // the runs' masses, up to four neighbours a lane: running sums, the whole, and the first run that exceeds the target
+  constexpr int PER = 8 * (PT / 32) / 32;
+  double v[PER], own = 0.0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    v[k] = lane * PER + k < warps ? part_s[lane * PER + k] : 0.0;
+    own += v[k];
+  }
+  double up_to = own;
+  for (int o = 1; o < 32; o <<= 1) {
+    const double n = __shfl_up_sync(0xffffffffu, up_to, o);
+    if (lane >= o) up_to += n;
+  }
+  const double total = __shfl_sync(0xffffffffu, up_to, 31);
   int pick = -1;
   if (total > 0.0) {
     float u = u_final[t];
     u = u != u ? 0.0f : fminf(1.0f, fmaxf(0.0f, u));
-    double target = (double)u * total, before = 0.0;
-    for (int k = 0; k < warps && w0 < 0; k += 32) {
-      const double next_before = prefix(k, before, v, up_to);
-      const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && up_to > target), some = __ballot_sync(0xffffffffu, v > 0.0);
-      if (over | some) {
-        const int l = over ? __ffs(over) - 1 : 31 - __clz(some);
-        (over ? w0 : last) = k + l;
-        base = __shfl_sync(0xffffffffu, up_to - v, l);
+    double target = (double)u * total, base = up_to - own, before = 0.0;      // before: the mass in front of the run that this lane offers
+    int offer = -1, last = -1;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if (v[k] > 0.0 && offer < 0) {
+        last = lane * PER + k;
+        before = base;
+        if (k + 1 == PER ? up_to > target : base + v[k] > target) offer = last;
       }
-      before = next_before;
+      base += v[k];
     }
-    if (w0 < 0) { w0 = last; target = INFINITY; }      // nothing exceeds it: the last weight of all
+    const unsigned over = __ballot_sync(0xffffffffu, offer >= 0), some = __ballot_sync(0xffffffffu, last >= 0);
+    const int from = over ? __ffs(over) - 1 : 31 - __clz(some);
+    const int w0 = __shfl_sync(0xffffffffu, over ? offer : last, from);
+    base = __shfl_sync(0xffffffffu, before, from);
+    if (!over) target = INFINITY;      // nothing exceeds it: the last weight of all
+    // the whole CTA goes over that run, 32 columns a warp at a time
     const i64 end = min((i64)cols, (i64)(w0 + 1) * run);
-    bool found = false;
-    for (i64 i0 = (i64)w0 * run + lane; i0 - lane < end && !found; i0 += 32 * BATCH) {
-      float p[BATCH], q[BATCH];
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const bool in = i0 + k * 32 < end;
-        p[k] = in ? pr[i0 + k * 32] : 0.0f;
-        q[k] = DRAFT && tries && in ? qr[i0 + k * 32] : 0.0f;
+    for (i64 i0 = (i64)w0 * run; i0 < end; i0 += PT) {
+      const i64 i = i0 + threadIdx.x;
+      const double r = i < end ? left((int)i, pr[i], DRAFT && tries ? qr[i] : 0.0f, tries) : 0.0;
+      double sum = r;
+      for (int o = 1; o < 32; o <<= 1) {
+        const double n = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += n;
       }
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const double r = left((int)i0 + k * 32, p[k], q[k], tries);
-        double s = r;
-        for (int o = 1; o < 32; o <<= 1) {
-          const double n = __shfl_up_sync(0xffffffffu, s, o);
-          if (lane >= o) s += n;
-        }
-        const unsigned over = __ballot_sync(0xffffffffu, r > 0.0 && base + s > target), some = __ballot_sync(0xffffffffu, r > 0.0);
-        if (!found) {
-          const int at = (int)(i0 - lane) + k * 32;
-          if (over) { pick = at + __ffs(over) - 1; found = true; }
-          else if (some) pick = at + 31 - __clz(some);
-        }
-        base += __shfl_sync(0xffffffffu, s, 31);
+      __syncthreads();
+      if (lane == 31) part_s[warp] = sum;
+      __syncthreads();
+      double before = base;
+      for (int w = 0; w < PT / 32; ++w) {
+        if (w == warp) sum += before;
+        before += part_s[w];
+      }
+      base = before;
+      if (r > 0.0) {
+        if (sum > target) atomicMin(&pick_s[0], (int)i);
+        atomicMax(&pick_s[1], (int)i);
       }
     }
+    __syncthreads();
+    pick = pick_s[0] != 0x7fffffff ? pick_s[0] : pick_s[1];
   }
+  if (warp != 0) return;
   for (int i = lane; i < max_path; i += 32) {
     my_path[i] = i < len ? path_s[i] : -1;
     my_tokens[i] = i + 1 < len ? tok_s[path_s[i + 1]] : i + 1 == len ? pick : -1;
@@ -458,10 +507,11 @@ __global__ void __launch_bounds__(256) kv_commit_kernel(uint4* __restrict__ kc, 
 
 // A launch whose blocks form clusters of `ctas`, as a programmatic dependent like launch_pdl's.
 template <typename... KArgs, typename... Args>
-static cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned block, int ctas, cudaStream_t st, Args&&... args) {
+static cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned block, int smem, int ctas, cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -492,7 +542,7 @@ static int launch_probs(const ProbsShape& s, const T* x, i64 ld, const float* te
   if (cols > PROBS_MAX) return (int)launch_pdl(token_probs_wide_kernel<T>, (unsigned)rows, 512, 0, st, x, ld, temperature, out, ld_out, (int)cols);
   auto kern = s.regs == 4 ? token_probs_kernel<T, 4> : s.regs == 8 ? token_probs_kernel<T, 8> : s.regs == 16 ? token_probs_kernel<T, 16>
             : s.regs == 32 ? token_probs_kernel<T, 32> : token_probs_kernel<T, 64>;
-  return (int)launch_cluster(kern, (unsigned)(rows * s.ctas), PT, s.ctas, st, x, ld, temperature, out, ld_out, (int)cols);
+  return (int)launch_cluster(kern, (unsigned)(rows * s.ctas), PT, 0, s.ctas, st, x, ld, temperature, out, ld_out, (int)cols);
 }
 // CTAs of a tree's cluster: as many as keep two per SM at work, each with 2048 columns at least.
 static int verify_ctas(i64 n_trees, i64 cols) {
@@ -527,7 +577,10 @@ int wkb_tree_verify(const float* probs, i64 ld_p, const float* draft_or_null, i6
   const int ctas = verify::verify_ctas(n_trees, cols);
   if (n_trees > 0x7fffffff / ctas) return (int)cudaErrorInvalidValue;
   auto kern = draft_or_null ? verify::tree_verify_kernel<true> : verify::tree_verify_kernel<false>;
-  return (int)verify::launch_cluster(kern, (unsigned)(n_trees * ctas), verify::PT, ctas, as_stream(stream), probs, ld_p, draft_or_null, ld_q, token, parent,
+  constexpr int SMEM = 2 * verify::HOLD * verify::PT * (int)sizeof(float);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (e != cudaSuccess) return (int)e;
+  return (int)verify::launch_cluster(kern, (unsigned)(n_trees * ctas), verify::PT, SMEM, ctas, as_stream(stream), probs, ld_p, draft_or_null, ld_q, token, parent,
                                      tree_row0, (int)rows, (int)cols, (int)max_nodes, u_node, u_final, path, tokens, n_path, (int)max_path);
 }
 
