@@ -84,7 +84,7 @@ def test_verify_refusals(L, over):
 
 
 @pytest.mark.parametrize("over,code", [(dict(n=65536), BAD), (dict(max_path=0), BAD), (dict(kvh=0), BAD), (dict(hd=4), BAD), (dict(hd=12), BAD), (dict(page=0), BAD), (dict(mbps=0), BAD),
-                                       (dict(pages=0), BAD), (dict(stride=1000), BAD), (dict(new_ctx=P + 64), BAD), (dict(k=P + 8), MISALIGNED), (dict(stride=(1 << 20) + 4), MISALIGNED)])
+                                       (dict(pages=0), BAD), (dict(stride=1000), BAD), (dict(pages=1 << 40, stride=1 << 56), BAD), (dict(new_ctx=P + 64), BAD), (dict(k=P + 8), MISALIGNED), (dict(stride=(1 << 20) + 4), MISALIGNED)])
 def test_commit_refusals(L, over, code):
     a = dict(k=P, layers=2, stride=1 << 20, pages=4, max_path=4, n=1, kvh=2, hd=64, page=16, mbps=4, new_ctx=None)
     a.update(over)

@@ -450,10 +450,11 @@ __global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restr
 }
 
 // ---- commit ---------------------------------------------------------------------------------------------------------
-// The K / V rows of node path[i] (i >= 1) move from position ctx + path[i] to ctx + i, 16 bytes a thread, eight nodes at a
-// time: their look-ups, then their loads, then their stores.  A path ascends, so path[j] > i for j > i: a row that is
+// The K / V rows of node path[i] (i >= 1) move from position ctx + path[i] to ctx + i, eight nodes at a time: their
+// look-ups, then for each 16 bytes of a token's rows in all layers the loads and the stores.  The grid is bounded, so that
+// the four dependent look-ups of a block are paid once for several of its elements.  A path ascends, so path[j] > i for j > i: a row that is
 // written was read before, in this round or an earlier one.  Bound: HBM for many sequences, two dependent trips for one.
-__global__ void __launch_bounds__(256) kv_commit_kernel(uint4* __restrict__ kc, uint4* __restrict__ vc, i64 layer_stride, i64 num_pages,
+__global__ void __launch_bounds__(256, 3) kv_commit_kernel(uint4* __restrict__ kc, uint4* __restrict__ vc, i64 layer_stride, i64 num_pages,
                                                         const uint32_t* __restrict__ block_table, const int* __restrict__ slots,
                                                         const int* __restrict__ ctxs, const int* __restrict__ path, const int* __restrict__ n_path,
                                                         int max_path, int layers, int kv_heads, int chunks, int page_tokens, int mbps,
@@ -462,21 +463,17 @@ __global__ void __launch_bounds__(256) kv_commit_kernel(uint4* __restrict__ kc, 
   pdl_trigger();
   const int t = blockIdx.y, slot = slots[t], ctx = ctxs[t], n = min(n_path[t], max_path);
   if (slot < 0 || ctx < 0) return;
-  const int per = layers * kv_heads * chunks;
-  const int at = (int)blockIdx.x * 256 + threadIdx.x;
-  if (at == 0 && new_ctx) new_ctx[t] = ctx + max(n, 0);
-  if (at >= 2 * per) return;
-  const int e = at < per ? at : at - per, lh = e / chunks, c = e - lh * chunks, layer = lh / kv_heads, head = lh - layer * kv_heads;
-  uint4* cache = (at < per ? kc : vc) + layer * layer_stride + (i64)head * page_tokens * chunks + c;
-  const i64 page_stride = (i64)kv_heads * page_tokens * chunks;
+  const int per = layers * kv_heads * chunks, at0 = (int)blockIdx.x * 256 + threadIdx.x;
+  if (at0 == 0 && new_ctx) new_ctx[t] = ctx + max(n, 0);
+  const uint32_t page_stride = (uint32_t)kv_heads * (uint32_t)page_tokens * (uint32_t)chunks;      // a slab is no more than 2^32 units
   const uint32_t* bt = block_table + (i64)slot * mbps;
   const i64 cover = (i64)mbps * page_tokens;
+  const uint32_t pt = (uint32_t)page_tokens;
   constexpr int BATCH = 8;
   int before = 0;
   for (int i0 = 1; i0 < n; i0 += BATCH) {
     int node[BATCH];
-    i64 from[BATCH], to[BATCH];
-    uint4 v[BATCH];
+    uint32_t from[BATCH], to[BATCH];      // in 16-byte units, of the first head
     int good = 0;      // entries of this round that belong to a path
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) node[k] = i0 + k < n ? path[(i64)t * max_path + i0 + k] : -1;
@@ -484,21 +481,26 @@ __global__ void __launch_bounds__(256) kv_commit_kernel(uint4* __restrict__ kc, 
     for (int k = 0; k < BATCH; ++k) {
       const i64 src = (i64)ctx + node[k], dst = (i64)ctx + i0 + k;
       const bool in = node[k] >= i0 + k && src < cover;
-      const uint32_t s32 = in ? (uint32_t)src : 0u, d32 = in ? (uint32_t)dst : 0u, pt = (uint32_t)page_tokens;
+      const uint32_t s32 = in ? (uint32_t)src : 0u, d32 = in ? (uint32_t)dst : 0u;
       const uint32_t ps = in ? bt[s32 / pt] : 0xffffffffu, pd = in ? bt[d32 / pt] : 0xffffffffu;
       const bool ok = ps < (uint64_t)num_pages && pd < (uint64_t)num_pages && node[k] > (k ? node[k ? k - 1 : 0] : before);
-      from[k] = ok ? ps * page_stride + (i64)(s32 % pt) * chunks : -1;
-      to[k] = ok ? pd * page_stride + (i64)(d32 % pt) * chunks : -1;
+      from[k] = ok ? ps * page_stride + (s32 % pt) * (uint32_t)chunks : 0u;
+      to[k] = ok ? pd * page_stride + (d32 % pt) * (uint32_t)chunks : 0u;
       if (ok && good == k) good = k + 1;
     }
+    for (int at = at0; at < 2 * per; at += (int)gridDim.x * 256) {
+      const int e = at < per ? at : at - per, lh = e / chunks, c = e - lh * chunks, layer = lh / kv_heads, head = lh - layer * kv_heads;
+      uint4* cache = (at < per ? kc : vc) + layer * layer_stride + (i64)head * page_tokens * chunks + c;
+      uint4 v[BATCH];
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k)
-      if (k < good) v[k] = cache[from[k]];
+      for (int k = 0; k < BATCH; ++k)
+        if (k < good && from[k] != to[k]) v[k] = cache[from[k]];
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k)
-      if (k < good && from[k] != to[k]) cache[to[k]] = v[k];
+      for (int k = 0; k < BATCH; ++k)
+        if (k < good && from[k] != to[k]) cache[to[k]] = v[k];
+    }
     if (good < min(BATCH, n - i0)) {      // not a path, or past the table or the cache: the moves end here
-      if (e == 0 && status) atomicExch(status, WKB_STATUS_KV_POS_RANGE);
+      if (at0 == 0 && status) atomicExch(status, WKB_STATUS_KV_POS_RANGE);
       return;
     }
     before = node[BATCH - 1];
@@ -589,16 +591,18 @@ int wkb_paged_kv_commit(void* kcache, void* vcache, i64 layers, i64 layer_stride
                         i64 page_tokens, i64 max_blocks_per_seq, int* new_ctx_or_null, void* stream) {
   if (n_trees <= 0 || layers <= 0) return 0;
   if (n_trees > 65535 || max_path < 1 || kv_heads < 1 || head_dim < 8 || head_dim % 8 != 0 || page_tokens < 1 || max_blocks_per_seq < 1 || num_pages < 1 ||
-      max_blocks_per_seq * page_tokens > 0x7fffff00 || max_path > 0x7fffffff)
+      max_blocks_per_seq * page_tokens > 0x7fffff00 || max_path > 0x7fffffff ||
+      (double)num_pages * (double)kv_heads * (double)page_tokens * (double)(head_dim / 8) > 4294967040.0)      // 64 GB a layer and cache
     return (int)cudaErrorInvalidValue;
   if (new_ctx_or_null == tree_ctx) return (int)cudaErrorInvalidValue;      // read by every block of the tree
   if (layers > 1 && layer_stride < num_pages * kv_heads * page_tokens * head_dim) return (int)cudaErrorInvalidValue;
   if (((((uintptr_t)kcache) | ((uintptr_t)vcache)) & 15) != 0 || layer_stride % 8 != 0) return (int)cudaErrorMisalignedAddress;
   const i64 threads = 2 * layers * kv_heads * (head_dim / 8), blocks = (threads + 255) / 256;
-  if (layers > 0x7fffffff / 2 / (head_dim / 8) / kv_heads) return (int)cudaErrorInvalidValue;
+  if (layers > 0x3fffffff / 2 / (head_dim / 8) / kv_heads) return (int)cudaErrorInvalidValue;
+  const i64 wave = (WKB_SM_COUNT * 3 + n_trees - 1) / n_trees;      // blocks a tree that fill the SMs once
   int* status = gemm_status_word();
   if (!status) return (int)cudaErrorMemoryAllocation;
-  return (int)launch_pdl(verify::kv_commit_kernel, dim3((unsigned)blocks, (unsigned)n_trees), 256, 0, as_stream(stream), (uint4*)kcache, (uint4*)vcache,
+  return (int)launch_pdl(verify::kv_commit_kernel, dim3((unsigned)(blocks < wave ? blocks : wave), (unsigned)n_trees), 256, 0, as_stream(stream), (uint4*)kcache, (uint4*)vcache,
                          layer_stride / 8, num_pages, block_table, tree_slot, tree_ctx, path, n_path, (int)max_path, (int)layers, (int)kv_heads,
                          (int)(head_dim / 8), (int)page_tokens, (int)max_blocks_per_seq, new_ctx_or_null, status);
 }
