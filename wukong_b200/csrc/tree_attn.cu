@@ -17,6 +17,7 @@ constexpr int MAX_NODES = 256, MAX_TREES = 4096;
 struct Geo {
   int rows, n_trees, max_nodes, mask_words, q_heads, kv_heads, page_tokens, page_shift, mbps;
   i64 num_pages, q_row_stride, out_row_stride;
+  int split;      // units may be cut into pieces (tensor-core kernel)
 };
 struct TreeRef {
   int row0, nodes, ctx, slot;
@@ -156,11 +157,14 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void
   int page_shift = 0;
   while ((1 << page_shift) < page_tokens) ++page_shift;
   tree::Geo g{(int)rows, (int)n_trees, (int)max_nodes, (int)mask_words, (int)q_heads, (int)kv_heads, (int)page_tokens, page_shift, (int)max_blocks_per_seq,
-              num_pages, q_row_stride, out_row_stride};
+              num_pages, q_row_stride, out_row_stride, 1};
   cudaStream_t st = as_stream(stream);
   if (page_tokens >= 8) {      // a page of 8 tokens fills whole swizzle atoms of the operand
     const i64 row_blocks = (max_nodes * group + tree::QROWS - 1) / tree::QROWS, key_blocks = (max_blocks_per_seq * page_tokens + tree::KBLK - 1) / tree::KBLK + tree::UNIT_COST;
     if ((double)n_trees * (double)kv_heads * (double)row_blocks * (double)key_blocks > 2147000000.0) return (int)cudaErrorInvalidValue;
+    // Up to one unit an SM and 6 blocks a unit: 5 more blocks in a row take 3.5 (head_dim 64) to 5 us, a second kernel 3.3 us
+    // and its launch.
+    if (n_trees * kv_heads * row_blocks <= WKB_SM_COUNT && key_blocks - tree::UNIT_COST <= 6) g.split = 0;
 #define WKB_TREE_CASE(HD_, QS_, PS_)                                   \
   if (head_dim == HD_ && (q_dtype == 0 ? 2 : 1) == QS_ && (out_dtype == 0 ? 2 : 1) == PS_) \
     return tree::launch_tc<HD_, QS_, PS_>(q, kcache, vcache, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, out_dtype, g, scale, scratch, st);

@@ -4,7 +4,8 @@
 // keys are cut into blocks of 128.  All blocks of all units form one list that is dealt out in equal contiguous shares to
 // one CTA per SM, whatever the lengths: a share may hold several units, or a piece of one.  A unit that a single share
 // covers is written at once; the pieces of the others go to scratch as (maximum, sum, unnormalised output) and are
-// joined by tree_attn_join_kernel in key order, so results are run-to-run identical.
+// joined by tree_attn_join_kernel in key order, so results are run-to-run identical.  When the arguments say that there are
+// no more units than SMs and that they are short, units stay whole and nothing is joined.
 //
 // A CTA has two TMA warps (pages of K and of V into a ring each), an MMA warp and two teams of four softmax warps.  The teams take
 // alternate key blocks with tensor-memory columns of their own, so one team's exponentials run while the other's products
@@ -34,7 +35,7 @@ constexpr int TC_THREADS = 384, KBLK = 128, QROWS = 128, SUB = 128 * 128;
 
 // Header of the scratch: where share c begins, for the join.  Then (m, l) and O of two pieces a share.
 struct ShareStart {
-  int unit_start, unit_len, share, tree, head, rowblk, total, pad;
+  int unit_start, unit_len, share, total, row0, live, head, rowblk;      // unit_len 0: it begins in none
 };
 struct Scratch {
   ShareStart* start;
@@ -177,7 +178,8 @@ __device__ __forceinline__ TreeWork tree_work(const Geo& g, const int* slot, con
 }
 // A unit counts as its blocks and UNIT_COST more: what beginning and ending one takes, in blocks.
 constexpr int UNIT_COST = 5;
-__device__ __forceinline__ int tree_items(const Geo& g, const TreeWork& w) { return (w.blocks + UNIT_COST) * w.rowblks * g.kv_heads; }
+__device__ __forceinline__ int unit_items(const Geo& g, const TreeWork& w) { return g.split ? w.blocks + UNIT_COST : 1; }
+__device__ __forceinline__ int tree_items(const Geo& g, const TreeWork& w) { return unit_items(g, w) * w.rowblks * g.kv_heads; }
 
 // One piece of a unit: blocks [b0, b1) of `unit_len`.
 struct Piece {
@@ -196,13 +198,13 @@ struct Walk {
         tree_start += items;
         if (++tree >= g.n_trees) return false;
       }
-      const int size = p.w.blocks + UNIT_COST, unit = (item - tree_start) / size;
+      const int size = unit_items(g, p.w), unit = (item - tree_start) / size;
       p.tree = tree;
       p.head = unit / p.w.rowblks;
       p.rowblk = unit - p.head * p.w.rowblks;
       p.unit_start = tree_start + unit * size;
       p.b0 = item - p.unit_start;
-      p.b1 = min(p.w.blocks, p.b0 + end - item);
+      p.b1 = g.split ? min(p.w.blocks, p.b0 + end - item) : p.w.blocks;
       item = p.unit_start + size;
       if (p.b0 < p.b1) return true;      // else the share begins behind the unit's last block
     }
@@ -295,11 +297,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const int group = g.q_heads / g.kv_heads, gshift = 31 - __clz(group);      // a power of two
   const bool none = walk.item >= walk.end;
   if (threadIdx.x == 320) {      // (of the warp without a part) what the join has to know about the unit that this share begins in
-    ShareStart st{0, 0, share, 0, 0, 0, total, 0};
+    ShareStart st{0, 0, share, total, 0, 0, 0, 0};
     if (!none) {
       Walk w = walk;
       Piece p;
-      if (w.next(g, slot, ctxs, row0s, p)) { st.unit_start = p.unit_start; st.unit_len = p.w.blocks; st.tree = p.tree; st.head = p.head; st.rowblk = p.rowblk; }
+      if (w.next(g, slot, ctxs, row0s, p)) {
+        st.unit_start = p.unit_start; st.unit_len = p.w.blocks; st.row0 = p.w.t.row0; st.head = p.head; st.rowblk = p.rowblk;
+        st.live = min(QROWS, p.w.t.nodes * group - p.rowblk * QROWS);
+      }
     }
     scr.start[blockIdx.x] = st;
   }
@@ -420,63 +425,61 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
     };
     auto teams_sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };      // every softmax thread passes every one of these
-    // The query operand (K-major, 128-byte swizzle) of a piece: rows are fetched to registers, BATCH chunks a thread, and
-    // stored to every copy.
-    constexpr int CH = HD / 8, BATCH = 4;      // 16-byte chunks of bf16 a row
-    float4 qx[BATCH], qy[QS == 1 ? 1 : BATCH];
+    // The query operand (K-major, 128-byte swizzle).  The raw rows of the next piece come to the stage while this piece's
+    // blocks are worked on (q_fetch); q_put turns them into the operand's parts and copies.  A thread reads back what it
+    // fetched itself.  Rows beyond the stage (f32, head_dim 128, rows 64 and up) are read where they lie.
+    constexpr int CH = HD / 8, RAW = 16 * (QS == 1 ? 1 : 2), KEPT = SM::STAGE_BYTES / RAW;      // chunks of 8 values a row, their bytes, chunks staged
     auto live_of = [&](const Piece& p) { return min(QROWS, p.w.t.nodes * group - p.rowblk * QROWS); };
     auto copies_of = [&](int live) { return live <= 32 ? 4 : live <= 64 ? 2 : 1; };
-    auto q_fetch = [&](const Piece& p, int i0) {
-      const int live = live_of(p);
+    auto q_at = [&](const Piece& p, int idx) {
+      const int qr = idx / CH, c = idx % CH, ur = p.rowblk * QROWS + qr;
+      return static_cast<const uint8_t*>(q) +
+             ((i64)(p.w.t.row0 + (ur >> gshift)) * g.q_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD + c * 8) * (QS == 1 ? 2 : 4);
+    };
+    auto q_fetch = [&](const Piece& p) {
+      const int n = min(live_of(p) * CH, KEPT);
+#pragma unroll 1
+      for (int idx = tid; idx < n; idx += 256) {
+        const uint8_t* src = q_at(p, idx);
 #pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        const int idx = i0 + b * 256, qr = idx / CH, c = idx % CH, ur = p.rowblk * QROWS + qr;
-        qx[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (QS > 1) qy[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (qr >= live) continue;
-        const i64 at = (i64)(p.w.t.row0 + (ur >> gshift)) * g.q_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD + c * 8;
-        if (QS == 1) qx[b] = *reinterpret_cast<const float4*>(static_cast<const u16*>(q) + at);
-        else {
-          qx[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
-          qy[b] = *reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + 4);
-        }
+        for (int k = 0; k < RAW; k += 16)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage_base + (uint32_t)idx * RAW + k), "l"(src + k) : "memory");
       }
     };
     auto q_put = [&](const Piece& p) {
-      const int copies = copies_of(live_of(p)), crows = QROWS / copies;
+      const int live = live_of(p), copies = copies_of(live), crows = QROWS / copies;
       const uint32_t flip = negate ? 0x80008000u : 0u;
-#pragma unroll 1
-      for (int i0 = tid;;) {
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-          const int idx = i0 + b * 256, qr = idx / CH, c = idx % CH;
-          if (idx >= crows * CH) break;
-          uint32_t w[QS][4];
-          if (QS == 1) { w[0][0] = f2u(qx[b].x); w[0][1] = f2u(qx[b].y); w[0][2] = f2u(qx[b].z); w[0][3] = f2u(qx[b].w); }
-          else {
-            const float4 y = qy[QS == 1 ? 0 : b];
-            float f[8] = {qx[b].x, qx[b].y, qx[b].z, qx[b].w, y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int k = 0; k < QS; ++k)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                w[k][e] = pack_bf16(f[2 * e], f[2 * e + 1]);
-                f[2 * e] -= u2f(w[k][e] << 16);
-                f[2 * e + 1] -= u2f(w[k][e] & 0xffff0000u);
-              }
-          }
-          const uint32_t dst = q_base + (uint32_t)(c >> 3) * SUB + (uint32_t)qr * 128u + (uint32_t)(((c & 7) ^ (qr & 7)) << 4);
-#pragma unroll 1
-          for (int cp = 0; cp < copies; ++cp)
-#pragma unroll
-            for (int k = 0; k < QS; ++k)
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * BLK + (uint32_t)(cp * crows) * 128u), "r"(w[k][0] ^ flip),
-                           "r"(w[k][1] ^ flip), "r"(w[k][2] ^ flip), "r"(w[k][3] ^ flip)
-                           : "memory");
+      asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+      for (int idx = tid; idx < crows * CH; idx += 256) {
+        const int qr = idx / CH, c = idx % CH;
+        float4 x[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+        if (qr < live) {
+          const float4* from = reinterpret_cast<const float4*>(idx < KEPT ? reinterpret_cast<const uint8_t*>(stage) + (size_t)idx * RAW : q_at(p, idx));
+          x[0] = from[0];
+          if (QS > 1) x[1] = from[1];
         }
-        i0 += 256 * BATCH;
-        if (i0 >= crows * CH) break;
-        q_fetch(p, i0);
+        uint32_t w[QS][4];
+        if (QS == 1) { w[0][0] = f2u(x[0].x); w[0][1] = f2u(x[0].y); w[0][2] = f2u(x[0].z); w[0][3] = f2u(x[0].w); }
+        else {
+          float f[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+#pragma unroll
+          for (int k = 0; k < QS; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[k][e] = pack_bf16(f[2 * e], f[2 * e + 1]);
+              f[2 * e] -= u2f(w[k][e] << 16);
+              f[2 * e + 1] -= u2f(w[k][e] & 0xffff0000u);
+            }
+        }
+        const uint32_t dst = q_base + (uint32_t)(c >> 3) * SUB + (uint32_t)qr * 128u + (uint32_t)(((c & 7) ^ (qr & 7)) << 4);
+#pragma unroll 1
+        for (int cp = 0; cp < copies; ++cp)
+#pragma unroll
+          for (int k = 0; k < QS; ++k)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * BLK + (uint32_t)(cp * crows) * 128u), "r"(w[k][0] ^ flip), "r"(w[k][1] ^ flip),
+                         "r"(w[k][2] ^ flip), "r"(w[k][3] ^ flip)
+                         : "memory");
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -484,13 +487,15 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     };
     Piece p, following;
     bool more = walk.next(g, slot, ctxs, row0s, following);
-    if (more) { q_fetch(following, tid); q_put(following); }
+    if (more) { q_fetch(following); q_put(following); }
     while (more) {
       p = following;
       more = walk.next(g, slot, ctxs, row0s, following);
       const int len = p.b1 - p.b0;
       const int live = live_of(p), copies = copies_of(live), crows = QROWS / copies;
       const int copy = a / crows, r = a % crows;
+      teams_sync();      // the stage is free
+      if (more) q_fetch(following);
       // ---- the team's key blocks
       auto mask_of = [&](int row) { return mask + (i64)(p.w.t.row0 + ((p.rowblk * QROWS + row) >> gshift)) * g.mask_words; };
       const uint32_t* own_mask = mask_of(min(r, live - 1));
@@ -631,7 +636,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
       // ---- the result: the teams' accumulators lie in the same lanes and are added in registers; the copies lie in other
       // lanes and are added through shared memory, 64 columns at a time
-      if (more) q_fetch(following, tid);
       ml_s[team * QROWS + a] = make_float2(team < len ? m : -INFINITY, team < len ? l : 0.0f);
       teams_sync();      // every product with this piece's query is done: the next one's can start while the result is written
       if (more) q_put(following);
@@ -657,8 +661,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       const int piece = p.unit_start + p.b0 == (int)blockIdx.x * share ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
       if (!whole && fine && team == 0 && copy == 0 && r < live) scr.ml[(i64)piece * scr.rows + r] = make_float2(m_all, l_all);
       // rare: V holds a NaN or an infinity that this row may see.  Its sum over those elements is then the result
+      // (a row with a NaN score stays NaN)
       auto bad_columns = [&](int row, int col, float4& v) {
         const uint32_t* mrow = mask_of(row);
+#pragma unroll 1
+        for (int i = row; i < (both ? 2 : 1) * QROWS; i += crows)
+          if (ml_s[i].y != ml_s[i].y) return;
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
         for (int pos = p.b0 * KBLK; pos < min(p.b1 * KBLK, p.w.keys); ++pos) {
@@ -674,6 +682,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         v.z = x[2] != 0.0f ? x[2] : v.z; v.w = x[3] != 0.0f ? x[3] : v.w;
       };
       const bool staged = copies > 1 || bad_v;
+      if (staged && more) teams_sync();      // the next query has been read from the stage
       auto out_at = [&](int row) {      // of column 0
         const int ur = p.rowblk * QROWS + row;
         return whole ? (i64)(p.w.t.row0 + (ur >> gshift)) * g.out_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD
@@ -722,19 +731,21 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         if (!staged) continue;
         teams_sync();
-        const int c4 = tid & 15;
-#pragma unroll 1
-        for (int row = tid >> 4; row < live; row += 16) {
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (int x = row; x < QROWS; x += crows) {
-            const float4 s4 = *reinterpret_cast<const float4*>(stage + x * 64 + ((c4 ^ (x & 7)) << 2));
-            v.x += s4.x; v.y += s4.y; v.z += s4.z; v.w += s4.w;
-          }
+        // a thread keeps its four columns and goes down the rows, 16 at a step (a multiple of the group)
+        const int c4 = tid & 15, first = tid >> 4;
+        const i64 down = whole ? (i64)(16 >> gshift) * g.out_row_stride : (i64)16 * HD;
+        i64 at = out_at(first) + c0 + c4 * 4;
+        auto part = [&](int x) { return *reinterpret_cast<const float4*>(stage + x * 64 + ((c4 ^ (x & 7)) << 2)); };
+        auto add = [](float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; };
+#pragma unroll 2
+        for (int row = first; row < live; row += 16, at += down) {
+          float4 v = part(row);
+          if (copies > 1) add(v, part(row + crows));
+          if (copies > 2) { add(v, part(row + 2 * crows)); add(v, part(row + 3 * crows)); }
           if (bad_v || !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) <= 3.402823466e+38f)) bad_columns(row, c0 + c4 * 4, v);
-          if (fine) put(out_at(row) + c0 + c4 * 4, v);
+          if (fine) put(at, v);
         }
-        teams_sync();
+        if (c0 + 64 < HD) teams_sync();
       }
       if (bad_v) {
         teams_sync();
@@ -754,40 +765,46 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 }
 
 // Block (c, rows): if the boundary before share c falls inside a unit, and is the first one that does, join the unit's
-// pieces (in key order) for these rows and write the result.
+// pieces (in key order) for these rows and write the result.  A row is HD / 4 lanes, which first share the pieces' (m, l)
+// out among them, so that the trips to L2 do not add up with the number of pieces.
 template <int HD>
-__global__ void __launch_bounds__(256) tree_attn_join_kernel(const int* __restrict__ slot, const int* __restrict__ ctxs, const int* __restrict__ row0s,
-                                                             void* __restrict__ out, int out_dtype, Geo g, Scratch scr, const int* __restrict__ status) {
+__global__ void __launch_bounds__(256) tree_attn_join_kernel(void* __restrict__ out, int out_dtype, Geo g, Scratch scr, const int* __restrict__ status) {
   pdl_wait();
   pdl_trigger();
   const int c = blockIdx.x + 1;
   const ShareStart st = scr.start[c];
+  const int failed = *status == WKB_STATUS_ATTN_WAIT;
   const int x = c * st.share;
-  if (x >= st.total || st.unit_len == 0 || x <= st.unit_start || x - st.share > st.unit_start) return;
-  if (*status == WKB_STATUS_ATTN_WAIT) return;
+  if (x >= st.total || st.unit_len == 0 || x <= st.unit_start || x - st.share > st.unit_start || failed) return;
   const int last = (st.unit_start + st.unit_len - 1) / st.share, group = g.q_heads / g.kv_heads;
-  const TreeRef t = tree_ref(g, slot, ctxs, row0s, st.tree);
-  const int live = min(QROWS, t.nodes * group - st.rowblk * QROWS);
   constexpr int LANES = HD / 4;
-  const int row = blockIdx.y * (256 / LANES) + threadIdx.x / LANES, col = threadIdx.x % LANES * 4;
-  if (row >= live) return;
+  const int lane = threadIdx.x % LANES, row = blockIdx.y * (256 / LANES) + threadIdx.x / LANES, col = lane * 4;
+  const unsigned team = LANES == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+  if (row >= st.live) return;      // (all lanes of a row)
   auto piece = [&](int k) { return (i64)(k * st.share >= st.unit_start ? 2 * k : 2 * k + 1) * scr.rows + row; };
   float m = -INFINITY;
-  for (int k = c - 1; k <= last; ++k) m = fmaxf(m, scr.ml[piece(k)].x);
+  for (int k = c - 1 + lane; k <= last; k += LANES) m = fmaxf(m, scr.ml[piece(k)].x);
+  for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(team, m, o, LANES));
   const float use = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int k = c - 1; k <= last; ++k) {
-    const float2 ml = scr.ml[piece(k)];
+  for (int k0 = c - 1; k0 <= last; k0 += LANES) {
+    const int n = min(LANES, last + 1 - k0);
+    const float2 ml = lane < n ? scr.ml[piece(k0 + lane)] : make_float2(-INFINITY, 0.0f);
     const float w = ex2(ml.x - use);
-    const float4 v = *reinterpret_cast<const float4*>(scr.o + piece(k) * HD + col);
     l += ml.y * w;
-    o.x += v.x * w; o.y += v.y * w; o.z += v.z * w; o.w += v.w * w;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float wk = __shfl_sync(team, w, k, LANES);
+      const float4 v = *reinterpret_cast<const float4*>(scr.o + piece(k0 + k) * HD + col);
+      o.x = ffma(v.x, wk, o.x); o.y = ffma(v.y, wk, o.y); o.z = ffma(v.z, wk, o.z); o.w = ffma(v.w, wk, o.w);
+    }
   }
+  for (int k = LANES / 2; k > 0; k >>= 1) l += __shfl_xor_sync(team, l, k, LANES);
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
   const int ur = st.rowblk * QROWS + row;
-  const i64 at = (i64)(t.row0 + ur / group) * g.out_row_stride + ((i64)st.head * group + ur % group) * HD + col;
+  const i64 at = (i64)(st.row0 + ur / group) * g.out_row_stride + ((i64)st.head * group + ur % group) * HD + col;
   if (out_dtype == 0) *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = o;
   else *reinterpret_cast<uint2*>(static_cast<u16*>(out) + at) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
 }
@@ -831,10 +848,9 @@ int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt,
   const Scratch scr = carve(scratch, g.max_nodes, group);
   cudaError_t e = launch_pdl(kern, WKB_SM_COUNT, TC_THREADS, (size_t)TcSmem<HD, QS>::BYTES, st, mk, mv, q, (const u16*)vc, bt, slot, ctx, row0, mask, out,
                              out_dtype, g, scale, scr, status);
-  if (e != cudaSuccess) return (int)e;
+  if (e != cudaSuccess || !g.split) return (int)e;
   const int rows_per = 256 / (HD / 4);
-  return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(WKB_SM_COUNT - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, slot, ctx, row0, out,
-                         out_dtype, g, scr, (const int*)status);
+  return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(WKB_SM_COUNT - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, out, out_dtype, g, scr, (const int*)status);
 }
 
 }  // namespace tree
