@@ -232,8 +232,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   auto s_full = [&](int t) { return more + 8u * t; };
   auto p_full = [&](int t) { return more + 8u * (2 + t); };
   auto o_done = [&](int t) { return more + 8u * (4 + t); };
-  const uint32_t q_full = more + 8u * 6;
-  static_assert(8 * (2 * NK + 2 * NV + 7) <= 256, "barriers fit the header");
+  const uint32_t q_full = more + 8u * 6, q_first = more + 8u * 7;      // the first piece's query is everybody's work
+  static_assert(8 * (2 * NK + 2 * NV + 8) <= 256, "barriers fit the header");
   volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + 256);      // 0 tensor memory, 1 failed, 2 V not finite, 3.. the share
   float2* ml_s = reinterpret_cast<float2*>(smem_raw + 512);
   float* stage = reinterpret_cast<float*>(smem_raw + (stage_base - raw));
@@ -247,7 +247,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     for (int s = 0; s < NK; ++s) { mbar_init(kfull(s), 1); mbar_init(kempty(s), 1); }
     for (int s = 0; s < NV; ++s) { mbar_init(vfull(s), 1); mbar_init(vempty(s), 1); }
     for (int t = 0; t < 2; ++t) { mbar_init(s_full(t), 1); mbar_init(p_full(t), 4); mbar_init(o_done(t), 1); }
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 4); mbar_init(q_first, 8);
     flags[1] = 0; flags[2] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
@@ -383,7 +383,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           umma_commit(kempty(s));
           return true;
         };
-        ok = bar_wait(q_full, pieces & 1);
+        ok = pieces == 0 ? bar_wait(q_first, 0) : bar_wait(q_full, (pieces - 1) & 1);
         ++pieces;
         ok = ok && scores(0);
         if (len > 1) ok = ok && scores(1);
@@ -426,8 +426,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     };
     auto teams_sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };      // every softmax thread passes every one of these
     // The query operand (K-major, 128-byte swizzle).  The raw rows of the next piece come to the stage while this piece's
-    // blocks are worked on (q_fetch); q_put turns them into the operand's parts and copies.  A thread reads back what it
-    // fetched itself.  Rows beyond the stage (f32, head_dim 128, rows 64 and up) are read where they lie.
+    // blocks are worked on (q_fetch), and the team that is not at work on the last block turns them into the operand's parts
+    // and copies (q_put) as soon as that block's scores have been multiplied.  A thread reads back what it fetched itself.
+    // Rows beyond the stage (f32, head_dim 128, rows 64 and up) come when the first ones have left it.
     constexpr int CH = HD / 8, RAW = 16 * (QS == 1 ? 1 : 2), KEPT = SM::STAGE_BYTES / RAW;      // chunks of 8 values a row, their bytes, chunks staged
     auto live_of = [&](const Piece& p) { return min(QROWS, p.w.t.nodes * group - p.rowblk * QROWS); };
     auto copies_of = [&](int live) { return live <= 32 ? 4 : live <= 64 ? 2 : 1; };
@@ -436,66 +437,69 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       return static_cast<const uint8_t*>(q) +
              ((i64)(p.w.t.row0 + (ur >> gshift)) * g.q_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD + c * 8) * (QS == 1 ? 2 : 4);
     };
-    auto q_fetch = [&](const Piece& p) {
-      const int n = min(live_of(p) * CH, KEPT);
+    auto q_fetch = [&](const Piece& p, int from, int self, int threads) {
+      const int n = min(live_of(p) * CH, from + KEPT);
 #pragma unroll 1
-      for (int idx = tid; idx < n; idx += 256) {
+      for (int idx = from + self; idx < n; idx += threads) {
         const uint8_t* src = q_at(p, idx);
 #pragma unroll
         for (int k = 0; k < RAW; k += 16)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage_base + (uint32_t)idx * RAW + k), "l"(src + k) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage_base + (uint32_t)(idx - from) * RAW + k), "l"(src + k) : "memory");
       }
     };
-    auto q_put = [&](const Piece& p) {
+    auto q_put = [&](const Piece& p, int self, int threads, uint32_t bar) {
       const int live = live_of(p), copies = copies_of(live), crows = QROWS / copies;
       const uint32_t flip = negate ? 0x80008000u : 0u;
-      asm volatile("cp.async.wait_all;" ::: "memory");
+      for (int from = 0; from < crows * CH; from += KEPT) {
+        if (from > 0) q_fetch(p, from, self, threads);
+        asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 2
-      for (int idx = tid; idx < crows * CH; idx += 256) {
-        const int qr = idx / CH, c = idx % CH;
-        float4 x[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-        if (qr < live) {
-          const float4* from = reinterpret_cast<const float4*>(idx < KEPT ? reinterpret_cast<const uint8_t*>(stage) + (size_t)idx * RAW : q_at(p, idx));
-          x[0] = from[0];
-          if (QS > 1) x[1] = from[1];
-        }
-        uint32_t w[QS][4];
-        if (QS == 1) { w[0][0] = f2u(x[0].x); w[0][1] = f2u(x[0].y); w[0][2] = f2u(x[0].z); w[0][3] = f2u(x[0].w); }
-        else {
-          float f[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+        for (int idx = from + self; idx < min(crows * CH, from + KEPT); idx += threads) {
+          const int qr = idx / CH, c = idx % CH;
+          float4 x[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+          if (qr < live) {
+            const float4* raw_q = reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(stage) + (idx - from) * RAW);
+            x[0] = raw_q[0];
+            if (QS > 1) x[1] = raw_q[1];
+          }
+          uint32_t w[QS][4];
+          if (QS == 1) { w[0][0] = f2u(x[0].x); w[0][1] = f2u(x[0].y); w[0][2] = f2u(x[0].z); w[0][3] = f2u(x[0].w); }
+          else {
+            float f[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
 #pragma unroll
-          for (int k = 0; k < QS; ++k)
+            for (int k = 0; k < QS; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              w[k][e] = pack_bf16(f[2 * e], f[2 * e + 1]);
-              f[2 * e] -= u2f(w[k][e] << 16);
-              f[2 * e + 1] -= u2f(w[k][e] & 0xffff0000u);
-            }
-        }
-        const uint32_t dst = q_base + (uint32_t)(c >> 3) * SUB + (uint32_t)qr * 128u + (uint32_t)(((c & 7) ^ (qr & 7)) << 4);
+              for (int e = 0; e < 4; ++e) {
+                w[k][e] = pack_bf16(f[2 * e], f[2 * e + 1]);
+                f[2 * e] -= u2f(w[k][e] << 16);
+                f[2 * e + 1] -= u2f(w[k][e] & 0xffff0000u);
+              }
+          }
+          const uint32_t dst = q_base + (uint32_t)(c >> 3) * SUB + (uint32_t)qr * 128u + (uint32_t)(((c & 7) ^ (qr & 7)) << 4);
 #pragma unroll 1
-        for (int cp = 0; cp < copies; ++cp)
+          for (int cp = 0; cp < copies; ++cp)
 #pragma unroll
-          for (int k = 0; k < QS; ++k)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * BLK + (uint32_t)(cp * crows) * 128u), "r"(w[k][0] ^ flip), "r"(w[k][1] ^ flip),
-                         "r"(w[k][2] ^ flip), "r"(w[k][3] ^ flip)
-                         : "memory");
+            for (int k = 0; k < QS; ++k)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + k * BLK + (uint32_t)(cp * crows) * 128u), "r"(w[k][0] ^ flip), "r"(w[k][1] ^ flip),
+                           "r"(w[k][2] ^ flip), "r"(w[k][3] ^ flip)
+                           : "memory");
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      if (lane == 0) mbar_arrive(bar);
     };
     Piece p, following;
     bool more = walk.next(g, slot, ctxs, row0s, following);
-    if (more) { q_fetch(following); q_put(following); }
+    if (more) { q_fetch(following, 0, tid, 256); q_put(following, tid, 256, q_first); }
     while (more) {
       p = following;
       more = walk.next(g, slot, ctxs, row0s, following);
       const int len = p.b1 - p.b0;
       const int live = live_of(p), copies = copies_of(live), crows = QROWS / copies;
       const int copy = a / crows, r = a % crows;
-      teams_sync();      // the stage is free
-      if (more) q_fetch(following);
+      const bool puts = more && team == (len & 1);      // the team without the last block
+      if (puts) q_fetch(following, 0, tid & 127, 128);
       // ---- the team's key blocks
       auto mask_of = [&](int row) { return mask + (i64)(p.w.t.row0 + ((p.rowblk * QROWS + row) >> gshift)) * g.mask_words; };
       const uint32_t* own_mask = mask_of(min(r, live - 1));
@@ -636,20 +640,23 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
       // ---- the result: the teams' accumulators lie in the same lanes and are added in registers; the copies lie in other
       // lanes and are added through shared memory, 64 columns at a time
-      ml_s[team * QROWS + a] = make_float2(team < len ? m : -INFINITY, team < len ? l : 0.0f);
-      teams_sync();      // every product with this piece's query is done: the next one's can start while the result is written
-      if (more) q_put(following);
-      const bool both = len > 1;      // team 1 had a block
       done[0] += (len + 1) >> 1;
       done[1] += len >> 1;
+      if (puts) {
+        wait(s_full(team ^ 1), (done[team ^ 1] - 1) & 1);      // the last product with this piece's query is done
+        q_put(following, tid & 127, 128, q_full);
+      }
+      ml_s[team * QROWS + a] = make_float2(team < len ? m : -INFINITY, team < len ? l : 0.0f);
+      teams_sync();
+      const bool both = len > 1;      // team 1 had a block
       wait(o_done(0), (done[0] - 1) & 1);
       if (both) wait(o_done(1), (done[1] - 1) & 1);
       tc_fence_after();
       float m_all = -INFINITY, l_all = 0.0f;
-#pragma unroll 1
+#pragma unroll 4
       for (int i = r; i < (both ? 2 : 1) * QROWS; i += crows) m_all = fmaxf(m_all, ml_s[i].x);      // copies of team 0, then of team 1
       const float m_use = m_all == -INFINITY ? 0.0f : m_all;
-#pragma unroll 1
+#pragma unroll 4
       for (int i = r; i < (both ? 2 : 1) * QROWS; i += crows) {
         const float2 v = ml_s[i];
         l_all += v.y * ex2(v.x - m_use);
@@ -682,7 +689,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         v.z = x[2] != 0.0f ? x[2] : v.z; v.w = x[3] != 0.0f ? x[3] : v.w;
       };
       const bool staged = copies > 1 || bad_v;
-      if (staged && more) teams_sync();      // the next query has been read from the stage
       auto out_at = [&](int row) {      // of column 0
         const int ur = p.rowblk * QROWS + row;
         return whole ? (i64)(p.w.t.row0 + (ur >> gshift)) * g.out_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD
@@ -752,7 +758,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (tid == 0) flags[2] = 0;
       }
       tc_fence_before();
-      teams_sync();      // the accumulators and ml_s are free
+      teams_sync();      // the accumulators, the stage and ml_s are free
     }
   }
   tc_fence_before();
