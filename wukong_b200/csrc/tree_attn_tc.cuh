@@ -137,6 +137,23 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two f32 at a time
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void of_two(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -541,8 +558,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           load(c);
           float b4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int e = 4; e < 32; ++e) b4[e & 3] = fmaxf(b4[e & 3], s[e]);
-          top = fmaxf(top, fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3])));
+          for (int e = 4; e < 28; e += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) b4[k] = fmaxf(fmaxf(b4[k], s[e + k]), s[e + 4 + k]);
+          top = fmaxf(fmaxf(top, b4[0]), b4[1]);
+          top = fmaxf(fmaxf(top, b4[2]), b4[3]);
+          top = fmaxf(fmaxf(top, s[28]), s[29]);
+          top = fmaxf(fmaxf(top, s[30]), s[31]);
         }
         top *= sc;
         const bool move = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
@@ -568,19 +590,23 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const float m_use = m == -INFINITY ? 0.0f : m;
 #pragma unroll 1
         for (int c = chunks - 1;; ) {
-          float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          uint64_t l2[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
           uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float p0 = ex2(ffma(s[e], sc, -m_use)), p1 = ex2(ffma(s[e + 1], sc, -m_use));
-            l4[(e >> 1) & 1] += p0;
-            l4[2 + ((e >> 1) & 1)] += p1;
+            float p0, p1;
+            of_two(fma_two(two(s[e], s[e + 1]), two(sc, sc), two(-m_use, -m_use)), p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            l2[(e >> 1) & 1] = add_two(l2[(e >> 1) & 1], two(p0, p1));
             pk[e >> 1] = pack_bf16(p0, p1);
             if (PS == 2) pk[16 + (e >> 1)] = pack_bf16(p0 - u2f(pk[e >> 1] << 16), p1 - u2f(pk[e >> 1] & 0xffff0000u));
           }
           if (PS == 2) tm_st32(s_col + col0 + c * 32, pk);
           else tm_st16(s_col + col0 + c * 32, pk);
-          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          float la, lb;
+          of_two(add_two(l2[0], l2[1]), la, lb);
+          l += la + lb;
           if (--c < 0) break;
           load(c);
         }

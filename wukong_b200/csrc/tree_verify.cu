@@ -580,8 +580,14 @@ int wkb_tree_verify(const float* probs, i64 ld_p, const float* draft_or_null, i6
   if (n_trees > 0x7fffffff / ctas) return (int)cudaErrorInvalidValue;
   auto kern = draft_or_null ? verify::tree_verify_kernel<true> : verify::tree_verify_kernel<false>;
   constexpr int SMEM = 2 * verify::HOLD * verify::PT * (int)sizeof(float);
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e != cudaSuccess) return (int)e;
+  static bool attr_set[64][2] = {{false}};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[dev & 63][draft_or_null != nullptr]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return (int)e;
+    attr_set[dev & 63][draft_or_null != nullptr] = true;
+  }
   return (int)verify::launch_cluster(kern, (unsigned)(n_trees * ctas), verify::PT, SMEM, ctas, as_stream(stream), probs, ld_p, draft_or_null, ld_q, token, parent,
                                      tree_row0, (int)rows, (int)cols, (int)max_nodes, u_node, u_final, path, tokens, n_path, (int)max_path);
 }
