@@ -134,7 +134,7 @@ extern "C" {
 
 i64 wkb_paged_attn_tree_scratch_bytes(i64 max_nodes, i64 q_heads, i64 kv_heads, i64 head_dim) {
   if (max_nodes <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0) return 0;
-  return tree::scratch_bytes(max_nodes, q_heads / kv_heads, head_dim);
+  return tree::scratch_bytes(max_nodes, q_heads / kv_heads, head_dim, tree::shares_of(head_dim));
 }
 
 int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void* kcache, const void* vcache, i64 num_pages, const uint32_t* block_table,
@@ -162,9 +162,9 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void
   if (page_tokens >= 8) {      // a page of 8 tokens fills whole swizzle atoms of the operand
     const i64 row_blocks = (max_nodes * group + tree::QROWS - 1) / tree::QROWS, key_blocks = (max_blocks_per_seq * page_tokens + tree::KBLK - 1) / tree::KBLK + tree::UNIT_COST;
     if ((double)n_trees * (double)kv_heads * (double)row_blocks * (double)key_blocks > 2147000000.0) return (int)cudaErrorInvalidValue;
-    // Up to one unit an SM and 6 blocks a unit: 5 more blocks in a row take 3.5 (head_dim 64) to 5 us, a second kernel 3.3 us
+    // Up to one unit a CTA and 6 blocks a unit: 5 more blocks in a row take 3.5 (head_dim 64) to 5 us, a second kernel 3.3 us
     // and its launch.
-    if (n_trees * kv_heads * row_blocks <= WKB_SM_COUNT && key_blocks - tree::UNIT_COST <= 6) g.split = 0;
+    if (n_trees * kv_heads * row_blocks <= tree::shares_of(head_dim) && key_blocks - tree::UNIT_COST <= 6) g.split = 0;
 #define WKB_TREE_CASE(HD_, QS_, PS_)                                   \
   if (head_dim == HD_ && (q_dtype == 0 ? 2 : 1) == QS_ && (out_dtype == 0 ? 2 : 1) == PS_) \
     return tree::launch_tc<HD_, QS_, PS_>(q, kcache, vcache, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, out_dtype, g, scale, scratch, st);

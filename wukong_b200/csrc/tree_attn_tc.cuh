@@ -2,7 +2,7 @@
 //
 // Work.  A unit is (tree, KV head, 128 of the tree's query rows, node-major with the heads of the group inside); its
 // keys are cut into blocks of 128.  All blocks of all units form one list that is dealt out in equal contiguous shares to
-// one CTA per SM, whatever the lengths: a share may hold several units, or a piece of one.  A unit that a single share
+// as many CTAs as the SMs hold, whatever the lengths: a share may hold several units, or a piece of one.  A unit that a single share
 // covers is written at once; the pieces of the others go to scratch as (maximum, sum, unnormalised output) and are
 // joined by tree_attn_join_kernel in key order, so results are run-to-run identical.  When the arguments say that there are
 // no more units than SMs and that they are short, units stay whole and nothing is joined.
@@ -31,7 +31,7 @@ int* gemm_status_word();
 
 namespace tree {
 
-constexpr int TC_THREADS = 384, KBLK = 128, QROWS = 128, SUB = 128 * 128;
+constexpr int KBLK = 128, QROWS = 128, SUB = 128 * 128;
 
 // Header of the scratch: where share c begins, for the join.  Then (m, l) and O of two pieces a share.
 struct ShareStart {
@@ -47,17 +47,17 @@ __host__ __device__ inline int piece_rows(i64 max_nodes, i64 group) {
   const i64 r = max_nodes * group;
   return (int)(r < QROWS ? r : QROWS);
 }
-inline i64 scratch_bytes(i64 max_nodes, i64 group, i64 hd) {
-  const i64 rows = 2 * WKB_SM_COUNT * (i64)piece_rows(max_nodes, group);
-  return (i64)sizeof(ShareStart) * WKB_SM_COUNT + rows * 8 + rows * hd * 4;
+inline i64 scratch_bytes(i64 max_nodes, i64 group, i64 hd, i64 shares) {
+  const i64 rows = 2 * shares * (i64)piece_rows(max_nodes, group);
+  return (i64)sizeof(ShareStart) * shares + rows * 8 + rows * hd * 4;
 }
-inline Scratch carve(void* p, i64 max_nodes, i64 group) {
+inline Scratch carve(void* p, i64 max_nodes, i64 group, i64 shares) {
   const int r = piece_rows(max_nodes, group);
   uint8_t* b = static_cast<uint8_t*>(p);
   Scratch s;
   s.start = reinterpret_cast<ShareStart*>(b);
-  s.ml = reinterpret_cast<float2*>(b + sizeof(ShareStart) * WKB_SM_COUNT);
-  s.o = reinterpret_cast<float*>(b + sizeof(ShareStart) * WKB_SM_COUNT + (i64)2 * WKB_SM_COUNT * r * 8);
+  s.ml = reinterpret_cast<float2*>(b + sizeof(ShareStart) * shares);
+  s.o = reinterpret_cast<float*>(b + sizeof(ShareStart) * shares + 2 * shares * r * 8);
   s.rows = r;
   return s;
 }
@@ -73,15 +73,29 @@ struct Layout {
   static __host__ __device__ int box_rows(int page_tokens) { return HALVES == 2 ? 8 : page_tokens < KBLK ? page_tokens : KBLK; }
 };
 
+// head_dim 128: one CTA per SM with two teams, which take alternate blocks.  head_dim 64: everything is half as large, so
+// two CTAs of one team fit an SM; they work on different units, and one's beginnings and ends run under the other's
+// products (33 us with two teams, 30 with two CTAs, for 32 trees of a GPT-2 shape).
+template <int HD>
+struct Shape {
+  static constexpr int TEAMS = HD == 64 ? 1 : 2, CTAS = 2 / TEAMS, THREADS = TEAMS == 2 ? 384 : 256, SHARES = WKB_SM_COUNT * CTAS;
+  static constexpr int SMEM = TEAMS == 2 ? 232448 : 115712;                       // a CTA's part of 228 KB, 1 KB of each CTA reserved
+  static constexpr int TM_COLS = 256 * TEAMS, O_COL = 128 * TEAMS;                // tensor memory: the teams' S (128 columns each), then their O
+};
+inline int shares_of(i64 hd) { return hd == 64 ? Shape<64>::SHARES : Shape<128>::SHARES; }
+
 template <int HD, int QS>
 struct TcSmem {
   static constexpr int NSUB = HD / 64, BLK = NSUB * SUB;                 // bytes of 128 rows of an operand
   static constexpr int HEADER = 3072;                                    // barriers, (m, l) of the teams, flags
-  static constexpr int Q_BYTES = QS * BLK, STAGE_BYTES = QROWS * 64 * 4;
-  static constexpr int ROOM = (232448 - HEADER - Q_BYTES - STAGE_BYTES) / BLK, SLOTS = ROOM > 12 ? 12 : ROOM;
+  // the stage (the copies' sums, and the next query's raw rows): of its own beside two teams; a single team's lies over the
+  // query, which is not needed when a result is written
+  static constexpr int TEAMS = Shape<HD>::TEAMS, STAGE = QROWS * 64 * 4, STAGE_BYTES = TEAMS == 2 ? STAGE : 0;
+  static constexpr int Q_BYTES = TEAMS == 1 && QS * BLK < STAGE ? STAGE : QS * BLK;
+  static constexpr int SLOTS = (Shape<HD>::SMEM - HEADER - Q_BYTES - STAGE_BYTES) / BLK;
   static constexpr int NK = (SLOTS + 1) / 2, NV = SLOTS / 2;
   static constexpr int BYTES = HEADER + Q_BYTES + STAGE_BYTES + SLOTS * BLK;
-  static_assert(NV >= 2 && BYTES <= 232448, "at least two blocks of each operand in flight");
+  static_assert(NV >= 2 && BYTES <= Shape<HD>::SMEM, "at least two blocks of each operand in flight");
 };
 
 __host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_mn) {      // kind::f16: D f32, A = B = bf16, M = 128
@@ -230,17 +244,17 @@ struct Walk {
 };
 
 template <int HD, int QS, int PS>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __launch_bounds__(Shape<HD>::THREADS, Shape<HD>::CTAS)
 tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const void* __restrict__ q,
                     const u16* __restrict__ vcache, const uint32_t* __restrict__ block_table, const int* __restrict__ slot,
                     const int* __restrict__ ctxs, const int* __restrict__ row0s, const uint32_t* __restrict__ mask, void* __restrict__ out, int out_dtype,
                     Geo g, float scale, Scratch scr, int* __restrict__ status) {
   using SM = TcSmem<HD, QS>;
-  constexpr int NK = SM::NK, NV = SM::NV, NSUB = SM::NSUB, BLK = SM::BLK;
+  constexpr int NK = SM::NK, NV = SM::NV, NSUB = SM::NSUB, BLK = SM::BLK, TEAMS = Shape<HD>::TEAMS, THREADS = Shape<HD>::THREADS, CREW = 128 * TEAMS;      // crew: the softmax threads
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   // header: barriers at 0, flags at 256, (m, l) at 512 .. 2560; the operands behind it on a 1024-byte boundary
-  const uint32_t q_base = (raw + 2560 + 1023u) & ~1023u, stage_base = q_base + SM::Q_BYTES, k_ring = stage_base + SM::STAGE_BYTES, v_ring = k_ring + NK * BLK;
+  const uint32_t q_base = (raw + 2560 + 1023u) & ~1023u, stage_base = TEAMS == 2 ? q_base + SM::Q_BYTES : q_base, k_ring = q_base + SM::Q_BYTES + SM::STAGE_BYTES, v_ring = k_ring + NK * BLK;
   auto kfull = [&](int s) { return raw + 8u * s; };
   auto kempty = [&](int s) { return raw + 8u * (NK + s); };
   auto vfull = [&](int s) { return raw + 8u * (2 * NK + s); };
@@ -264,22 +278,22 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     for (int s = 0; s < NK; ++s) { mbar_init(kfull(s), 1); mbar_init(kempty(s), 1); }
     for (int s = 0; s < NV; ++s) { mbar_init(vfull(s), 1); mbar_init(vempty(s), 1); }
     for (int t = 0; t < 2; ++t) { mbar_init(s_full(t), 1); mbar_init(p_full(t), 4); mbar_init(o_done(t), 1); }
-    mbar_init(q_full, 4); mbar_init(q_first, 8);
+    mbar_init(q_full, 4); mbar_init(q_first, 4 * TEAMS);
     flags[1] = 0; flags[2] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(raw + 256), "r"(512u) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(raw + 256), "r"((uint32_t)Shape<HD>::TM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
   pdl_trigger();
   // ---- this CTA's share: prefix sums of the trees' items over the threads, a contiguous run of trees each
   {
-    int* sums = reinterpret_cast<int*>(ml_s);      // 10 warps
-    const int per = (g.n_trees + TC_THREADS - 1) / TC_THREADS, t0 = threadIdx.x * per, t1 = min(t0 + per, g.n_trees);
+    int* sums = reinterpret_cast<int*>(ml_s);
+    const int per = (g.n_trees + THREADS - 1) / THREADS, t0 = threadIdx.x * per, t1 = min(t0 + per, g.n_trees);
     int mine = 0;
     for (int t = t0; t < t1; ++t) mine += tree_items(g, tree_work(g, slot, ctxs, row0s, t));
     int scan = mine;
@@ -292,7 +306,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     __syncthreads();
     tc_fence_after();
     int before = 0, total = 0;
-    for (int w = 0; w < TC_THREADS / 32; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
+    for (int w = 0; w < THREADS / 32; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
     const int share = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     const int first = (int)blockIdx.x * share;
     int at = before + scan - mine;
@@ -313,7 +327,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const int share = flags[7], total = flags[8];
   const int group = g.q_heads / g.kv_heads, gshift = 31 - __clz(group);      // a power of two
   const bool none = walk.item >= walk.end;
-  if (threadIdx.x == 320) {      // (of the warp without a part) what the join has to know about the unit that this share begins in
+  if (threadIdx.x == THREADS - 64) {      // (of the warp without a part) what the join has to know about the unit that this share begins in
     ShareStart st{0, 0, share, total, 0, 0, 0, 0};
     if (!none) {
       Walk w = walk;
@@ -327,7 +341,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   }
   if (none) {
     // nothing to do
-  } else if (warp == 0 || warp == TC_THREADS / 32 - 1) {
+  } else if (warp == 0 || warp == THREADS / 32 - 1) {
     // ---------------- TMA: one warp for K, one for V; lane i brings the i-th box of a block ----------------
     const bool is_v = warp != 0;
     const uint32_t ring = is_v ? v_ring : k_ring;
@@ -375,7 +389,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int i = max(0, n - slots); i < n; ++i) bar_wait(is_v ? vfull(i % slots) : kfull(i % slots), (i / slots) & 1);      // copies in flight
     }
   } else if (warp == 1) {
-    // ---------------- MMA: S two blocks ahead, each P V as its team delivers P ----------------
+    // ---------------- MMA: S a block ahead for each team, each P V as its team delivers P ----------------
     if (lane == 0) {
       constexpr uint32_t ID_S = tc_idesc(KBLK, false), ID_O = tc_idesc(HD, true);
       using LY = Layout<HD>;
@@ -386,7 +400,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       while (ok && walk.next(g, slot, ctxs, row0s, p)) {
         const int len = p.b1 - p.b0;
         auto scores = [&](int j) {
-          const int i = n + j, s = i % NK;
+          const int i = n + j, s = i % NK, t = j % TEAMS;
           if (!bar_wait(kfull(s), (i / NK) & 1)) return false;
           tc_fence_after();
           const uint32_t kaddr = k_ring + s * BLK;
@@ -394,42 +408,42 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           for (int part = 0; part < QS; ++part)
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k)
-              umma_bf16(tmem + (j & 1) * 128, sdesc(q_base + part * BLK + (uint32_t)(k >> 2) * SUB + (uint32_t)(k & 3) * 32u, 16, 1024),
+              umma_bf16(tmem + t * 128, sdesc(q_base + part * BLK + (uint32_t)(k >> 2) * SUB + (uint32_t)(k & 3) * 32u, 16, 1024),
                         sdesc(kaddr + (uint32_t)(k >> 2) * LY::HALF + (uint32_t)(k & 3) * 32u, 16, LY::GROUP), ID_S, (part > 0 || k > 0) ? 1u : 0u);
-          umma_commit(s_full(j & 1));
+          umma_commit(s_full(t));
           umma_commit(kempty(s));
           return true;
         };
         ok = pieces == 0 ? bar_wait(q_first, 0) : bar_wait(q_full, (pieces - 1) & 1);
         ++pieces;
         ok = ok && scores(0);
-        if (len > 1) ok = ok && scores(1);
+        if (TEAMS == 2 && len > 1) ok = ok && scores(1);
         for (int j = 0; j < len && ok; ++j) {
-          const int t = j & 1, i = n + j, s = i % NV;
+          const int t = j % TEAMS, i = n + j, s = i % NV;
           ok = bar_wait(p_full(t), uses[t] & 1) && bar_wait(vfull(s), (i / NV) & 1);
           if (!ok) break;
           ++uses[t];
           tc_fence_after();
-          const uint32_t vaddr = v_ring + s * BLK, o_col = tmem + 256 + t * HD;
+          const uint32_t vaddr = v_ring + s * BLK, o_col = tmem + Shape<HD>::O_COL + t * HD;
           // 32 keys take 32 columns of P: 16 of the hi part (two keys a column), 16 of the lo part
 #pragma unroll
           for (int k = 0; k < KBLK / 16; ++k)
 #pragma unroll
             for (int part = 0; part < PS; ++part)
               mma_ts(o_col, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8, sdesc(vaddr + (uint32_t)k * 2u * LY::GROUP, LY::HALF, LY::GROUP), ID_O,
-                     (j > 1 || k > 0 || part > 0) ? 1u : 0u);
+                     (j >= TEAMS || k > 0 || part > 0) ? 1u : 0u);
           umma_commit(vempty(s));
           umma_commit(o_done(t));
-          if (j + 2 < len) ok = scores(j + 2);
+          if (j + TEAMS < len) ok = scores(j + TEAMS);
         }
         n += len;
       }
       if (!ok) { atomicExch(status, WKB_STATUS_ATTN_WAIT); flags[1] = 1; }
     }
-  } else if (warp < 10) {      // (warp 10 has no part: it makes the V warp the third of another scheduler)
+  } else if (warp < 2 + 4 * TEAMS) {      // (one more warp has no part: it makes the V warp another scheduler's)
     // ---------------- softmax teams ----------------
     const int team = (warp - 2) >> 2, quarter = warp & 3, a = quarter * 32 + lane, tid = threadIdx.x - 64;
-    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), s_col = lane_base + team * 128, o_col = lane_base + 256 + team * HD;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), s_col = lane_base + team * 128, o_col = lane_base + Shape<HD>::O_COL + team * HD;
     // scores in base 2; the sign of `scale` goes into the query; never 0, which would make NaN of a hidden key's -inf
     const float sc = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-37f);
     const bool negate = scale < 0.0f;
@@ -441,12 +455,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (lane == 0) { atomicExch(status, WKB_STATUS_ATTN_WAIT); flags[1] = 1; }
       }
     };
-    auto teams_sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };      // every softmax thread passes every one of these
+    auto teams_sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(CREW) : "memory"); };      // every softmax thread passes every one of these
     // The query operand (K-major, 128-byte swizzle).  The raw rows of the next piece come to the stage while this piece's
     // blocks are worked on (q_fetch), and the team that is not at work on the last block turns them into the operand's parts
     // and copies (q_put) as soon as that block's scores have been multiplied.  A thread reads back what it fetched itself.
-    // Rows beyond the stage (f32, head_dim 128, rows 64 and up) come when the first ones have left it.
-    constexpr int CH = HD / 8, RAW = 16 * (QS == 1 ? 1 : 2), KEPT = SM::STAGE_BYTES / RAW;      // chunks of 8 values a row, their bytes, chunks staged
+    // Rows beyond the stage (f32, head_dim 128, rows 64 and up) come when the first ones have left it.  A single team reads
+    // the rows where they lie, after its result is written.
+    constexpr int CH = HD / 8, RAW = 16 * (QS == 1 ? 1 : 2), KEPT = SM::STAGE / RAW;      // chunks of 8 values a row, their bytes, chunks staged
     auto live_of = [&](const Piece& p) { return min(QROWS, p.w.t.nodes * group - p.rowblk * QROWS); };
     auto copies_of = [&](int live) { return live <= 32 ? 4 : live <= 64 ? 2 : 1; };
     auto q_at = [&](const Piece& p, int idx) {
@@ -468,14 +483,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       const int live = live_of(p), copies = copies_of(live), crows = QROWS / copies;
       const uint32_t flip = negate ? 0x80008000u : 0u;
       for (int from = 0; from < crows * CH; from += KEPT) {
-        if (from > 0) q_fetch(p, from, self, threads);
+        if (TEAMS == 2 && from > 0) q_fetch(p, from, self, threads);
         asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 2
         for (int idx = from + self; idx < min(crows * CH, from + KEPT); idx += threads) {
           const int qr = idx / CH, c = idx % CH;
           float4 x[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
           if (qr < live) {
-            const float4* raw_q = reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(stage) + (idx - from) * RAW);
+            const float4* raw_q = reinterpret_cast<const float4*>(TEAMS == 2 ? reinterpret_cast<const uint8_t*>(stage) + (idx - from) * RAW : q_at(p, idx));
             x[0] = raw_q[0];
             if (QS > 1) x[1] = raw_q[1];
           }
@@ -508,14 +523,17 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     };
     Piece p, following;
     bool more = walk.next(g, slot, ctxs, row0s, following);
-    if (more) { q_fetch(following, 0, tid, 256); q_put(following, tid, 256, q_first); }
+    if (more) {
+      if (TEAMS == 2) q_fetch(following, 0, tid, CREW);
+      q_put(following, tid, CREW, q_first);
+    }
     while (more) {
       p = following;
       more = walk.next(g, slot, ctxs, row0s, following);
       const int len = p.b1 - p.b0;
       const int live = live_of(p), copies = copies_of(live), crows = QROWS / copies;
       const int copy = a / crows, r = a % crows;
-      const bool puts = more && team == (len & 1);      // the team without the last block
+      const bool puts = TEAMS == 2 && more && team == (len & 1);      // the team without the last block
       if (puts) q_fetch(following, 0, tid & 127, 128);
       // ---- the team's key blocks
       auto mask_of = [&](int row) { return mask + (i64)(p.w.t.row0 + ((p.rowblk * QROWS + row) >> gshift)) * g.mask_words; };
@@ -571,7 +589,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (__any_sync(0xffffffffu, move)) {
           const float next = move ? top : m;
           const float corr = move ? ex2(m - next) : 1.0f;      // 0 when nothing had been seen
-          if (j > 1) {      // the accumulator holds this team's earlier blocks
+          if (j >= TEAMS) {      // the accumulator holds this team's earlier blocks
             wait(o_done(team), (uses - 1) & 1);
             tc_fence_after();
 #pragma unroll 1
@@ -622,7 +640,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
         }
       };
-      for (int j = team; j < len; j += 2) {
+      for (int j = team; j < len; j += TEAMS) {
         wait(s_full(team), uses & 1);
         tc_fence_after();
         block(j);
@@ -666,15 +684,15 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
       // ---- the result: the teams' accumulators lie in the same lanes and are added in registers; the copies lie in other
       // lanes and are added through shared memory, 64 columns at a time
-      done[0] += (len + 1) >> 1;
-      done[1] += len >> 1;
+      done[0] += TEAMS == 2 ? (len + 1) >> 1 : len;
+      done[1] += TEAMS == 2 ? len >> 1 : 0;
       if (puts) {
         wait(s_full(team ^ 1), (done[team ^ 1] - 1) & 1);      // the last product with this piece's query is done
         q_put(following, tid & 127, 128, q_full);
       }
       ml_s[team * QROWS + a] = make_float2(team < len ? m : -INFINITY, team < len ? l : 0.0f);
       teams_sync();
-      const bool both = len > 1;      // team 1 had a block
+      const bool both = TEAMS == 2 && len > 1;      // team 1 had a block
       wait(o_done(0), (done[0] - 1) & 1);
       if (both) wait(o_done(1), (done[1] - 1) & 1);
       tc_fence_after();
@@ -727,13 +745,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       };
 #pragma unroll 1
       for (int c0 = 0; c0 < HD; c0 += 64) {
-        {
-          const int col = c0 + team * 32;
+#pragma unroll 1
+        for (int half = team; half < 2; half += TEAMS) {
+          const int col = c0 + half * 32;
           uint32_t o[32];
-          tm_ld32(lane_base + 256 + col, o);
+          tm_ld32(lane_base + Shape<HD>::O_COL + col, o);
           if (both) {
             uint32_t o1[32];
-            tm_ld32(lane_base + 256 + HD + col, o1);
+            tm_ld32(lane_base + Shape<HD>::O_COL + HD + col, o1);
             tm_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = f2u(ffma(u2f(o1[e]), w1, u2f(o[e]) * w0));
@@ -743,7 +762,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             for (int e = 0; e < 32; ++e) o[e] = f2u(u2f(o[e]) * w0);
           }
           if (staged) {
-            float4* d = reinterpret_cast<float4*>(stage + a * 64 + team * 32);
+            float4* d = reinterpret_cast<float4*>(stage + a * 64 + half * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[e ^ (a & 7)] = make_float4(u2f(o[4 * e]), u2f(o[4 * e + 1]), u2f(o[4 * e + 2]), u2f(o[4 * e + 3]));
           } else if (r < live && fine) {
@@ -763,14 +782,15 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         if (!staged) continue;
         teams_sync();
-        // a thread keeps its four columns and goes down the rows, 16 at a step (a multiple of the group)
+        // a thread keeps its four columns and goes down the rows, STEP at a time (a multiple of the group)
+        constexpr int STEP = CREW / 16;
         const int c4 = tid & 15, first = tid >> 4;
-        const i64 down = whole ? (i64)(16 >> gshift) * g.out_row_stride : (i64)16 * HD;
+        const i64 down = whole ? (i64)(STEP >> gshift) * g.out_row_stride : (i64)STEP * HD;
         i64 at = out_at(first) + c0 + c4 * 4;
         auto part = [&](int x) { return *reinterpret_cast<const float4*>(stage + x * 64 + ((c4 ^ (x & 7)) << 2)); };
         auto add = [](float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; };
 #pragma unroll 2
-        for (int row = first; row < live; row += 16, at += down) {
+        for (int row = first; row < live; row += STEP, at += down) {
           float4 v = part(row);
           if (copies > 1) add(v, part(row + crows));
           if (copies > 2) { add(v, part(row + 2 * crows)); add(v, part(row + 3 * crows)); }
@@ -785,6 +805,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       tc_fence_before();
       teams_sync();      // the accumulators, the stage and ml_s are free
+      if (TEAMS == 1 && more) q_put(following, tid, CREW, q_full);
     }
   }
   tc_fence_before();
@@ -792,7 +813,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Shape<HD>::TM_COLS) : "memory");
   }
 }
 
@@ -868,6 +889,7 @@ int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt,
   int* status = gemm_status_word();
   if (!status) return (int)cudaErrorMemoryAllocation;
   auto kern = tree_attn_tc_kernel<HD, QS, PS>;
+  using SH = Shape<HD>;
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -877,12 +899,12 @@ int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt,
     attr_set[dev & 63] = true;
   }
   const int group = g.q_heads / g.kv_heads;
-  const Scratch scr = carve(scratch, g.max_nodes, group);
-  cudaError_t e = launch_pdl(kern, WKB_SM_COUNT, TC_THREADS, (size_t)TcSmem<HD, QS>::BYTES, st, mk, mv, q, (const u16*)vc, bt, slot, ctx, row0, mask, out,
+  const Scratch scr = carve(scratch, g.max_nodes, group, SH::SHARES);
+  cudaError_t e = launch_pdl(kern, SH::SHARES, SH::THREADS, (size_t)TcSmem<HD, QS>::BYTES, st, mk, mv, q, (const u16*)vc, bt, slot, ctx, row0, mask, out,
                              out_dtype, g, scale, scr, status);
   if (e != cudaSuccess || !g.split) return (int)e;
   const int rows_per = 256 / (HD / 4);
-  return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(WKB_SM_COUNT - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, out, out_dtype, g, scr, (const int*)status);
+  return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(SH::SHARES - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, out, out_dtype, g, scr, (const int*)status);
 }
 
 }  // namespace tree
