@@ -207,8 +207,9 @@ __device__ __forceinline__ TreeWork tree_work(const Geo& g, const int* slot, con
   w.rowblks = (w.t.nodes * (g.q_heads / g.kv_heads) + QROWS - 1) / QROWS;      // 0 for a tree without rows
   return w;
 }
-// A unit counts as its blocks and UNIT_COST more: what beginning and ending one takes, in blocks.
-constexpr int UNIT_COST = 5;
+// A unit counts as its blocks and UNIT_COST more: what beginning and ending one takes, in blocks (0: 161 us, 2: 118, 3: 116,
+// 4: 114, 7: 118, 10: 123 for the 64 trees of a Llama-shape batch).
+constexpr int UNIT_COST = 4;
 __device__ __forceinline__ int unit_items(const Geo& g, const TreeWork& w) { return g.split ? w.blocks + UNIT_COST : 1; }
 __device__ __forceinline__ int tree_items(const Geo& g, const TreeWork& w) { return unit_items(g, w) * w.rowblks * g.kv_heads; }
 

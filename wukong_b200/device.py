@@ -297,9 +297,10 @@ def _on(dev, t, n, dtype, what):
 
 def _matrix(dev, t, cols, what):
     """(address, row pitch) of a matrix on device `dev` whose rows hold `cols` values."""
-    if t.dim() != 2 or t.shape[1] < cols or t.stride(1) != 1 or t.get_device() != dev:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] < cols or stride[1] != 1 or t.get_device() != dev:
         raise ValueError("%s must be a matrix of at least %d columns with unit column stride on the current CUDA device" % (what, cols))
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return t.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], shape[1])
 
 
 def _table(dev, t, mbps):
@@ -358,10 +359,12 @@ def token_probs(logits, temperature=None, out=None):
         raise ValueError("logits are f32 or bf16")
     px, ld = _matrix(dev, logits, cols, "logits")
     if out is None:
-        out = torch.empty((rows, cols), dtype=torch.float32, device=logits.device)
-    if out.dtype is not torch.float32 or out.shape != logits.shape:
-        raise ValueError("out must be f32 of the logits' shape")
-    po, ldo = _matrix(dev, out, cols, "out")
+        out = logits.new_empty((rows, cols), dtype=torch.float32)
+        po, ldo = out.data_ptr(), cols
+    else:
+        if out.dtype is not torch.float32 or out.shape != logits.shape:
+            raise ValueError("out must be f32 of the logits' shape")
+        po, ldo = _matrix(dev, out, cols, "out")
     check(lib().wkb_token_probs(px, dt, ld, None if temperature is None else _on(dev, temperature, rows, torch.float32, "temperature"), po, ldo, rows, cols,
                                 _raw_stream(dev)), "wkb_token_probs")
     return out
@@ -378,9 +381,7 @@ def tree_verify(probs, draft, token, parent, tree_row0, u_node, u_final, max_nod
     pp, ldp = _matrix(dev, probs, cols, "probs")
     pd, ldq = (None, 0) if draft is None else _matrix(dev, draft, cols, "draft")
     if out is None:
-        buf = torch.empty(n * (2 * max_path + 1), dtype=torch.int32, device=probs.device)
-        shape, pitch, part = (n, max_path), (max_path, 1), n * max_path
-        out = buf.as_strided(shape, pitch, 0), buf.as_strided((n,), (1,), 2 * part), buf.as_strided(shape, pitch, part)
+        out = probs.new_empty((n, max_path), dtype=torch.int32), probs.new_empty(n, dtype=torch.int32), probs.new_empty((n, max_path), dtype=torch.int32)
     path, n_path, tokens = out
     i32, f32 = torch.int32, torch.float32
     check(lib().wkb_tree_verify(pp, ldp, pd, ldq, _on(dev, token, rows, i32, "token"), _on(dev, parent, rows, i32, "parent"),
