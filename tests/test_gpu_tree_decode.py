@@ -177,6 +177,22 @@ def test_tree_attention_matches_f64(dev, shape, types):
     assert torch.equal(out, again), "run-to-run identical"
 
 
+@pytest.mark.parametrize("types", ["f32-f32", "f32-bf16", "bf16-bf16"])
+@pytest.mark.parametrize("hd,kvh,group,nodes", [(128, 8, 4, 16), (128, 4, 8, 61), (128, 8, 1, 5), (64, 12, 1, 16), (64, 6, 2, 100)])
+def test_tree_attention_batches_with_many_units(dev, hd, kvh, group, nodes, types):
+    """More units than the GPU works on at a time: a block of the kernel goes through several trees and heads, whole and in pieces."""
+    import torch
+    rng = np.random.default_rng(hd + nodes)
+    trees = [(int(c), int(n)) for c, n in zip(rng.integers(0, 1500, 48), rng.integers(1, nodes + 1, 48))]
+    tq, to = ({"f32": torch.float32, "bf16": torch.bfloat16}[t] for t in types.split("-"))
+    c = Case(dev, trees, kvh * group, kvh, hd, seed=nodes, q_dtype=tq, q_gain=2.0)
+    expected = c.expected()
+    for _ in range(3):
+        out = torch.full((c.rows, kvh * group * hd), 7.0, dtype=to, device="cuda")
+        c.run(dev, out)
+        c.check(out, expected)
+
+
 @pytest.mark.parametrize("masks", ["random", "sparse"])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_tree_attention_any_mask_and_rows_that_see_nothing(dev, masks, hd):

@@ -527,6 +527,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (more) {
       if (TEAMS == 2) q_fetch(following, 0, tid, CREW);
       q_put(following, tid, CREW, q_first);
+      if (TEAMS == 2) teams_sync();      // the stage is free for the next piece's rows
     }
     while (more) {
       p = following;
