@@ -337,7 +337,9 @@ int wkb_paged_kv_append(const float* ksrc, const float* vsrc, int64_t src_row_st
  * does not see never reaches its output, NaN included; a row that sees nothing gives zeros.  q and out: dtype 0 f32, 1 bf16,
  * row strides in elements, multiples of 8; all bases 16-byte aligned.  bf16 outputs carry bf16 softmax weights; f32 outputs
  * keep f32 accuracy.  head_dim in {64, 128}; q_heads / kv_heads in {1, 2, 4, 8}; page_tokens a power of two >= 4;
- * n_trees <= 4096.  A block-table entry >= num_pages reads as a page of zeros, positions past the table row are not seen.
+ * n_trees <= 4096, and trees x kv_heads x 128-row blocks x (128-key blocks of a table row + 4) < 2^31.  A block-table entry
+ * >= num_pages reads as a page of zeros, positions past the table row are not seen.  Call wkb_gemm_init once per device
+ * before the first call of this or of the commit is captured.  A bounded wait that runs out records 41 (wkb_gemm_status).
  * `scratch`: wkb_paged_attn_tree_scratch_bytes(...) bytes, uninitialised, one per stream (calls that may overlap need their
  * own, two captured graphs that may replay at the same time too). */
 int64_t wkb_paged_attn_tree_scratch_bytes(int64_t max_nodes, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
@@ -373,7 +375,7 @@ int wkb_tree_verify(const float* probs, int64_t ld_p, const float* draft_or_null
  * each), and new_ctx[t] (may be null, must not be tree_ctx) = tree_ctx[t] + n_path[t], the context of the next step.  A path must
  * ascend, and no two trees of a call may share a slot.  An entry that does not ascend, or whose positions lie past the
  * block-table row or the cache, ends that tree's moves and records 31 (wkb_gemm_status); trees that are switched off are
- * left alone. */
+ * left alone.  A layer's slab is at most 64 GB. */
 int wkb_paged_kv_commit(void* kcache, void* vcache, int64_t layers, int64_t layer_stride, int64_t num_pages, const uint32_t* block_table,
                         const int* tree_slot, const int* tree_ctx, const int* path, const int* n_path, int64_t max_path, int64_t n_trees,
                         int64_t kv_heads, int64_t head_dim, int64_t page_tokens, int64_t max_blocks_per_seq, int* new_ctx_or_null,
@@ -470,7 +472,7 @@ int wkb_gemm_bf16_nt_addto(const void* a, int64_t lda, const void* b, int64_t ld
 int wkb_gemm_b_static(int on);
 /* Reads and clears the library's device status word of the current device (synchronises): 0, or the code of the last
  * event -- 1-4 / 11-17 a bounded pipeline wait of the dense / W4A16 GEMM ran out, 21 the tensor-parallel reduce's flag
- * wait ran out (22: a peer had given up), 31 a KV append met a position past its block-table row (the row was skipped),
+ * wait ran out (22: a peer had given up), 31 a KV append met a position past its block-table row (the row was skipped) or a KV commit a bad path,
  * 41 a bounded wait on an asynchronous K/V copy of the paged attention ran out (that unit's output was not written).  The word is one per
  * device, shared by every stream and thread: concurrent users see each other's codes and the read clears them all. */
 int wkb_gemm_status(void);
