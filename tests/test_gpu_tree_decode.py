@@ -275,6 +275,28 @@ def test_tree_attention_context_past_the_table_row(dev):
     d.check(out)
 
 
+def test_cache_of_more_than_four_gigabytes(dev):
+    """Pages beyond 2^32 bytes of a slab, in the attention and in the commit."""
+    import torch
+    small = Case(dev, [(300, 12), (40, 5)], 8, 8, 128, seed=13)
+    pages = 150000                                        # x 8 heads x 16 tokens x 128 x 2 bytes = 4.9 GB a slab
+    big = dev.PagedKV(1, 1, 8, 128)
+    big.num_pages = pages
+    big.k, big.v = (torch.empty((1, pages, 8, 16, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    for at, used in ((pages - small.pages, small.kv), ):
+        big.k[0, at:at + small.pages] = used.k[0]
+        big.v[0, at:at + small.pages] = used.v[0]
+    expected = small.expected()
+    small.kv, small.table = big, small.table + pages - small.pages
+    out = torch.zeros((small.rows, 8 * 128), device="cuda")
+    small.run(dev, out)
+    small.check(out, expected)
+    page, off = int(small.table[0, (300 + 7) // 16]), (300 + 7) % 16
+    want = big.k[0, page, :, off].clone()
+    dev.paged_kv_commit(big, i32(small.table), i32([0, 1]), i32([300, 40]), i32([[0, 7, -1], [0, -1, -1]]), i32([2, 1]), small.mbps)
+    assert torch.equal(big.k[0, int(small.table[0, 301 // 16]), :, 301 % 16], want) and dev.gemm_status() == 0
+
+
 def test_tree_attention_one_chain_equals_decode(dev):
     """A chain's rows are ordinary decode rows with ctx + i + 1 visible keys."""
     import torch

@@ -35,7 +35,7 @@ constexpr int KBLK = 128, QROWS = 128, SUB = 128 * 128;
 
 // Header of the scratch: where share c begins, for the join.  Then (m, l) and O of two pieces a share.
 struct ShareStart {
-  int unit_start, unit_len, share, total, row0, live, head, rowblk;      // unit_len 0: it begins in none
+  int unit_start, unit_len, share, total, row0, live, head, rowblk;      // unit_len 0: it begins in none; total -1: a wait ran out
 };
 struct Scratch {
   ShareStart* start;
@@ -812,6 +812,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && flags[1]) scr.start[blockIdx.x].total = -1;
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -823,14 +824,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 // pieces (in key order) for these rows and write the result.  A row is HD / 4 lanes, which first share the pieces' (m, l)
 // out among them, so that the trips to L2 do not add up with the number of pieces.
 template <int HD>
-__global__ void __launch_bounds__(256) tree_attn_join_kernel(void* __restrict__ out, int out_dtype, Geo g, Scratch scr, const int* __restrict__ status) {
+__global__ void __launch_bounds__(256) tree_attn_join_kernel(void* __restrict__ out, int out_dtype, Geo g, Scratch scr) {
   pdl_wait();
   pdl_trigger();
   const int c = blockIdx.x + 1;
   const ShareStart st = scr.start[c];
-  const int failed = *status == WKB_STATUS_ATTN_WAIT;
   const int x = c * st.share;
-  if (x >= st.total || st.unit_len == 0 || x <= st.unit_start || x - st.share > st.unit_start || failed) return;
+  if (x >= st.total || st.unit_len == 0 || x <= st.unit_start || x - st.share > st.unit_start) return;
   const int last = (st.unit_start + st.unit_len - 1) / st.share, group = g.q_heads / g.kv_heads;
   constexpr int LANES = HD / 4;
   const int lane = threadIdx.x % LANES, row = blockIdx.y * (256 / LANES) + threadIdx.x / LANES, col = lane * 4;
@@ -838,7 +838,12 @@ __global__ void __launch_bounds__(256) tree_attn_join_kernel(void* __restrict__ 
   if (row >= st.live) return;      // (all lanes of a row)
   auto piece = [&](int k) { return (i64)(k * st.share >= st.unit_start ? 2 * k : 2 * k + 1) * scr.rows + row; };
   float m = -INFINITY;
-  for (int k = c - 1 + lane; k <= last; k += LANES) m = fmaxf(m, scr.ml[piece(k)].x);
+  bool failed = false;
+  for (int k = c - 1 + lane; k <= last; k += LANES) {
+    m = fmaxf(m, scr.ml[piece(k)].x);
+    failed |= scr.start[k].total < 0;
+  }
+  if (__any_sync(team, failed)) return;      // not all pieces were written
   for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(team, m, o, LANES));
   const float use = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
@@ -906,7 +911,7 @@ int launch_tc(const void* q, const void* kc, const void* vc, const uint32_t* bt,
                              out_dtype, g, scale, scr, status);
   if (e != cudaSuccess || !g.split) return (int)e;
   const int rows_per = 256 / (HD / 4);
-  return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(SH::SHARES - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, out, out_dtype, g, scr, (const int*)status);
+  return (int)launch_pdl(tree_attn_join_kernel<HD>, dim3(SH::SHARES - 1, (unsigned)((scr.rows + rows_per - 1) / rows_per)), 256, 0, st, out, out_dtype, g, scr);
 }
 
 }  // namespace tree
