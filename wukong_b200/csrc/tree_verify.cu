@@ -218,6 +218,8 @@ __global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restr
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int t = blockIdx.x / size, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)size * (PT / 32);
   const int a = min(max(row0[t], 0), rows), nodes = min(min(max(row0[t + 1], a), rows) - a, max_nodes);
+  float u = u_final[t];
+  u = u != u ? 0.0f : fminf(1.0f, fmaxf(0.0f, u));
   int* const my_path = path + (i64)t * max_path;
   int* const my_tokens = tokens + (i64)t * max_path;
   if (nodes <= 0) {      // (uniform over the cluster: nobody meets)
@@ -231,10 +233,10 @@ __global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restr
     for (int i = threadIdx.x; i < nodes; i += PT) {
       const int x = token[a + i], par = parent[a + i];
       const bool known = i > 0 && par >= 0 && par < nodes && x >= 0 && x < cols;
-      const float u = u_node[a + i];
+      const float un = u_node[a + i];
       tok_s[i] = x;
       par_s[i] = i > 0 ? par : -1;
-      u_s[i] = u != u ? 0.0f : fminf(1.0f, fmaxf(0.0f, u));
+      u_s[i] = un != un ? 0.0f : fminf(1.0f, fmaxf(0.0f, un));
       p_s[i] = known ? probs[(i64)(a + par) * ld_p + x] : 0.0f;
       q_s[i] = DRAFT && known ? draft[(i64)(a + par) * ld_q + x] : 0.0f;
     }
@@ -396,8 +398,6 @@ __global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restr
   const double total = __shfl_sync(0xffffffffu, up_to, 31);
   int pick = -1;
   if (total > 0.0) {
-    float u = u_final[t];
-    u = u != u ? 0.0f : fminf(1.0f, fmaxf(0.0f, u));
     double target = (double)u * total, base = up_to - own, before = 0.0;      // before: the mass in front of the run that this lane offers
     int offer = -1, last = -1;
 #pragma unroll
@@ -427,12 +427,14 @@ __global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restr
       __syncthreads();
       if (lane == 31) part_s[warp] = sum;
       __syncthreads();
-      double before = base;
-      for (int w = 0; w < PT / 32; ++w) {
-        if (w == warp) sum += before;
-        before += part_s[w];
+      double sums = lane < PT / 32 ? part_s[lane] : 0.0;      // running sums of the warps, lane w for warp w
+      for (int o = 1; o < PT / 32; o <<= 1) {
+        const double n = __shfl_up_sync(0xffffffffu, sums, o);
+        if (lane >= o) sums += n;
       }
-      base = before;
+      const double front = __shfl_sync(0xffffffffu, sums, warp > 0 ? warp - 1 : 0);
+      sum += warp > 0 ? base + front : base;
+      base += __shfl_sync(0xffffffffu, sums, PT / 32 - 1);
       if (r > 0.0) {
         if (sum > target) atomicMin(&pick_s[0], (int)i);
         atomicMax(&pick_s[1], (int)i);
