@@ -25,6 +25,7 @@
 #pragma once
 #include "common.cuh"
 #include "tc_common.cuh"
+#include <type_traits>
 
 namespace wkb {
 int* gemm_status_word();
@@ -559,9 +560,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       // One block, 32 columns at a time in rolled loops: the kernel is short enough that first executions of unrolled code
       // (instruction fetches) took longer than the work.  The last columns of the first pass stay in registers.
       const int chunks = 4 / copies, col0 = copy * chunks * 32;
-      auto block = [&](int j) {
+      auto block = [&](auto masked_c, int j) {
+        constexpr bool masked = decltype(masked_c)::value;      // some row does not see some key
         const int pos0 = (p.b0 + j) * KBLK + col0;
-        const bool masked = (p.b0 + j + 1) * KBLK > p.w.t.ctx;
         float s[32];
         auto load = [&](int c) {
           tm_ld32(s_col + col0 + c * 32, reinterpret_cast<uint32_t*>(s));
@@ -645,9 +646,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int j = team; j < len; j += TEAMS) {
         wait(s_full(team), uses & 1);
         tc_fence_after();
-        block(j);
+        const bool masked = (p.b0 + j + 1) * KBLK > p.w.t.ctx;
+        if (masked) block(std::true_type(), j);
+        else block(std::false_type(), j);
         // V of keys that some row does not see
-        if ((p.b0 + j + 1) * KBLK > p.w.t.ctx) {
+        if (masked) {
           const int i = n + j, sl = i % NV, row = quarter * 32 + lane;
           wait(vfull(sl), (i / NV) & 1);
           const uint32_t vrow = v_ring + sl * BLK + (uint32_t)(row >> 3) * Layout<HD>::GROUP + (uint32_t)(row & 7) * 128u;
