@@ -1,14 +1,18 @@
 """Build step: compile every CUDA source under csrc/ for sm_100a into one C-ABI shared library,
-in-tree (wukong_b200/libwukong_b200.so).  nvcc cross-compiles without a GPU."""
+in-tree (wukong_b200/libwukong_b200.so), and csrc/host/torch_calls.cpp -- calls on torch tensors that skip the Python level
+-- into an extension module beside it (wukong_b200/_torch_calls.so).  nvcc cross-compiles without a GPU."""
 import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libwukong_b200.so")
 OBJ = os.path.join(HERE, "build")
+CALLS = os.path.join(CSRC, "host", "torch_calls.cpp")
+CALLS_OUT = os.path.join(HERE, "_torch_calls.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -30,7 +34,33 @@ def needs_build():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def build_calls(force=False, verbose=False):
+    """The extension module of csrc/host: linked against torch and, beside it, the C-ABI library."""
+    header = os.path.join(HERE, "..", "include", "wukong_b200.h")
+    if not force and os.path.exists(CALLS_OUT) and os.path.getmtime(CALLS_OUT) > max(os.path.getmtime(p) for p in (CALLS, header, os.path.abspath(__file__))):
+        return CALLS_OUT
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I" + sysconfig.get_paths()["include"],
+           "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(cuda, "include"), CALLS,
+           "-o", CALLS_OUT, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + HERE, "-l:libwukong_b200.so",
+           "-Wl,-rpath,$ORIGIN:" + os.path.join(root, "lib")]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0 or verbose:
+        sys.stderr.write("== torch_calls.cpp\n%s\n" % r.stdout)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed")
+    return CALLS_OUT
+
+
 def build(force=False, verbose=False):
+    build_library(force, verbose)
+    build_calls(force, verbose)
+    return OUT
+
+
+def build_library(force=False, verbose=False):
     if not force and not needs_build():
         return OUT
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

@@ -3,7 +3,7 @@ is this library's own).  Thin wrappers over the `wkb_*` entry points of the C AB
 import numpy as np
 import torch
 
-from ._lib import lib, check, vp
+from ._lib import WukongB200Error, lib, check, vp
 
 
 def _s():
@@ -249,12 +249,22 @@ def paged_attn_decode_int8(q, q_row_stride, kv, layer, block_table, row_slot, ro
 
 # ---- speculative decoding: a tree of drafted tokens is checked in one step --------------------------------------------
 
-_TREE_DT = {torch.float32: 0, torch.bfloat16: 1}
+_calls_module = None
 
 
-def _raw_stream(dev):
-    """The current stream of device `dev` as an address, without building a torch.cuda.Stream."""
-    return torch._C._cuda_getCurrentRawStream(dev)
+def _calls():
+    """The extension module with these calls' checks and argument passing (csrc/host/torch_calls.cpp): they run once a layer
+    or once a step, often eagerly, and Python-level checks would take longer than the GPU."""
+    global _calls_module
+    if _calls_module is None:
+        lib()
+        try:
+            from . import _torch_calls
+        except ImportError as e:
+            raise WukongB200Error("the _torch_calls extension is missing or does not load (%s): run `python -m wukong_b200.build`" % e)
+        _torch_calls.set_error(WukongB200Error)
+        _calls_module = _torch_calls
+    return _calls_module
 
 
 def tree_layout(parent, row0):
@@ -278,47 +288,6 @@ def tree_layout(parent, row0):
     return mask.view(np.int32), depth
 
 
-# A decode step makes these calls once a layer or once a step, often eagerly, so the checks are kept to what a wrong call
-# would otherwise turn into a fault: types, extents, strides and the device.
-
-def _here(t):
-    dev = t.get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
-        raise ValueError("every tensor must lie on the current CUDA device")
-    return dev
-
-
-def _on(dev, t, n, dtype, what):
-    """A contiguous tensor of n values on device `dev`."""
-    if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError("%s must be a contiguous %s tensor of %d values on the current CUDA device" % (what, dtype, n))
-    return t.data_ptr()
-
-
-def _matrix(dev, t, cols, what):
-    """(address, row pitch) of a matrix on device `dev` whose rows hold `cols` values."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or shape[1] < cols or stride[1] != 1 or t.get_device() != dev:
-        raise ValueError("%s must be a matrix of at least %d columns with unit column stride on the current CUDA device" % (what, cols))
-    return t.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], shape[1])
-
-
-def _table(dev, t, mbps):
-    if t.dtype is not torch.int32 or mbps < 1 or t.numel() % mbps or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError("block_table must be a contiguous int32 [slots, mbps] on the current CUDA device")
-    return t.data_ptr()
-
-
-def _slabs(dev, kv):
-    k, v = kv.k, kv.v
-    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.get_device() != dev or v.get_device() != dev or \
-            not k.is_contiguous() or not v.is_contiguous():
-        raise ValueError("the cache must be contiguous bf16 on the current CUDA device")
-    if k.shape != (kv.layers, kv.num_pages, kv.kv_heads, kv.page_tokens, kv.head_dim) or v.shape != k.shape:
-        raise ValueError("the cache must be [layers, pages, kv_heads, page_tokens, head_dim]")
-    return k.data_ptr(), v.data_ptr(), k.stride(0)
-
-
 def paged_attn_tree_scratch(max_nodes, q_heads, kv_heads, head_dim, device="cuda"):
     return torch.empty(int(lib().wkb_paged_attn_tree_scratch_bytes(max_nodes, q_heads, kv_heads, head_dim)), dtype=torch.uint8, device=device)
 
@@ -326,81 +295,26 @@ def paged_attn_tree_scratch(max_nodes, q_heads, kv_heads, head_dim, device="cuda
 def paged_attn_tree(q, q_row_stride, kv, layer, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, q_heads, mbps, max_nodes, scale, scratch):
     """Attention of the nodes of draft trees over the paged bf16 cache (wkb_paged_attn_tree): row r = node i of tree t sees
     the tree_ctx[t] committed tokens and the nodes that its mask names.  q f32 or bf16, out f32 or bf16 [rows, q_heads * head_dim]."""
-    dev, n, rows, width = _here(out), tree_slot.numel(), out.shape[0], q_heads * kv.head_dim
-    tq, to = _TREE_DT.get(q.dtype), _TREE_DT.get(out.dtype)
-    if tq is None or to is None:
-        raise ValueError("q and out are f32 or bf16")
-    k, v, layer_stride = _slabs(dev, kv)
-    if not 0 <= layer < kv.layers:
-        raise ValueError("no such layer")
-    if q.get_device() != dev or (rows and (q.storage_offset() + (rows - 1) * q_row_stride + width) * q.element_size() > q.untyped_storage().nbytes()):
-        raise ValueError("q must hold %d rows of pitch %d on the current CUDA device" % (rows, q_row_stride))
-    words = tree_mask.shape[1] if tree_mask.dim() == 2 else 0
-    if tree_mask.shape[0] < rows:
-        raise ValueError("tree_mask must have a row for each row of out")
-    po, ldo = _matrix(dev, out, width, "out")
-    at = layer * layer_stride * 2
-    check(lib().wkb_paged_attn_tree(q.data_ptr(), tq, q_row_stride, k + at, v + at, kv.num_pages, _table(dev, block_table, mbps),
-                                    _on(dev, tree_slot, n, torch.int32, "tree_slot"), _on(dev, tree_ctx, n, torch.int32, "tree_ctx"),
-                                    _on(dev, tree_row0, n + 1, torch.int32, "tree_row0"),
-                                    _on(dev, tree_mask, tree_mask.shape[0] * words, torch.int32, "tree_mask"), words, po, to, ldo, rows, n, max_nodes,
-                                    q_heads, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps, scale,
-                                    _on(dev, scratch, scratch.numel(), torch.uint8, "scratch"), scratch.numel(), _raw_stream(dev)), "wkb_paged_attn_tree")
-    return out
+    return _calls().paged_attn_tree(q, q_row_stride, kv.k, kv.v, kv.layers, kv.num_pages, kv.kv_heads, kv.page_tokens, kv.head_dim, layer, block_table,
+                                    tree_slot, tree_ctx, tree_row0, tree_mask, out, q_heads, mbps, max_nodes, scale, scratch)
 
 
 def token_probs(logits, temperature=None, out=None):
     """f32 probabilities softmax(logits / temperature) of vocabulary rows; a temperature of 0 gives the greedy one-hot row
     (wkb_token_probs).  logits f32 or bf16 [rows, cols] (any row pitch), temperature f32 [rows]."""
-    dev = _here(logits)
-    rows, cols = logits.shape
-    dt = _TREE_DT.get(logits.dtype)
-    if dt is None:
-        raise ValueError("logits are f32 or bf16")
-    px, ld = _matrix(dev, logits, cols, "logits")
-    if out is None:
-        out = logits.new_empty((rows, cols), dtype=torch.float32)
-        po, ldo = out.data_ptr(), cols
-    else:
-        if out.dtype is not torch.float32 or out.shape != logits.shape:
-            raise ValueError("out must be f32 of the logits' shape")
-        po, ldo = _matrix(dev, out, cols, "out")
-    check(lib().wkb_token_probs(px, dt, ld, None if temperature is None else _on(dev, temperature, rows, torch.float32, "temperature"), po, ldo, rows, cols,
-                                _raw_stream(dev)), "wkb_token_probs")
-    return out
+    return _calls().token_probs(logits, temperature, out)
 
 
 def tree_verify(probs, draft, token, parent, tree_row0, u_node, u_final, max_nodes, max_path, out=None):
     """Accept / reject the drafted tokens of each tree and draw the token that follows (wkb_tree_verify).  probs, draft (or
     None): f32 [rows, vocabulary].  Returns (path int32 [n, max_path], n_path int32 [n], tokens int32 [n, max_path])."""
-    dev = _here(probs)
-    rows, cols = probs.shape
-    n = tree_row0.numel() - 1
-    if probs.dtype is not torch.float32 or (draft is not None and (draft.dtype is not torch.float32 or draft.shape != probs.shape)):
-        raise ValueError("probs and draft must be f32 of one shape")
-    pp, ldp = _matrix(dev, probs, cols, "probs")
-    pd, ldq = (None, 0) if draft is None else _matrix(dev, draft, cols, "draft")
-    if out is None:
-        out = probs.new_empty((n, max_path), dtype=torch.int32), probs.new_empty(n, dtype=torch.int32), probs.new_empty((n, max_path), dtype=torch.int32)
-    path, n_path, tokens = out
-    i32, f32 = torch.int32, torch.float32
-    check(lib().wkb_tree_verify(pp, ldp, pd, ldq, _on(dev, token, rows, i32, "token"), _on(dev, parent, rows, i32, "parent"),
-                                _on(dev, tree_row0, n + 1, i32, "tree_row0"), rows, n, max_nodes, cols, _on(dev, u_node, rows, f32, "u_node"),
-                                _on(dev, u_final, n, f32, "u_final"), _on(dev, path, n * max_path, i32, "path"),
-                                _on(dev, tokens, n * max_path, i32, "tokens"), _on(dev, n_path, n, i32, "n_path"), max_path, _raw_stream(dev)),
-          "wkb_tree_verify")
-    return path, n_path, tokens
+    path, n_path, tokens = out or (None, None, None)
+    return _calls().tree_verify(probs, draft, token, parent, tree_row0, u_node, u_final, max_nodes, max_path, path, n_path, tokens)
 
 
 def paged_kv_commit(kv, block_table, tree_slot, tree_ctx, path, n_path, mbps, new_ctx=None):
     """Move the accepted nodes' K / V to the positions behind the context, in every layer (wkb_paged_kv_commit); new_ctx
     (optional int32 [n], other memory than tree_ctx) receives the context of the next step."""
-    dev, n, i32 = _here(tree_slot), tree_slot.numel(), torch.int32
-    k, v, layer_stride = _slabs(dev, kv)
-    if path.dim() != 2 or path.shape[0] != n:
-        raise ValueError("path must be int32 [n, max_path]")
-    check(lib().wkb_paged_kv_commit(k, v, kv.layers, layer_stride, kv.num_pages, _table(dev, block_table, mbps), _on(dev, tree_slot, n, i32, "tree_slot"),
-                                    _on(dev, tree_ctx, n, i32, "tree_ctx"), _on(dev, path, n * path.shape[1], i32, "path"),
-                                    _on(dev, n_path, n, i32, "n_path"), path.shape[1], n, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps,
-                                    None if new_ctx is None else _on(dev, new_ctx, n, i32, "new_ctx"), _raw_stream(dev)), "wkb_paged_kv_commit")
+    _calls().paged_kv_commit(kv.k, kv.v, kv.layers, kv.num_pages, kv.kv_heads, kv.page_tokens, kv.head_dim, block_table, tree_slot, tree_ctx, path, n_path,
+                             mbps, new_ctx)
     return kv
