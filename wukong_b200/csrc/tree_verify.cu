@@ -13,6 +13,12 @@ constexpr int MAX_NODES = 256;
 // ---- temperature softmax --------------------------------------------------------------------------------------------
 __device__ __forceinline__ float logit(const float* x, int i) { return x[i]; }
 __device__ __forceinline__ float logit(const __nv_bfloat16* x, int i) { return bf16_bits_to_f32(reinterpret_cast<const u16*>(x)[i]); }
+// 2^x to 2^-22 of the result; 0 below 2^-126
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // log2(e) / t, finite and not 0, so that the maximum keeps weight 1 and a token that is ruled out weight 0
 __device__ __forceinline__ float exponent_scale(float t) { return t != t ? t : fmaxf(fminf(1.4426950408889634f / t, 3.402823466e+38f), 1e-37f); }
 
@@ -48,7 +54,7 @@ __global__ void __launch_bounds__(512) token_probs_wide_kernel(const T* __restri
   const float scale = exponent_scale(temp);
   float sum = 0.0f;
   if (temp > 0.0f) {
-    for (int i = threadIdx.x; i < cols; i += 512) sum += exp2f((logit(x + row * ld, i) - best) * scale);
+    for (int i = threadIdx.x; i < cols; i += 512) sum += ex2((logit(x + row * ld, i) - best) * scale);
     sum = warp_sum(sum);
     if (lane == 0) red_v[warp] = sum;
     __syncthreads();
@@ -59,7 +65,7 @@ __global__ void __launch_bounds__(512) token_probs_wide_kernel(const T* __restri
     float p;
     if (nan) p = NAN;
     else if (best == -INFINITY) p = 0.0f;                 // every token is ruled out
-    else if (temp > 0.0f) p = exp2f((logit(x + row * ld, i) - best) * scale) / sum;
+    else if (temp > 0.0f) p = ex2((logit(x + row * ld, i) - best) * scale) / sum;
     else p = i == at ? 1.0f : 0.0f;
     out[row * ld_out + i] = p;
   }
@@ -81,16 +87,18 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 constexpr int PT = 512;      // threads of a CTA
+// columns of a CTA when `ctas` share a row: whole 128-byte lines of f32
+__host__ __device__ __forceinline__ int probs_run(i64 cols, int ctas) { return (int)((cols + ctas - 1) / ctas + 31) / 32 * 32; }
 
-// A row is a cluster's: each CTA keeps its E * 512 columns in registers, so the logits are read once and the probabilities
+// A row is a cluster's: each CTA keeps up to E * 512 columns in registers, so the logits are read once and the probabilities
 // written once (HBM is the bound).  Every warp reduces its columns to (maximum, sum relative to it) and puts the pair into
 // every CTA's table; one cluster barrier later each warp adds up the whole table, so that nothing else is waited for
 // between the last load and the first store (block-wide reductions and a second barrier cost 65 us instead of 55 for
-// 1024 x 32000).  Element loads are 4 (2) bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no
-// more than that.
+// 1024 x 32000).  Loads and stores are 4 bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no more
+// than that, and where they are, 16 bytes a thread took longer (54 against 49 us).
 template <typename T, int E>
-__global__ void __launch_bounds__(PT, E > 32 ? 1 : 2) token_probs_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature,
-                                                                         float* __restrict__ out, i64 ld_out, int cols) {
+__global__ void __launch_bounds__(PT, E > 32 ? 1 : E > 8 ? 2 : 4) token_probs_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature,
+                                                                                                  float* __restrict__ out, i64 ld_out, int cols) {
   pdl_wait();
   pdl_trigger();
   __shared__ float2 table[8 * PT / 32];
@@ -98,12 +106,27 @@ __global__ void __launch_bounds__(PT, E > 32 ? 1 : 2) token_probs_kernel(const T
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const i64 row = blockIdx.x / size;
-  const int first = (int)rank * E * PT + threadIdx.x, mine = cols - first;      // column e * PT behind `first` exists below `mine`
-  const T* xr = x + row * ld + first;
+  // The CTAs' columns: equal runs of the row.  Of f32 a thread takes every PT-th one, of bf16 every PT-th pair in an aligned
+  // word, whose first pair may begin and whose last may end a column outside the run.
+  constexpr int PAIR = sizeof(T) == 2 ? 2 : 1;
+  const int run = probs_run(cols, (int)size), start = (int)rank * run, end = min(cols, start + run);
+  const T* xr = x + row * ld + start;
+  const int shift = PAIR == 2 ? (int)((reinterpret_cast<uintptr_t>(xr) >> 1) & 1) : 0, first = start - shift + PAIR * (int)threadIdx.x;
+  const int mine = end - first;      // column at(e) behind `first` is this CTA's below `mine`, and not in front of the run
+  auto at = [](int e) { return e / PAIR * PAIR * PT + e % PAIR; };
+  auto own = [&](int e) { return at(e) < mine && (e > 0 || first >= start); };
+  xr += first - start;
   float* const o = out + row * ld_out + first;
   float v[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = e * PT < mine ? logit(xr, e * PT) : -INFINITY;
+  for (int e = 0; e < E; e += PAIR) {
+    if (PAIR == 1) v[e] = own(e) ? logit(xr, at(e)) : -INFINITY;
+    else {
+      const uint32_t w = at(e) < mine ? *reinterpret_cast<const uint32_t*>(xr + at(e)) : 0u;
+      v[e] = own(e) ? u2f(w << 16) : -INFINITY;
+      v[e + PAIR - 1] = at(e + PAIR - 1) < mine ? u2f(w & 0xffff0000u) : -INFINITY;
+    }
+  }
   const float temp = temperature ? temperature[row] : 1.0f;
   const bool cold = temp <= 0.0f;      // alike in all CTAs of the row
   const float scale = exponent_scale(temp);
@@ -112,31 +135,31 @@ __global__ void __launch_bounds__(PT, E > 32 ? 1 : 2) token_probs_kernel(const T
   for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
   float base;
   if (cold) {
-    int at = 0x7fffffff;
+    int col = 0x7fffffff;
     bool nan = false;
 #pragma unroll
     for (int e = E - 1; e >= 0; --e) {
-      if (v[e] == m && e * PT < mine) at = first + e * PT;
+      if (v[e] == m && own(e)) col = first + at(e);
       nan |= v[e] != v[e];
     }
     for (int k = 16; k > 0; k >>= 1) {
       const float om = __shfl_xor_sync(0xffffffffu, m, k);
-      const int oa = __shfl_xor_sync(0xffffffffu, at, k);
-      if (om > m || (om == m && oa < at)) { m = om; at = oa; }
+      const int oc = __shfl_xor_sync(0xffffffffu, col, k);
+      if (om > m || (om == m && oc < col)) { m = om; col = oc; }
     }
     if (__any_sync(0xffffffffu, nan)) m = NAN;
     base = 0.0f;
-    second = __int_as_float(at);
+    second = __int_as_float(col);
   } else {
     base = m == -INFINITY ? 0.0f : m;
     second = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      v[e] = exp2f((v[e] - base) * scale);      // a NaN spoils the sum and with it the row
+      v[e] = ex2((v[e] - base) * scale);      // a NaN spoils the sum and with it the row
       second += v[e];
     }
     const float mw = warp_max(m);
-    second = warp_sum(m == -INFINITY ? second : second * exp2f((m - mw) * scale));
+    second = warp_sum(m == -INFINITY ? second : second * ex2((m - mw) * scale));
     m = mw;
   }
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
@@ -150,22 +173,22 @@ __global__ void __launch_bounds__(PT, E > 32 ? 1 : 2) token_probs_kernel(const T
   if (cold) {
     bool nan = false;
     float top = -INFINITY;
-    int at = 0x7fffffff;
+    int col = 0x7fffffff;
     for (int k = lane; k < entries; k += 32) {
       const float2 p = table[k];
       nan |= p.x != p.x;
-      if (p.x > top || (p.x == top && __float_as_int(p.y) < at)) { top = p.x; at = __float_as_int(p.y); }
+      if (p.x > top || (p.x == top && __float_as_int(p.y) < col)) { top = p.x; col = __float_as_int(p.y); }
     }
     for (int k = 16; k > 0; k >>= 1) {
       const float om = __shfl_xor_sync(0xffffffffu, top, k);
-      const int oa = __shfl_xor_sync(0xffffffffu, at, k);
-      if (om > top || (om == top && oa < at)) { top = om; at = oa; }
+      const int oc = __shfl_xor_sync(0xffffffffu, col, k);
+      if (om > top || (om == top && oc < col)) { top = om; col = oc; }
     }
-    if (top == -INFINITY) at = -1;      // every token is ruled out
+    if (top == -INFINITY) col = -1;      // every token is ruled out
     nan = __any_sync(0xffffffffu, nan);
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (e * PT < mine) o[e * PT] = nan ? NAN : first + e * PT == at ? 1.0f : 0.0f;
+      if (own(e)) o[at(e)] = nan ? NAN : first + at(e) == col ? 1.0f : 0.0f;
     return;
   }
   float top = -INFINITY, l = 0.0f;
@@ -173,14 +196,25 @@ __global__ void __launch_bounds__(PT, E > 32 ? 1 : 2) token_probs_kernel(const T
   top = warp_max(top);
   for (int k = lane; k < entries; k += 32) {
     const float2 p = table[k];
-    l += p.x == -INFINITY ? p.y : p.y * exp2f((p.x - top) * scale);
+    l += p.x == -INFINITY ? p.y : p.y * ex2((p.x - top) * scale);
   }
   l = warp_sum(l);
-  const float own = (base - top) * scale;      // this thread's exponentials are relative to its own maximum
-  const float f = top == -INFINITY ? (l == l ? 0.0f : NAN) : (mine > 0 && base <= top ? exp2f(own) : 1.0f) / l;
+  const float behind = (base - top) * scale;      // this thread's exponentials are relative to its own maximum
+  const float f = top == -INFINITY ? (l == l ? 0.0f : NAN) : (mine > 0 && base <= top ? ex2(behind) : 1.0f) / l;
+  if (PAIR == 2 && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {      // stores of half pairs would be masked sectors, twice as many
+#pragma unroll
+    for (int e = 0; e < E; e += PAIR) {
+      if (own(e) && at(e + 1) < mine) *reinterpret_cast<float2*>(o + at(e)) = make_float2(v[e] * f, v[e + PAIR - 1] * f);
+      else {
+        if (own(e)) o[at(e)] = v[e] * f;
+        if (at(e + PAIR - 1) < mine) o[at(e + PAIR - 1)] = v[e + PAIR - 1] * f;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e)
-    if (e * PT < mine) o[e * PT] = v[e] * f;
+    if (own(e)) o[at(e)] = v[e] * f;
 }
 
 // ---- verification ---------------------------------------------------------------------------------------------------
@@ -531,14 +565,14 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsig
 
 // A row's columns over the CTAs of a cluster and the registers of their threads: clusters grow until two CTAs per SM are
 // at work (small batches) and a thread holds at most 32 columns (large vocabularies), or at 8.
-constexpr i64 PROBS_MAX = 8 * 64 * (i64)PT;
+constexpr i64 PROBS_MAX = 8 * (64 * (i64)PT - 32);      // (a run of bf16 may begin with half a pair)
 struct ProbsShape {
   int ctas, regs;
 };
 static ProbsShape probs_shape(i64 rows, i64 cols) {
   ProbsShape s{1, 4};
   while (s.ctas < 8 && (cols > (i64)s.ctas * 32 * PT || (rows * s.ctas < 2 * WKB_SM_COUNT && cols > (i64)s.ctas * 4 * PT))) s.ctas *= 2;
-  while (s.regs < 64 && (i64)s.ctas * s.regs * PT < cols) s.regs *= 2;
+  while (s.regs < 64 && s.regs * PT < probs_run(cols, s.ctas) + 1) s.regs *= 2;
   return s;
 }
 template <typename T>
