@@ -267,7 +267,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   auto o_done = [&](int t) { return more + 8u * (4 + t); };
   const uint32_t q_full = more + 8u * 6, q_first = more + 8u * 7;      // the first piece's query is everybody's work
   static_assert(8 * (2 * NK + 2 * NV + 8) <= 256, "barriers fit the header");
-  volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + 256);      // 0 tensor memory, 1 failed, 2 V not finite, 3.. the share
+  volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + 256);      // 0 tensor memory, 1 failed, 2 V not finite, 3 and 4 the share's first tree and its start
   float2* ml_s = reinterpret_cast<float2*>(smem_raw + 512);
   float* stage = reinterpret_cast<float*>(smem_raw + (stage_base - raw));
 
@@ -290,10 +290,31 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(raw + 256), "r"((uint32_t)Shape<HD>::TM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)flags[0];
   pdl_wait();
   pdl_trigger();
-  // ---- this CTA's share: prefix sums of the trees' items over the threads, a contiguous run of trees each
-  {
+  // ---- this CTA's share: prefix sums of the trees' items.  Up to 32 trees every warp for itself, which saves the barriers;
+  // more over all threads, a contiguous run of trees each
+  int share, total;
+  Walk walk;
+  if (g.n_trees <= 32) {
+    const int mine = lane < g.n_trees ? tree_items(g, tree_work(g, slot, ctxs, row0s, lane)) : 0;
+    int scan = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    total = __shfl_sync(0xffffffffu, scan, 31);
+    share = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    walk.item = min((int)blockIdx.x * share, total);
+    walk.end = min(walk.item + share, total);
+    const int t = __ffs(__ballot_sync(0xffffffffu, walk.item < scan)) - 1;      // -1: nothing to do
+    walk.tree = max(t, 0);
+    walk.tree_start = __shfl_sync(0xffffffffu, scan - mine, walk.tree);
+  } else {
     int* sums = reinterpret_cast<int*>(ml_s);
     const int per = (g.n_trees + THREADS - 1) / THREADS, t0 = threadIdx.x * per, t1 = min(t0 + per, g.n_trees);
     int mine = 0;
@@ -304,12 +325,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (lane >= o) scan += v;
     }
     if (lane == 31) sums[warp] = scan;
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    int before = 0, total = 0;
+    int before = 0;
+    total = 0;
     for (int w = 0; w < THREADS / 32; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
-    const int share = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    share = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     const int first = (int)blockIdx.x * share;
     int at = before + scan - mine;
     if (first < total && first >= at && first < at + mine) {
@@ -321,12 +341,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       flags[3] = t; flags[4] = at;
     }
-    if (threadIdx.x == 0) { flags[5] = min(first, total); flags[6] = min(first + share, total); flags[7] = share; flags[8] = total; }
     __syncthreads();
+    walk = Walk{min(first, total), min(first + share, total), flags[3], flags[4]};
   }
-  const uint32_t tmem = (uint32_t)flags[0];
-  Walk walk{flags[5], flags[6], flags[3], flags[4]};
-  const int share = flags[7], total = flags[8];
   const int group = g.q_heads / g.kv_heads, gshift = 31 - __clz(group);      // a power of two
   const bool none = walk.item >= walk.end;
   if (threadIdx.x == THREADS - 64) {      // (of the warp without a part) what the join has to know about the unit that this share begins in
