@@ -57,8 +57,9 @@ def attn(L, **over):
 @pytest.mark.parametrize("over,code", [
     (dict(qh=3), BAD), (dict(qh=12), BAD), (dict(qh=32, kvh=2), BAD), (dict(kvh=0), BAD), (dict(hd=96), BAD), (dict(hd=256), BAD), (dict(page=2), BAD), (dict(page=24), BAD), (dict(page=0), BAD),
     (dict(nodes=0), BAD), (dict(nodes=257, words=9), BAD), (dict(nodes=65), BAD), (dict(n=4097), BAD), (dict(mbps=0), BAD), (dict(pages=0), BAD), (dict(qd=2), BAD), (dict(od=3), BAD),
-    (dict(pages=1 << 30), BAD), (dict(mbps=1 << 28), BAD), (dict(scratch=None), BAD), (dict(size=0), BAD), (dict(rows=1 << 40), BAD),
-    (dict(qs=516), MISALIGNED), (dict(os=4), MISALIGNED), (dict(q=P + 4), MISALIGNED), (dict(k=P + 8), MISALIGNED), (dict(v=P + 2), MISALIGNED), (dict(out=P + 8), MISALIGNED),
+    (dict(pages=1 << 30), BAD), (dict(mbps=1 << 28), BAD), (dict(scratch=None), BAD), (dict(size=0), BAD), (dict(rows=1 << 40), BAD), (dict(qs=-8), BAD), (dict(os=504), BAD), (dict(os=-512, rows=1), BAD),
+    (dict(n=4096, kvh=8, qh=64, nodes=256, words=8, mbps=1 << 20), BAD),
+    (dict(qs=516), MISALIGNED), (dict(os=516), MISALIGNED), (dict(q=P + 4), MISALIGNED), (dict(k=P + 8), MISALIGNED), (dict(v=P + 2), MISALIGNED), (dict(out=P + 8), MISALIGNED),
     (dict(scratch=P + 4), MISALIGNED)])
 def test_attention_refusals(L, over, code):
     assert attn(L, **over) == code

@@ -33,7 +33,8 @@ __device__ __forceinline__ TreeRef tree_ref(const Geo& g, const int* __restrict_
   return r;
 }
 
-// One warp per (row, query head).  32 keys at a time: a lane scores one key, then the lanes turn to the head's
+// For pages of 4 tokens, which fill no swizzle atom of the tensor-core kernel's operands.  One warp per (row, query head),
+// bound by the latency of its loads (5.7 ms where the tensor-core kernel takes 0.12, 64 Llama-shape trees).  32 keys at a time: a lane scores one key, then the lanes turn to the head's
 // dimensions and add the visible keys' values one after the other.  A key that a row does not see is skipped, so
 // whatever its V holds stays out of the sum.
 template <int HD>
@@ -151,6 +152,7 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void
     return (int)cudaErrorInvalidValue;
   if (num_pages > 0x7fffff00 / (kv_heads * page_tokens)) return (int)cudaErrorInvalidValue;
   if ((q_dtype != 0 && q_dtype != 1) || (out_dtype != 0 && out_dtype != 1)) return (int)cudaErrorInvalidValue;
+  if (q_row_stride < 0 || out_row_stride < 0 || (rows > 1 && out_row_stride < q_heads * head_dim)) return (int)cudaErrorInvalidValue;      // result rows do not overlap
   if (q_row_stride % 8 != 0 || out_row_stride % 8 != 0) return (int)cudaErrorMisalignedAddress;
   if (((((uintptr_t)q) | ((uintptr_t)kcache) | ((uintptr_t)vcache) | ((uintptr_t)out) | ((uintptr_t)scratch)) & 15) != 0) return (int)cudaErrorMisalignedAddress;
   if (!scratch || scratch_bytes < wkb_paged_attn_tree_scratch_bytes(max_nodes, q_heads, kv_heads, head_dim)) return (int)cudaErrorInvalidValue;

@@ -2,17 +2,24 @@
 //
 // Work.  A unit is (tree, KV head, 128 of the tree's query rows, node-major with the heads of the group inside); its
 // keys are cut into blocks of 128.  All blocks of all units form one list that is dealt out in equal contiguous shares to
-// as many CTAs as the SMs hold, whatever the lengths: a share may hold several units, or a piece of one.  A unit that a single share
-// covers is written at once; the pieces of the others go to scratch as (maximum, sum, unnormalised output) and are
-// joined by tree_attn_join_kernel in key order, so results are run-to-run identical.  When the arguments say that there are
-// no more units than SMs and that they are short, units stay whole and nothing is joined.
+// as many CTAs as the SMs hold, whatever the lengths: a share may hold several units, or a piece of one.  A unit that a
+// single share covers is written at once; the pieces of the others go to scratch as (maximum, sum, unnormalised output) and
+// are joined by tree_attn_join_kernel in key order, so results are run-to-run identical.  When the arguments say that there
+// are no more units than CTAs and that they are short, units stay whole and nothing is joined.
 //
-// A CTA has two TMA warps (pages of K and of V into a ring each), an MMA warp and two teams of four softmax warps.  The teams take
-// alternate key blocks with tensor-memory columns of their own, so one team's exponentials run while the other's products
-// do:   S = Q K^T (128 x 128) -> P = exp2(S - m), bf16, over the same columns -> O += P V (128 x head_dim).
-// The running maximum m of a row moves only when a block exceeds it by 2^8; the accumulator is rescaled then and not at
-// every block.  f32 queries are two bf16 parts (hi + lo, two products); for f32 results P
-// is two parts as well (5e-6 of the result over 8192 keys, of which the products' accumulation is the larger share).
+// A CTA has two TMA warps (pages of K and of V into a ring each), an MMA warp and one or two teams of four softmax warps.
+//   S = Q K^T (128 x 128) -> P = exp2(S - m), bf16, over the same columns -> O += P V (128 x head_dim)
+// Two teams take alternate key blocks with tensor-memory columns of their own, so one team's exponentials run while the
+// other's products do; a single team leaves that to the SM's other CTA.  The running maximum m of a row moves only when a
+// block exceeds it by 2^8; the accumulator is rescaled then and not at every block.  f32 queries are two bf16 parts (hi +
+// lo, two products); for f32 results P is two parts as well (5e-6 of the result over 8192 keys, of which the products'
+// accumulation is the larger share).
+//
+// Bound.  K and V are read once from HBM (569.9 MB for 571.6 MB of work in the Llama-shape batch of 64 trees) and stream at
+// the copy rate inside a unit: 1.41 us a block of head_dim 128 on all SMs together, 0.79 us of head_dim 64.  The batch takes 118 us
+// against 87 us of its bytes; the rest is the beginnings and ends of units (8 k cycles each, partly under the rings'
+// prefetch), the first trip to memory and the join (4 us).  With 128 rows a unit it is the chain S -> softmax -> P V of
+// the teams, 2200 cycles a block against 1330 of the tensor pipe and the shared-memory port.
 //
 // With 64 (32) query rows or fewer the operand's 128 rows hold 2 (4) copies of them, and each copy takes its own half
 // (quarter) of a block's keys, with zeros for the others': a team's warps share the exponentials of a small tree that

@@ -93,8 +93,8 @@ __host__ __device__ __forceinline__ int probs_run(i64 cols, int ctas) { return (
 // A row is a cluster's: each CTA keeps up to E * 512 columns in registers, so the logits are read once and the probabilities
 // written once (HBM is the bound).  Every warp reduces its columns to (maximum, sum relative to it) and puts the pair into
 // every CTA's table; one cluster barrier later each warp adds up the whole table, so that nothing else is waited for
-// between the last load and the first store (block-wide reductions and a second barrier cost 65 us instead of 55 for
-// 1024 x 32000).  Loads and stores are 4 bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no more
+// between the last load and the first store (with block-wide reductions and a second barrier 1024 x 32000 took 65 us,
+// now 48, 0.84 of the copy rate).  Loads and stores are 4 bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no more
 // than that, and where they are, 16 bytes a thread took longer (54 against 49 us).
 template <typename T, int E>
 __global__ void __launch_bounds__(PT, E > 32 ? 1 : E > 8 ? 2 : 4) token_probs_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature,
@@ -233,7 +233,8 @@ struct alignas(16) Ask {
 // rejection (before the next sibling is tried) and the final draw need a pass over the vocabulary, a contiguous run of
 // columns per warp of the cluster; the row is read from HBM once and the run that holds the draw a second time, from L2.
 // The leader alone decides, so every CTA takes the same steps.  Sums are in a fixed order.  Bound: the latency of the four
-// dependent trips to memory for a few trees, the rows' bytes for many.
+// dependent trips to memory for a few trees (8.2 us for one chain over 50257 columns, 5 of them a warp's instructions and
+// barriers), the longest walk's passes for many (27 us for 64 trees over 32000).
 constexpr int HOLD = 16;
 template <bool DRAFT>
 __global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restrict__ probs, i64 ld_p, const float* __restrict__ draft, i64 ld_q,
@@ -489,7 +490,8 @@ __global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restr
 // The K / V rows of node path[i] (i >= 1) move from position ctx + path[i] to ctx + i, eight nodes at a time: their
 // look-ups, then for each 16 bytes of a token's rows in all layers the loads and the stores.  The grid is bounded, so that
 // the four dependent look-ups of a block are paid once for several of its elements.  A path ascends, so path[j] > i for j > i: a row that is
-// written was read before, in this round or an earlier one.  Bound: HBM for many sequences, two dependent trips for one.
+// written was read before, in this round or an earlier one.  Bound: HBM in 256-byte pieces for many sequences (10 us
+// for 64 of 32 layers), dependent trips for one (3.5 us).
 __global__ void __launch_bounds__(256, 3) kv_commit_kernel(uint4* __restrict__ kc, uint4* __restrict__ vc, i64 layer_stride, i64 num_pages,
                                                         const uint32_t* __restrict__ block_table, const int* __restrict__ slots,
                                                         const int* __restrict__ ctxs, const int* __restrict__ path, const int* __restrict__ n_path,
