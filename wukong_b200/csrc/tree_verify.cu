@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(PT, 2) tree_verify_kernel(const float* __restr
 // The K / V rows of node path[i] (i >= 1) move from position ctx + path[i] to ctx + i, eight nodes at a time: their
 // look-ups, then for each 16 bytes of a token's rows in all layers the loads and the stores.  The grid is bounded, so that
 // the four dependent look-ups of a block are paid once for several of its elements.  A path ascends, so path[j] > i for j > i: a row that is
-// written was read before, in this round or an earlier one.  Bound: HBM in 256-byte pieces for many sequences (10 us
+// written was read before, in this batch or an earlier one.  Bound: HBM in 256-byte pieces for many sequences (10 us
 // for 64 of 32 layers), dependent trips for one (3.5 us).
 __global__ void __launch_bounds__(256, 3) kv_commit_kernel(uint4* __restrict__ kc, uint4* __restrict__ vc, i64 layer_stride, i64 num_pages,
                                                         const uint32_t* __restrict__ block_table, const int* __restrict__ slots,
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(256, 3) kv_commit_kernel(uint4* __restrict__ k
   for (int i0 = 1; i0 < n; i0 += BATCH) {
     int node[BATCH];
     uint32_t from[BATCH], to[BATCH];      // in 16-byte units, of the first head
-    int good = 0;      // entries of this round that belong to a path
+    int good = 0;      // entries of this batch that belong to a path
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) node[k] = i0 + k < n ? path[(i64)t * max_path + i0 + k] : -1;
 #pragma unroll
