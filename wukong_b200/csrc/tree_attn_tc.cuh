@@ -95,7 +95,7 @@ inline int shares_of(i64 hd) { return hd == 64 ? Shape<64>::SHARES : Shape<128>:
 template <int HD, int QS>
 struct TcSmem {
   static constexpr int NSUB = HD / 64, BLK = NSUB * SUB;                 // bytes of 128 rows of an operand
-  static constexpr int HEADER = 3072;                                    // barriers, (m, l) of the teams, flags
+  static constexpr int HEADER = 3 * 1024;                                  // barriers, (m, l) of the teams, flags
   // the stage (the copies' sums, and the next query's raw rows): of its own beside two teams; a single team's lies over the
   // query, which is not needed when a result is written
   static constexpr int TEAMS = Shape<HD>::TEAMS, STAGE = QROWS * 64 * 4, STAGE_BYTES = TEAMS == 2 ? STAGE : 0;
@@ -224,7 +224,7 @@ __device__ __forceinline__ int tree_items(const Geo& g, const TreeWork& w) { ret
 // One piece of a unit: blocks [b0, b1) of `unit_len`.
 struct Piece {
   TreeWork w;
-  int tree, head, rowblk, unit_start, b0, b1;
+  int head, rowblk, unit_start, b0, b1;
 };
 // Walks a share: item is its position in the list, tree_start that of tree `tree`.
 struct Walk {
@@ -239,7 +239,6 @@ struct Walk {
         if (++tree >= g.n_trees) return false;
       }
       const int size = unit_items(g, p.w), unit = (item - tree_start) / size;
-      p.tree = tree;
       p.head = unit / p.w.rowblks;
       p.rowblk = unit - p.head * p.w.rowblks;
       p.unit_start = tree_start + unit * size;
