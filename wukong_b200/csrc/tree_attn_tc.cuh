@@ -8,7 +8,7 @@
 // are no more units than CTAs and that they are short, units stay whole and nothing is joined.
 //
 // A CTA has two TMA warps (pages of K and of V into a ring each), an MMA warp and one or two teams of four softmax warps.
-//   S = Q K^T (128 x 128) -> P = exp2(S - m), bf16, over the same columns -> O += P V (128 x head_dim)
+//   S = Q K^T (128 x 128) -> P = exp2(S - m), bf16 -> O += P V (128 x head_dim)      (P over S, or beside it where there is room)
 // Two teams take alternate key blocks with tensor-memory columns of their own, so one team's exponentials run while the
 // other's products do; a single team leaves that to the SM's other CTA.  The running maximum m of a row moves only when a
 // block exceeds it by 2^8; the accumulator is rescaled then and not at every block.  f32 queries are two bf16 parts (hi +
@@ -16,7 +16,7 @@
 // accumulation is the larger share).
 //
 // Bound.  K and V are read once from HBM (569.9 MB for 571.6 MB of work in the Llama-shape batch of 64 trees) and stream at
-// the copy rate inside a unit: 1.41 us a block of head_dim 128 on all SMs together, 0.79 us of head_dim 64.  The batch takes 118 us
+// the copy rate inside a unit: 1.41 us a block of head_dim 128 on all SMs together, 0.72 us of head_dim 64.  The batch takes 118 us
 // against 87 us of its bytes; the rest is the beginnings and ends of units (8 k cycles each, partly under the rings'
 // prefetch), the first trip to memory and the join (4 us).  With 128 rows a unit it is the chain S -> softmax -> P V of
 // the teams, 2200 cycles a block against 1330 of the tensor pipe and the shared-memory port.
@@ -258,6 +258,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     const int* __restrict__ ctxs, const int* __restrict__ row0s, const uint32_t* __restrict__ mask, void* __restrict__ out, int out_dtype,
                     Geo g, float scale, Scratch scr, int* __restrict__ status) {
   using SM = TcSmem<HD, QS>;
+  // Tensor memory: with one team and one part of P there is room for P beside S, so that the next block's scores need not wait
+  // for this block's P V; else P lies over S, 32 columns (16 of each part) for 32 keys.
+  constexpr bool BESIDE = Shape<HD>::TEAMS == 1 && PS == 1;
+  constexpr int P_BASE = BESIDE ? Shape<HD>::O_COL + HD : 0, P_CHUNK = BESIDE ? 16 : 32;
+  static_assert(!BESIDE || P_BASE + 64 <= Shape<HD>::TM_COLS, "P fits behind O");
   constexpr int NK = SM::NK, NV = SM::NV, NSUB = SM::NSUB, BLK = SM::BLK, TEAMS = Shape<HD>::TEAMS, THREADS = Shape<HD>::THREADS, CREW = 128 * TEAMS;      // crew: the softmax threads
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -445,7 +450,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (TEAMS == 2 && len > 1) ok = ok && scores(1);
         for (int j = 0; j < len && ok; ++j) {
           const int t = j % TEAMS, i = n + j, s = i % NV;
-          ok = bar_wait(p_full(t), uses[t] & 1) && bar_wait(vfull(s), (i / NV) & 1);
+          ok = bar_wait(p_full(t), uses[t] & 1);
+          if (BESIDE && j + 1 < len) ok = ok && scores(j + 1);
+          ok = ok && bar_wait(vfull(s), (i / NV) & 1);
           if (!ok) break;
           ++uses[t];
           tc_fence_after();
@@ -455,11 +462,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           for (int k = 0; k < KBLK / 16; ++k)
 #pragma unroll
             for (int part = 0; part < PS; ++part)
-              mma_ts(o_col, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8, sdesc(vaddr + (uint32_t)k * 2u * LY::GROUP, LY::HALF, LY::GROUP), ID_O,
+              mma_ts(o_col, tmem + t * 128 + P_BASE + (k >> 1) * P_CHUNK + part * 16 + (k & 1) * 8, sdesc(vaddr + (uint32_t)k * 2u * LY::GROUP, LY::HALF, LY::GROUP), ID_O,
                      (j >= TEAMS || k > 0 || part > 0) ? 1u : 0u);
           umma_commit(vempty(s));
           umma_commit(o_done(t));
-          if (j + TEAMS < len) ok = scores(j + TEAMS);
+          if (!BESIDE && j + TEAMS < len) ok = scores(j + TEAMS);
         }
         n += len;
       }
@@ -468,7 +475,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   } else if (warp < 2 + 4 * TEAMS) {      // (one more warp has no part: it makes the V warp another scheduler's)
     // ---------------- softmax teams ----------------
     const int team = (warp - 2) >> 2, quarter = warp & 3, a = quarter * 32 + lane, tid = threadIdx.x - 64;
-    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), s_col = lane_base + team * 128, o_col = lane_base + Shape<HD>::O_COL + team * HD;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), s_col = lane_base + team * 128, p_col = s_col + P_BASE, o_col = lane_base + Shape<HD>::O_COL + team * HD;
     // scores in base 2; the sign of `scale` goes into the query; never 0, which would make NaN of a hidden key's -inf
     const float sc = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-37f);
     const bool negate = scale < 0.0f;
@@ -632,6 +639,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           m = next;
         }
         const float m_use = m == -INFINITY ? 0.0f : m;
+        if (BESIDE && j > 0) {      // the last block's P V has read P
+          wait(o_done(team), (uses - 1) & 1);
+          tc_fence_after();
+        }
 #pragma unroll 1
         for (int c = chunks - 1;; ) {
           uint64_t l2[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
@@ -646,23 +657,23 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             pk[e >> 1] = pack_bf16(p0, p1);
             if (PS == 2) pk[16 + (e >> 1)] = pack_bf16(p0 - u2f(pk[e >> 1] << 16), p1 - u2f(pk[e >> 1] & 0xffff0000u));
           }
-          if (PS == 2) tm_st32(s_col + col0 + c * 32, pk);
-          else tm_st16(s_col + col0 + c * 32, pk);
+          if (PS == 2) tm_st32(p_col + (copy * chunks + c) * P_CHUNK, pk);
+          else tm_st16(p_col + (copy * chunks + c) * P_CHUNK, pk);
           float la, lb;
           of_two(add_two(l2[0], l2[1]), la, lb);
           l += la + lb;
           if (--c < 0) break;
           load(c);
         }
-        if (copies > 1) {      // zeros for the other copies' keys
+        if (copies > 1 && (!BESIDE || j == 0)) {      // zeros for the other copies' keys; beside S they stay
           uint32_t zero[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) zero[e] = 0u;
 #pragma unroll 1
-          for (int c = 0; c < 128; c += 32)
-            if (c < col0 || c >= col0 + chunks * 32) {
-              if (PS == 2) tm_st32(s_col + c, zero);
-              else tm_st16(s_col + c, zero);
+          for (int c = 0; c < 4; ++c)
+            if (c / chunks != copy) {
+              if (PS == 2) tm_st32(p_col + c * P_CHUNK, zero);
+              else tm_st16(p_col + c * P_CHUNK, zero);
             }
         }
       };
