@@ -351,7 +351,7 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, int64_t q_row_stride, const 
 /* Vocabulary probabilities: out[r, :] = softmax(logits[r, :] / temperature[r]) in f32 (in_dtype 0 f32, 1 bf16; temperature
  * null: 1).  Temperature <= 0 gives the greedy row: 1 at the lowest column of the maximum, 0 elsewhere.  A token with logit
  * -inf has probability 0, a row of only those is all zeros; a row with a NaN, or whose maximum is +inf at a positive
- * temperature, holds NaN.  ld / ld_out >= cols; out may be the f32 logits themselves. */
+ * temperature, holds NaN.  ld / ld_out >= cols, cols <= 2^30; out may be the f32 logits themselves. */
 int wkb_token_probs(const void* logits, int in_dtype, int64_t ld, const float* temperature_or_null, float* out, int64_t ld_out,
                     int64_t rows, int64_t cols, void* stream);
 /* Verification of drafted tokens from given random numbers.  Row r of `probs` holds the target's probabilities after node r,

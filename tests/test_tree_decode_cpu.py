@@ -72,7 +72,7 @@ def test_nothing_to_do_is_fine(L):
     assert L.wkb_paged_kv_commit(P, P, 1, 0, 1, P, P, P, P, P, 1, 0, 1, 64, 16, 1, None, None) == 0
 
 
-@pytest.mark.parametrize("dtype,ld,ld_out,rows,cols", [(2, 10, 10, 1, 10), (0, 9, 10, 1, 10), (0, 10, 9, 1, 10), (0, 1 << 40, 1 << 40, 1, 1 << 35), (0, 10, 10, 1 << 40, 10)])
+@pytest.mark.parametrize("dtype,ld,ld_out,rows,cols", [(2, 10, 10, 1, 10), (0, 9, 10, 1, 10), (0, 10, 9, 1, 10), (0, 1 << 40, 1 << 40, 1, 1 << 35), (0, 1 << 31, 1 << 31, 1, (1 << 30) + 1), (0, 10, 10, 1 << 40, 10)])
 def test_probs_refusals(L, dtype, ld, ld_out, rows, cols):
     assert L.wkb_token_probs(P, dtype, ld, None, P, ld_out, rows, cols, None) == BAD
 

@@ -602,7 +602,7 @@ extern "C" {
 
 int wkb_token_probs(const void* logits, int in_dtype, i64 ld, const float* temperature_or_null, float* out, i64 ld_out, i64 rows, i64 cols, void* stream) {
   if (rows <= 0 || cols <= 0) return 0;
-  if ((in_dtype != 0 && in_dtype != 1) || ld < cols || ld_out < cols || cols > 0x7fffff00 || rows > 0x7fffffff / 8) return (int)cudaErrorInvalidValue;
+  if ((in_dtype != 0 && in_dtype != 1) || ld < cols || ld_out < cols || cols > (1 << 30) || rows > 0x7fffffff / 8) return (int)cudaErrorInvalidValue;
   const verify::ProbsShape s = verify::probs_shape(rows, cols);
   if (in_dtype == 0) return verify::launch_probs<float>(s, static_cast<const float*>(logits), ld, temperature_or_null, out, ld_out, rows, cols, as_stream(stream));
   return verify::launch_probs<__nv_bfloat16>(s, static_cast<const __nv_bfloat16*>(logits), ld, temperature_or_null, out, ld_out, rows, cols, as_stream(stream));
