@@ -376,6 +376,23 @@ def test_token_probs_match_f64(dev, rows, cols, dtype):
         assert bool(((y.double() - plain).abs() <= plain * 2.0 ** -15 + 1e-38).all())
 
 
+@pytest.mark.parametrize("rows,cols", [(300, 8192), (300, 16320), (300, 16384), (160, 32768), (3, 65536), (150, 65281), (150, 131072), (2, 262113)])
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_token_probs_full_runs(dev, rows, cols, shift, dtype):
+    """Rows that fill every register of their threads, starting on a word of two bf16 and in the middle of one: the last
+    column counts (it holds a large part of the row), and the columns beside the row do not (they are NaN).  Tolerance as above."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(rows + cols + shift)
+    wide = torch.full((rows, cols + 2 + shift), math.nan, device="cuda", dtype={"f32": torch.float32, "bf16": torch.bfloat16}[dtype])
+    x = wide[:, shift:shift + cols]
+    x.copy_(torch.randn((rows, cols), generator=g, device="cuda") * 3)
+    x[:, 0] = x[:, -1] = 13.0
+    got = dev.token_probs(x, None)
+    want = torch.softmax(x.double(), 1)
+    assert bool(((got.double() - want).abs() <= want * 2.0 ** -15 + 1e-38).all())
+
+
 def test_token_probs_special_rows(dev):
     import torch
     inf, nan = math.inf, math.nan

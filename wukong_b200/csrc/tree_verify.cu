@@ -90,14 +90,14 @@ constexpr int PT = 512;      // threads of a CTA
 // columns of a CTA when `ctas` share a row: whole 128-byte lines of f32
 __host__ __device__ __forceinline__ int probs_run(i64 cols, int ctas) { return (int)((cols + ctas - 1) / ctas + 31) / 32 * 32; }
 
-// A row is a cluster's: each CTA keeps up to E * 512 columns in registers, so the logits are read once and the probabilities
+// A row is a cluster's: each CTA keeps up to E * PT columns in registers, so the logits are read once and the probabilities
 // written once (HBM is the bound).  Every warp reduces its columns to (maximum, sum relative to it) and puts the pair into
 // every CTA's table; one cluster barrier later each warp adds up the whole table, so that nothing else is waited for
 // between the last load and the first store (with block-wide reductions and a second barrier 1024 x 32000 took 65 us,
-// now 48, 0.84 of the copy rate).  Loads and stores are 4 bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no more
+// now 46, 0.86 of the copy rate).  Loads and stores are 4 bytes a thread, coalesced, because the rows of an odd vocabulary are aligned to no more
 // than that, and where they are, 16 bytes a thread took longer (54 against 49 us).
-template <typename T, int E>
-__global__ void __launch_bounds__(PT, E > 32 ? 1 : E > 8 ? 2 : 4) token_probs_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature,
+template <typename T, int E, int PT>
+__global__ void __launch_bounds__(PT, (E > 32 ? 1 : E > 8 ? 2 : 4) * (512 / PT)) token_probs_kernel(const T* __restrict__ x, i64 ld, const float* __restrict__ temperature,
                                                                                                   float* __restrict__ out, i64 ld_out, int cols) {
   pdl_wait();
   pdl_trigger();
@@ -566,23 +566,39 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsig
 }
 
 // A row's columns over the CTAs of a cluster and the registers of their threads: clusters grow until two CTAs per SM are
-// at work (small batches) and a thread holds at most 32 columns (large vocabularies), or at 8.
-constexpr i64 PROBS_MAX = 8 * (64 * (i64)PT - 32);      // (a run of bf16 may begin with half a pair)
+// at work (small batches) and a thread holds at most 32 columns (large vocabularies), or at 8.  CTAs of 256 threads,
+// which leave an SM more of them to overlap, while eight hold a row: 1024 x 7582 f32 in 14.8 us, of 512 threads 17.9;
+// 128 x 32000 in 9.1 and 10.9.  Only full batches of bf16 rows that two CTAs of 512 threads hold and 256 do not keep those:
+// 1024 x 32000 in 53.9 us, of 256 threads 58.2; 640 x 50257 in 69 and 73.
+constexpr i64 PROBS_MAX = 8 * (64 * 512 - 32);      // (a run of bf16 may begin with half a pair)
 struct ProbsShape {
-  int ctas, regs;
+  int ctas, regs, threads;
 };
-static ProbsShape probs_shape(i64 rows, i64 cols) {
-  ProbsShape s{1, 4};
-  while (s.ctas < 8 && (cols > (i64)s.ctas * 32 * PT || (rows * s.ctas < 2 * WKB_SM_COUNT && cols > (i64)s.ctas * 4 * PT))) s.ctas *= 2;
-  while (s.regs < 64 && s.regs * PT < probs_run(cols, s.ctas) + 1) s.regs *= 2;
+template <typename T>
+static ProbsShape probs_shape(const T* x, i64 ld, i64 rows, i64 cols) {
+  constexpr bool PAIRS = sizeof(T) == 2;
+  // the column in front of a run: only where a row may begin with half a word (1024 x 32768 bf16: 53.5 us without it, 85 with it)
+  const int half = PAIRS && (((reinterpret_cast<uintptr_t>(x) >> 1) | (uintptr_t)ld) & 1);
+  const bool small = cols <= 2 * 32 * 256 - 32 * half || (cols <= 8 * (32 * 256 - 32 * half) && (!PAIRS || rows <= WKB_SM_COUNT));
+  ProbsShape s{1, 4, small ? 256 : 512};
+  auto need = [&] { return probs_run(cols, s.ctas) + half; };
+  while (s.ctas < 8 && (need() > 32 * s.threads || (rows * s.ctas < 2 * WKB_SM_COUNT && cols > (i64)s.ctas * 4 * s.threads))) s.ctas *= 2;
+  while (s.regs < 64 && s.regs * s.threads < need()) s.regs *= 2;
   return s;
 }
-template <typename T>
+template <typename T, int PT>
 static int launch_probs(const ProbsShape& s, const T* x, i64 ld, const float* temperature, float* out, i64 ld_out, i64 rows, i64 cols, cudaStream_t st) {
-  if (cols > PROBS_MAX) return (int)launch_pdl(token_probs_wide_kernel<T>, (unsigned)rows, 512, 0, st, x, ld, temperature, out, ld_out, (int)cols);
-  auto kern = s.regs == 4 ? token_probs_kernel<T, 4> : s.regs == 8 ? token_probs_kernel<T, 8> : s.regs == 16 ? token_probs_kernel<T, 16>
-            : s.regs == 32 ? token_probs_kernel<T, 32> : token_probs_kernel<T, 64>;
+  auto kern = s.regs == 4 ? token_probs_kernel<T, 4, PT> : s.regs == 8 ? token_probs_kernel<T, 8, PT> : s.regs == 16 ? token_probs_kernel<T, 16, PT> : token_probs_kernel<T, 32, PT>;
+  if constexpr (PT == 512) {
+    if (s.regs == 64) kern = token_probs_kernel<T, 64, PT>;
+  }
   return (int)launch_cluster(kern, (unsigned)(rows * s.ctas), PT, 0, s.ctas, st, x, ld, temperature, out, ld_out, (int)cols);
+}
+template <typename T>
+static int launch_probs(const T* x, i64 ld, const float* temperature, float* out, i64 ld_out, i64 rows, i64 cols, cudaStream_t st) {
+  if (cols > PROBS_MAX) return (int)launch_pdl(token_probs_wide_kernel<T>, (unsigned)rows, 512, 0, st, x, ld, temperature, out, ld_out, (int)cols);
+  const ProbsShape s = probs_shape(x, ld, rows, cols);
+  return s.threads == 256 ? launch_probs<T, 256>(s, x, ld, temperature, out, ld_out, rows, cols, st) : launch_probs<T, 512>(s, x, ld, temperature, out, ld_out, rows, cols, st);
 }
 // CTAs of a tree's cluster: as many as keep two per SM at work, each with 2048 columns at least.
 static int verify_ctas(i64 n_trees, i64 cols) {
@@ -603,9 +619,8 @@ extern "C" {
 int wkb_token_probs(const void* logits, int in_dtype, i64 ld, const float* temperature_or_null, float* out, i64 ld_out, i64 rows, i64 cols, void* stream) {
   if (rows <= 0 || cols <= 0) return 0;
   if ((in_dtype != 0 && in_dtype != 1) || ld < cols || ld_out < cols || cols > (1 << 30) || rows > 0x7fffffff / 8) return (int)cudaErrorInvalidValue;
-  const verify::ProbsShape s = verify::probs_shape(rows, cols);
-  if (in_dtype == 0) return verify::launch_probs<float>(s, static_cast<const float*>(logits), ld, temperature_or_null, out, ld_out, rows, cols, as_stream(stream));
-  return verify::launch_probs<__nv_bfloat16>(s, static_cast<const __nv_bfloat16*>(logits), ld, temperature_or_null, out, ld_out, rows, cols, as_stream(stream));
+  if (in_dtype == 0) return verify::launch_probs(static_cast<const float*>(logits), ld, temperature_or_null, out, ld_out, rows, cols, as_stream(stream));
+  return verify::launch_probs(static_cast<const __nv_bfloat16*>(logits), ld, temperature_or_null, out, ld_out, rows, cols, as_stream(stream));
 }
 
 int wkb_tree_verify(const float* probs, i64 ld_p, const float* draft_or_null, i64 ld_q, const int* token, const int* parent, const int* tree_row0,
