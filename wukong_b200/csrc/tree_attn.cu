@@ -135,6 +135,7 @@ extern "C" {
 
 i64 wkb_paged_attn_tree_scratch_bytes(i64 max_nodes, i64 q_heads, i64 kv_heads, i64 head_dim) {
   if (max_nodes <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0) return 0;
+  if (max_nodes > 0x7fffffff || q_heads > 0x7fffffff || head_dim > 0x7fffffff) return 0;
   return tree::scratch_bytes(max_nodes, q_heads / kv_heads, head_dim, tree::shares_of(head_dim));
 }
 
@@ -143,12 +144,16 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void
                         int out_dtype, i64 out_row_stride, i64 rows, i64 n_trees, i64 max_nodes, i64 q_heads, i64 kv_heads, i64 head_dim,
                         i64 page_tokens, i64 max_blocks_per_seq, float scale, void* scratch, i64 scratch_bytes, void* stream) {
   if (rows <= 0 || n_trees <= 0) return 0;
+  // every extent first, so that no product below wraps around (and no row's address in the kernels)
+  if (rows > 0x7fffffff || q_heads > 0x7fffffff || max_blocks_per_seq > 0x7fffffff || mask_words > 0x7fffffff || q_row_stride > (i64)1 << 31 ||
+      out_row_stride > (i64)1 << 31)
+    return (int)cudaErrorInvalidValue;
   if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0) return (int)cudaErrorInvalidValue;
   const i64 group = q_heads / kv_heads;
   if ((group != 1 && group != 2 && group != 4 && group != 8) || (head_dim != 64 && head_dim != 128)) return (int)cudaErrorInvalidValue;
   if (page_tokens < 4 || page_tokens > 65536 || (page_tokens & (page_tokens - 1)) != 0) return (int)cudaErrorInvalidValue;   // power of two, >= 4
   if (max_nodes < 1 || max_nodes > tree::MAX_NODES || n_trees > tree::MAX_TREES || mask_words * 32 < max_nodes) return (int)cudaErrorInvalidValue;
-  if (max_blocks_per_seq < 1 || max_blocks_per_seq * page_tokens > 0x7fffff00 || num_pages < 1 || rows > 0x7fffffff || rows * q_heads > 0x7fffffffff)
+  if (max_blocks_per_seq < 1 || max_blocks_per_seq * page_tokens > 0x7fffff00 || num_pages < 1 || rows * q_heads > 0x7fffffffff)
     return (int)cudaErrorInvalidValue;
   if (num_pages > 0x7fffff00 / (kv_heads * page_tokens)) return (int)cudaErrorInvalidValue;
   if ((q_dtype != 0 && q_dtype != 1) || (out_dtype != 0 && out_dtype != 1)) return (int)cudaErrorInvalidValue;

@@ -649,6 +649,8 @@ int wkb_paged_kv_commit(void* kcache, void* vcache, i64 layers, i64 layer_stride
                         const int* tree_ctx, const int* path, const int* n_path, i64 max_path, i64 n_trees, i64 kv_heads, i64 head_dim,
                         i64 page_tokens, i64 max_blocks_per_seq, int* new_ctx_or_null, void* stream) {
   if (n_trees <= 0 || layers <= 0) return 0;
+  // every extent first, so that no product below wraps around
+  if (layers > 0x7fffffff || kv_heads > 0x7fffffff || head_dim > 0x7fffffff || page_tokens > 0x7fffffff || max_blocks_per_seq > 0x7fffffff) return (int)cudaErrorInvalidValue;
   if (n_trees > 65535 || max_path < 1 || kv_heads < 1 || head_dim < 8 || head_dim % 8 != 0 || page_tokens < 1 || max_blocks_per_seq < 1 || num_pages < 1 ||
       max_blocks_per_seq * page_tokens > 0x7fffff00 || max_path > 0x7fffffff ||
       (double)num_pages * (double)kv_heads * (double)page_tokens * (double)(head_dim / 8) > 4294967040.0)      // 64 GB a layer and cache
@@ -656,8 +658,8 @@ int wkb_paged_kv_commit(void* kcache, void* vcache, i64 layers, i64 layer_stride
   if (new_ctx_or_null == tree_ctx) return (int)cudaErrorInvalidValue;      // read by every block of the tree
   if (layers > 1 && layer_stride < num_pages * kv_heads * page_tokens * head_dim) return (int)cudaErrorInvalidValue;
   if (((((uintptr_t)kcache) | ((uintptr_t)vcache)) & 15) != 0 || layer_stride % 8 != 0) return (int)cudaErrorMisalignedAddress;
-  const i64 threads = 2 * layers * kv_heads * (head_dim / 8), blocks = (threads + 255) / 256;
   if (layers > 0x3fffffff / 2 / (head_dim / 8) / kv_heads) return (int)cudaErrorInvalidValue;
+  const i64 threads = 2 * layers * kv_heads * (head_dim / 8), blocks = (threads + 255) / 256;
   const i64 wave = (WKB_SM_COUNT * 3 + n_trees - 1) / n_trees;      // blocks a tree that fill the SMs once
   int* status = gemm_status_word();
   if (!status) return (int)cudaErrorMemoryAllocation;
