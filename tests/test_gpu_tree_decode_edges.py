@@ -1,0 +1,68 @@
+"""GPU tests of the speculative-decoding operators where they are easily wrong: values that are not finite in long contexts,
+accuracy in the mean, refused calls."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_tree_decode import Case, dev, i32  # noqa: F401  (dev: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- V that is not finite -------------------------------------------------------------------------------------------
+
+def plant(c, cache, t, pos, head, dim, what):
+    cache[0, int(c.table[t, pos // c.page]), head, pos % c.page, dim] = what
+
+
+@pytest.mark.parametrize("types", ["f32-f32", "f32-bf16", "bf16-bf16", "bf16-f32"])
+@pytest.mark.parametrize("hd,kvh,nodes", [(64, 2, 5), (64, 1, 30), (128, 2, 9), (128, 1, 16)])
+def test_not_finite_values_in_long_contexts(dev, hd, kvh, nodes, types):
+    """Whatever the length: a column's NaN or infinities in the context reach every row, those of nodes the rows that see them."""
+    import torch
+    tq, to = ({"f32": torch.float32, "bf16": torch.bfloat16}[t] for t in types.split("-"))
+    c = Case(dev, [(20011, nodes), (700, 3), (0, nodes), (4096, nodes)], 2 * kvh, kvh, hd, seed=nodes, q_dtype=tq)
+    for t, pos, dim, what in [(0, 0, 3, math.inf), (0, 9000, 3, math.inf), (0, 12345, 7, math.nan), (0, 17, 20, -math.inf), (0, 19999, 21, math.inf),
+                              (0, 20005, 22, -math.inf), (0, 20011 + 2, 23, math.inf), (0, 20011 + 3, 21, -math.inf), (1, 701, 5, math.nan),
+                              (2, nodes - 1, 9, math.inf), (3, 4095, 11, -math.inf), (3, 4096 + nodes - 1, 12, math.nan)]:
+        plant(c, c.kv.v, t, pos, kvh - 1, dim, what)
+    out = torch.zeros((c.rows, 2 * kvh * hd), dtype=to, device="cuda")
+    c.run(dev, out)
+    c.check(out)
+    assert dev.gemm_status() == 0
+
+
+@pytest.mark.parametrize("hd,ctx", [(64, 150000), (128, 150000)])
+def test_not_finite_values_in_long_pieces(dev, hd, ctx):
+    """One block of the kernel works on 150 000 keys in one piece, and its other warps' waits do not run out while the results
+    are mended.  All trees' tables repeat the same pages.  Expected: softmax over the pages' keys, each as often as it
+    occurs; the tolerance is that of the other attention tests."""
+    import torch
+    n, pool, page = 148 * (2 if hd == 64 else 1), 512, 16
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    kv = dev.PagedKV(1, pool, 1, hd, page)
+    kv.k.normal_(generator=g); kv.v.normal_(generator=g)
+    kv.v[0, 37, 0, 5, 3] = math.inf
+    kv.v[0, 400, 0, 0, 60] = math.nan
+    kv.v[0, 401, 0, 0, 61], kv.v[0, 401, 0, 1, 61] = -math.inf, math.inf
+    mbps = -(-(ctx + 1) // page)
+    table = torch.arange(mbps, dtype=torch.int32, device="cuda").remainder(pool).repeat(n, 1)
+    q = torch.randn((n, hd), generator=g, device="cuda")
+    out, scale = torch.zeros((n, hd), device="cuda"), 1.0 / math.sqrt(hd)
+    dev.paged_attn_tree(q, hd, kv, 0, table, i32(np.arange(n)), i32(np.full(n, ctx)), i32(np.arange(n + 1)), i32(np.ones((n, 1))), out, 1, mbps, 1, scale,
+                        dev.paged_attn_tree_scratch(1, 1, 1, hd))
+    assert dev.gemm_status() == 0
+    k, v = (x[0, :, 0].reshape(-1, hd).double() for x in (kv.k, kv.v))
+    at = torch.arange(pool * page, device="cuda")
+    count = ((ctx + 1 - at + pool * page - 1) // (pool * page)).double()
+    s = q.double() @ k.T * scale
+    p = torch.exp(s - s.amax(1, keepdim=True)) * count
+    p /= p.sum(1, keepdim=True)
+    fine = torch.isfinite(v)
+    want, mag = p @ torch.where(fine, v, 0.0), p @ torch.where(fine, v, 0.0).abs()
+    most = float((q.double().abs() @ k.abs().T).max()) * scale
+    tol = 2.0 ** -14 * most + 2.0 ** -15 + (ctx + 1) * 2.0 ** -22
+    ok = fine.all(0)
+    assert bool(((out.double() - want).abs() <= tol * mag)[:, ok].all())
+    assert bool((out[:, 3] == math.inf).all()) and bool(out[:, 60:62].isnan().all())

@@ -198,6 +198,20 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
 }
 // non-zero when one of a word's two bf16 has an exponent of all ones
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+// What 8 bf16 hold that is not finite, a nibble for each: 1 infinity, 2 minus infinity, 4 NaN.  Or-ing nibbles adds elements
+// up, in any order: the sum is what kind_sum gives (none, an infinity, or NaN for a NaN or both infinities).
+__device__ __forceinline__ uint32_t kinds_of(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t kinds = 0u;
+  if (!(not_finite2(w[0]) | not_finite2(w[1]) | not_finite2(w[2]) | not_finite2(w[3]))) return kinds;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+    if ((b & 0x7f80u) == 0x7f80u) kinds |= ((b & 0x7fu) ? 4u : (b >> 15) ? 2u : 1u) << (4 * e);
+  }
+  return kinds;
+}
+__device__ __forceinline__ float kind_sum(uint32_t kind) { return kind == 1u ? INFINITY : kind == 2u ? -INFINITY : NAN; }
 __device__ __forceinline__ uint32_t low_bits(i64 n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 // A tree's share of the work list.
@@ -278,7 +292,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   auto o_done = [&](int t) { return more + 8u * (4 + t); };
   const uint32_t q_full = more + 8u * 6, q_first = more + 8u * 7;      // the first piece's query is everybody's work
   static_assert(8 * (2 * NK + 2 * NV + 8) <= 256, "barriers fit the header");
-  volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + 256);      // 0 tensor memory, 1 failed, 2 V not finite, 3 and 4 the share's first tree and its start
+  volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + 256);      // 0 tensor memory, 1 failed, 3 and 4 the share's first tree and its start
+  // of the (up to three) blocks from that with the context's end on: which keys have a V that is not finite, a bit each
+  volatile uint32_t* bad_keys = reinterpret_cast<volatile uint32_t*>(smem_raw + 288);
   float2* ml_s = reinterpret_cast<float2*>(smem_raw + 512);
   float* stage = reinterpret_cast<float*>(smem_raw + (stage_base - raw));
 
@@ -292,7 +308,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     for (int s = 0; s < NV; ++s) { mbar_init(vfull(s), 1); mbar_init(vempty(s), 1); }
     for (int t = 0; t < 2; ++t) { mbar_init(s_full(t), 1); mbar_init(p_full(t), 4); mbar_init(o_done(t), 1); }
     mbar_init(q_full, 4); mbar_init(q_first, 4 * TEAMS);
-    flags[1] = 0; flags[2] = 0;
+    flags[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
@@ -488,6 +504,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
     };
     auto teams_sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(CREW) : "memory"); };      // every softmax thread passes every one of these
+    auto teams_any = [&](bool mine) {      // the same barrier, and whether any thread says so
+      uint32_t any;
+      asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(any) : "r"((uint32_t)mine), "n"(CREW) : "memory");
+      return any != 0u;
+    };
     // The query operand (K-major, 128-byte swizzle).  The raw rows of the next piece come to the stage while this piece's
     // blocks are worked on (q_fetch), and the team that is not at work on the last block turns them into the operand's parts
     // and copies (q_put) as soon as that block's scores have been multiplied.  A thread reads back what it fetched itself.
@@ -589,6 +610,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       float m = -INFINITY, l = 0.0f;      // m in base 2, the maximum in use
       // One block, 32 columns at a time in rolled loops: the kernel is short enough that first executions of unrolled code
       // (instruction fetches) took longer than the work.  The last columns of the first pass stay in registers.
+      bool mend = false;      // results of this piece need mending: V holds something that is not finite
       const int chunks = 4 / copies, col0 = copy * chunks * 32;
       auto block = [&](auto masked_c, int j) {
         constexpr bool masked = decltype(masked_c)::value;      // some row does not see some key
@@ -709,9 +731,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               w &= ((b & 0x8000u) ? 0u : 0xffffu) | ((b & 0x80000000u) ? 0u : 0xffff0000u);
               asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
             }
-            if ((p.b0 + j) * KBLK + row < p.w.keys) flags[2] = 1;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
+          const uint32_t which = __ballot_sync(0xffffffffu, bad != 0u && (p.b0 + j) * KBLK + row < p.w.keys);
+          if (lane == 0) bad_keys[(p.b0 + j - p.w.t.ctx / KBLK) * 4 + quarter] = which;
+          mend |= which != 0u;
         }
         tm_st_wait();
         tc_fence_before();
@@ -744,34 +768,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const float2 v = ml_s[i];
         l_all += v.y * ex2(v.x - m_use);
       }
-      const bool whole = len == p.w.blocks, fine = flags[1] == 0, bad_v = flags[2] != 0;
+      const bool whole = len == p.w.blocks, fine = flags[1] == 0;
       const float inv = !whole ? 1.0f : l_all != 0.0f ? 1.0f / l_all : 0.0f;      // a unit in one piece is normalised here
       const float w0 = ex2(ml_s[a].x - m_use) * inv, w1 = both ? ex2(ml_s[QROWS + a].x - m_use) * inv : 0.0f;
       // a share's piece that begins the share is its even one; a later one that it does not finish is its odd one
       const int piece = p.unit_start + p.b0 == (int)blockIdx.x * share ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
       if (!whole && fine && team == 0 && copy == 0 && r < live) scr.ml[(i64)piece * scr.rows + r] = make_float2(m_all, l_all);
-      // rare: V holds a NaN or an infinity that this row may see.  Its sum over those elements is then the result
-      // (a row with a NaN score stays NaN)
-      auto bad_columns = [&](int row, int col, float4& v) {
-        const uint32_t* mrow = mask_of(row);
-#pragma unroll 1
-        for (int i = row; i < (both ? 2 : 1) * QROWS; i += crows)
-          if (ml_s[i].y != ml_s[i].y) return;
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-        for (int pos = p.b0 * KBLK; pos < min(p.b1 * KBLK, p.w.keys); ++pos) {
-          if (!(visible(mrow, pos) & 1u)) continue;
-          const uint32_t page = block_table[(i64)p.w.t.slot * g.mbps + (pos >> g.page_shift)];
-          if (page >= (uint64_t)g.num_pages) continue;
-          const u16* vp = vcache + (((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) * HD + col;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if ((vp[e] & 0x7f80u) == 0x7f80u) x[e] += bf16_bits_to_f32(vp[e]);
-        }
-        v.x = x[0] != 0.0f ? x[0] : v.x; v.y = x[1] != 0.0f ? x[1] : v.y;      // untouched where there was none
-        v.z = x[2] != 0.0f ? x[2] : v.z; v.w = x[3] != 0.0f ? x[3] : v.w;
-      };
-      const bool staged = copies > 1 || bad_v;
+      const bool staged = copies > 1;
       auto out_at = [&](int row) {      // of column 0
         const int ur = p.rowblk * QROWS + row;
         return whole ? (i64)(p.w.t.row0 + (ur >> gshift)) * g.out_row_stride + ((i64)p.head * group + (ur & (group - 1))) * HD
@@ -833,17 +836,62 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           float4 v = part(row);
           if (copies > 1) add(v, part(row + crows));
           if (copies > 2) { add(v, part(row + 2 * crows)); add(v, part(row + 3 * crows)); }
-          if (bad_v || !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) <= 3.402823466e+38f)) bad_columns(row, c0 + c4 * 4, v);
+          mend |= !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) <= 3.402823466e+38f);
           if (fine) put(at, v);
         }
         if (c0 + 64 < HD) teams_sync();
       }
-      if (bad_v) {
-        teams_sync();
-        if (tid == 0) flags[2] = 0;
-      }
       tc_fence_before();
-      teams_sync();      // the accumulators, the stage and ml_s are free
+      if (teams_any(mend)) {
+        // Rare: V holds a NaN or an infinity.  The sum of those elements over the keys that a row sees is then its result
+        // (a row with a NaN score stays NaN).  The whole blocks of the context are everybody's: their columns' kinds are
+        // gathered once, 16 keys at a time, and the keys of the other blocks are known: 2.5 ms for 150 000 keys in one
+        // piece (which the products take 1.7 to 3.6 ms for), so the other warps' waits of a second do not run out.
+        constexpr int CH8 = HD / 8;
+        uint32_t* kinds_s = reinterpret_cast<uint32_t*>(stage);      // [HD / 8]
+        if (tid < CH8) kinds_s[tid] = 0u;
+        teams_sync();
+        auto kinds_at = [&](int pos, int c) {
+          const uint32_t page = block_table[(i64)p.w.t.slot * g.mbps + (pos >> g.page_shift)];
+          if (page >= (uint64_t)g.num_pages) return 0u;
+          return kinds_of(*reinterpret_cast<const uint4*>(vcache + (((i64)page * g.kv_heads + p.head) * g.page_tokens + (pos & (g.page_tokens - 1))) * HD + c * 8));
+        };
+        const int shared_end = min(p.b1, p.w.t.ctx / KBLK) * KBLK;
+        uint32_t kinds = 0u;
+#pragma unroll 4
+        for (int pos = p.b0 * KBLK + tid / CH8; pos < shared_end; pos += CREW / CH8) kinds |= kinds_at(pos, tid % CH8);
+        if (kinds) atomicOr(&kinds_s[tid % CH8], kinds);
+        teams_sync();
+#pragma unroll 1
+        for (int it = tid; it < live * CH8; it += CREW) {
+          const int row = it / CH8, c = it % CH8;
+          bool nan = false;
+#pragma unroll 1
+          for (int i = row; i < (both ? 2 : 1) * QROWS; i += crows) nan |= ml_s[i].y != ml_s[i].y;
+          kinds = kinds_s[c];
+#pragma unroll 1
+          for (int w = 0; w < 12; ++w) {
+            const int blk = p.w.t.ctx / KBLK + (w >> 2);
+            if (blk < p.b0 || blk >= p.b1) continue;
+            const int pos = blk * KBLK + (w & 3) * 32;
+            uint32_t bits = bad_keys[w];
+            if (bits) bits &= visible(mask_of(row), pos);
+            for (; bits; bits &= bits - 1) kinds |= kinds_at(pos + __ffs(bits) - 1, c);
+          }
+          if (nan || !fine) continue;
+          const i64 at = out_at(row) + c * 8;
+#pragma unroll 1
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t kind = (kinds >> (4 * e)) & 7u;
+            if (!kind) continue;
+            if (!whole) scr.o[at + e] = kind_sum(kind);
+            else if (out_dtype == 0) static_cast<float*>(out)[at + e] = kind_sum(kind);
+            else static_cast<u16*>(out)[at + e] = f32_to_bf16_bits(kind_sum(kind));
+          }
+        }
+        teams_sync();
+      }
+      // the accumulators, the stage and ml_s are free
       if (TEAMS == 1 && more) q_put(following, tid, CREW, q_full);
     }
   }
