@@ -334,7 +334,8 @@ int wkb_paged_kv_append(const float* ksrc, const float* vsrc, int64_t src_row_st
  *
  * Attention: row r = node i of tree t sees every position below tree_ctx[t] and the node at tree_ctx[t] + j where bit j % 32
  * of tree_mask[r * mask_words + j / 32] is set (the node itself and its ancestors; other patterns are allowed).  What a row
- * does not see never reaches its output, NaN included; a row that sees nothing gives zeros.  q and out: dtype 0 f32, 1 bf16,
+ * does not see never reaches its output, NaN included; a row that sees nothing gives zeros.  Of V elements that are not finite a
+ * row's result is the sum over those that it sees, however small their weights; a K that is not finite may make the rows that see it NaN.  q and out: dtype 0 f32, 1 bf16,
  * row strides in elements, multiples of 8, at most 2^31; all bases 16-byte aligned; out overlaps no input.  bf16 outputs carry bf16 softmax weights; f32 outputs
  * keep f32 accuracy.  head_dim in {64, 128}; q_heads / kv_heads in {1, 2, 4, 8}; page_tokens a power of two >= 4;
  * n_trees <= 4096, and trees x kv_heads x 128-row blocks x (128-key blocks of a table row + 4) < 2^31.  A block-table entry

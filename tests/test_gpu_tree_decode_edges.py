@@ -66,3 +66,26 @@ def test_not_finite_values_in_long_pieces(dev, hd, ctx):
     ok = fine.all(0)
     assert bool(((out.double() - want).abs() <= tol * mag)[:, ok].all())
     assert bool((out[:, 3] == math.inf).all()) and bool(out[:, 60:62].isnan().all())
+
+
+@pytest.mark.parametrize("types", ["f32-f32", "f32-bf16", "bf16-bf16", "bf16-f32"])
+@pytest.mark.parametrize("gain", [1.0, 40.0])
+@pytest.mark.parametrize("hd,group,page,trees", [(64, 1, 16, [(300, 100), (40, 70)]), (128, 1, 16, [(300, 100), (40, 70)]), (64, 4, 16, [(9000, 140), (2000, 3)]),
+                                                 (128, 4, 16, [(9000, 140), (2000, 3)]), (128, 8, 16, [(30011, 40)]), (64, 2, 4, [(300, 20), (9, 9)])])
+def test_infinities_in_the_context_whatever_the_tree_and_the_weights(dev, hd, group, page, trees, gain, types):
+    """An infinity in a column gives that infinity in every row, for wide trees as for narrow ones, in a joined result as in one
+    piece, and where the key's weight is below what f32 holds (gain 40: exp(-300))."""
+    import torch
+    tq, to = ({"f32": torch.float32, "bf16": torch.bfloat16}[t] for t in types.split("-"))
+    c = Case(dev, trees, group, 1, hd, page, seed=hd + group, q_dtype=tq, q_gain=gain)
+    for t, (ctx, nodes) in enumerate(trees):
+        for dim, pos in enumerate([0, 3, 8, ctx // 3, ctx // 2, ctx - 1]):
+            plant(c, c.kv.v, t, pos, 0, dim, math.inf if dim % 2 else -math.inf)
+        plant(c, c.kv.v, t, 1, 0, 40, math.inf)
+        plant(c, c.kv.v, t, ctx - 2, 0, 40, -math.inf)
+        plant(c, c.kv.v, t, 2, 0, 41, math.nan)
+        plant(c, c.kv.v, t, ctx, 0, 42, math.inf)
+    out = torch.zeros((c.rows, group * hd), dtype=to, device="cuda")
+    c.run(dev, out)
+    c.check(out)
+    assert dev.gemm_status() == 0

@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(256) tree_attn_rows_kernel(const void* __restr
       l = l * corr + warp_sum(pr);
       m = m_new;
 #pragma unroll
-      for (int e = 0; e < HD / 32; ++e) acc[e] *= corr;
+      for (int e = 0; e < HD / 32; ++e) acc[e] *= fabsf(acc[e]) <= 3.402823466e+38f ? corr : 1.0f;      // an infinity of V stays one where corr is 0 ...
       while (todo) {
         const int b = __ffs(todo) - 1;
         todo &= todo - 1;
@@ -111,7 +111,10 @@ __global__ void __launch_bounds__(256) tree_attn_rows_kernel(const void* __restr
         const i64 ob = __shfl_sync(0xffffffffu, off, b);
         if (ob < 0) continue;
 #pragma unroll
-        for (int e = 0; e < HD / 32; ++e) acc[e] = ffma(pb, bf16_bits_to_f32(vc[ob + e * 32 + lane]), acc[e]);
+        for (int e = 0; e < HD / 32; ++e) {
+          const float x = bf16_bits_to_f32(vc[ob + e * 32 + lane]);
+          acc[e] = ffma(fabsf(x) <= 3.402823466e+38f ? pb : 1.0f, x, acc[e]);      // ... or the weight
+        }
       }
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;      // a row that sees nothing: zeros

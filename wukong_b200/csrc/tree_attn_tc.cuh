@@ -27,8 +27,9 @@
 //
 // V and 0 x NaN: a probability of zero does not silence a NaN or an infinity in the product.  In the blocks with tree
 // nodes and behind the last key, where rows see different keys, V elements that are not finite are set to zero in shared
-// memory before the product.  Where the copies' zeros meet one in the committed context, which every row sees, the result
-// is not finite, as it has to be.  Either way the elements' own sum over the keys that a row sees is its result.
+// memory before the product.  In the committed context, which every row sees, one makes the result something that is not
+// finite, but not always the right thing: a weight below f32, a copy's zero or a negative lo part of P makes NaN of an
+// infinity.  Either way the elements' own sum over the keys that a row sees is put in the result's place.
 #pragma once
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -803,6 +804,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = f2u(u2f(o[e]) * w0);
           }
+          uint64_t zero = two(0.0f, 0.0f);      // stays 0 unless an element is not finite
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) zero = fma_two(two(u2f(o[e]), u2f(o[e + 1])), two(0.0f, 0.0f), zero);
+          float zero_a, zero_b;
+          of_two(zero, zero_a, zero_b);
+          mend |= !(zero_a + zero_b == 0.0f);
           if (staged) {
             float4* d = reinterpret_cast<float4*>(stage + a * 64 + half * 32);
 #pragma unroll
@@ -836,7 +843,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           float4 v = part(row);
           if (copies > 1) add(v, part(row + crows));
           if (copies > 2) { add(v, part(row + 2 * crows)); add(v, part(row + 3 * crows)); }
-          mend |= !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) <= 3.402823466e+38f);
           if (fine) put(at, v);
         }
         if (c0 + 64 < HD) teams_sync();
@@ -942,7 +948,9 @@ __global__ void __launch_bounds__(256) tree_attn_join_kernel(void* __restrict__ 
     for (int k = 0; k < n; ++k) {
       const float wk = __shfl_sync(team, w, k, LANES);
       const float4 v = *reinterpret_cast<const float4*>(scr.o + piece(k0 + k) * HD + col);
-      o.x = ffma(v.x, wk, o.x); o.y = ffma(v.y, wk, o.y); o.z = ffma(v.z, wk, o.z); o.w = ffma(v.w, wk, o.w);
+      // what is not finite counts as it is: its piece's weight may be 0 in f32, and 0 x inf is NaN
+      auto add = [&](float& to, float x) { to = ffma(x, fabsf(x) <= 3.402823466e+38f ? wk : 1.0f, to); };
+      add(o.x, v.x); add(o.y, v.y); add(o.z, v.z); add(o.w, v.w);
     }
   }
   for (int k = LANES / 2; k > 0; k >>= 1) l += __shfl_xor_sync(team, l, k, LANES);
