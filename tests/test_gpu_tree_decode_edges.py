@@ -89,3 +89,26 @@ def test_infinities_in_the_context_whatever_the_tree_and_the_weights(dev, hd, gr
     c.run(dev, out)
     c.check(out)
     assert dev.gemm_status() == 0
+
+
+# ---- commit ---------------------------------------------------------------------------------------------------------
+
+def test_commit_of_a_broken_path_counts_what_was_moved(dev):
+    """Where a path breaks off, the next context ends with the last node that was moved: what lies behind it is not the
+    sequence's.  Breaks in the first eight nodes, in the second eight and at the first one; whole paths beside them."""
+    import torch
+    kv = dev.PagedKV(1, 12, 1, 64, 16)
+    up = list(range(12))
+    paths = [[0, 3, 3], [0, 2, 1], [0, 60, 61], [0, -4, 5], [0, 5, 2 ** 31 - 1], up[:9] + [9, 9, 10], up[:8] + [7, 9], up, [0], []]
+    good = [2, 2, 1, 1, 2, 10, 8, 12, 1, 0]
+    n = len(paths)
+    path = np.full((n, 12), -1)
+    for t, p in enumerate(paths):
+        path[t, :len(p)] = p
+    table = np.arange(12).reshape(1, 12).repeat(n, 0)[:, :3]      # (all broken or in place: the trees' moves do not meet)
+    ctx = np.arange(n)
+    for t in range(n):
+        new = torch.full((1,), -9, dtype=torch.int32, device="cuda")
+        dev.paged_kv_commit(kv, i32(table[t:t + 1]), i32([0]), i32(ctx[t:t + 1]), i32(path[t:t + 1]), i32([len(paths[t])]), 3, new_ctx=new)
+        assert dev.gemm_status() == (0 if good[t] == len(paths[t]) else 31), t
+        assert int(new) == ctx[t] + good[t], t

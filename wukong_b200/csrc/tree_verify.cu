@@ -502,7 +502,6 @@ __global__ void __launch_bounds__(256, 3) kv_commit_kernel(uint4* __restrict__ k
   const int t = blockIdx.y, slot = slots[t], ctx = ctxs[t], n = min(n_path[t], max_path);
   if (slot < 0 || ctx < 0) return;
   const int per = layers * kv_heads * chunks, at0 = (int)blockIdx.x * 256 + threadIdx.x;
-  if (at0 == 0 && new_ctx) new_ctx[t] = ctx + max(n, 0);
   const uint32_t page_stride = (uint32_t)kv_heads * (uint32_t)page_tokens * (uint32_t)chunks;      // a slab is no more than 2^32 units
   const uint32_t* bt = block_table + (i64)slot * mbps;
   const i64 cover = (i64)mbps * page_tokens;
@@ -538,11 +537,15 @@ __global__ void __launch_bounds__(256, 3) kv_commit_kernel(uint4* __restrict__ k
         if (k < good && from[k] != to[k]) cache[to[k]] = v[k];
     }
     if (good < min(BATCH, n - i0)) {      // not a path, or past the table or the cache: the moves end here
-      if (at0 == 0 && status) atomicExch(status, WKB_STATUS_KV_POS_RANGE);
+      if (at0 == 0) {
+        atomicExch(status, WKB_STATUS_KV_POS_RANGE);
+        if (new_ctx) new_ctx[t] = ctx + i0 + good;
+      }
       return;
     }
     before = node[BATCH - 1];
   }
+  if (at0 == 0 && new_ctx) new_ctx[t] = ctx + max(n, 0);
 }
 
 // A launch whose blocks form clusters of `ctas`, as a programmatic dependent like launch_pdl's.
