@@ -376,7 +376,7 @@ int wkb_tree_verify(const float* probs, int64_t ld_p, const float* draft_or_null
  * each), and new_ctx[t] (may be null, must not be tree_ctx) = tree_ctx[t] + n_path[t], the context of the next step.  A path must
  * ascend, and no two trees of a call may share a slot.  An entry that does not ascend, or whose positions lie past the
  * block-table row or the cache, ends that tree's moves and records 31 (wkb_gemm_status), and new_ctx[t] counts the entries
- * in front of it; trees that are switched off are left alone.  A layer's slab is at most 64 GB. */
+ * in front of it; a length above max_path counts as max_path and records 31 too; trees that are switched off are left alone.  A layer's slab is at most 64 GB. */
 int wkb_paged_kv_commit(void* kcache, void* vcache, int64_t layers, int64_t layer_stride, int64_t num_pages, const uint32_t* block_table,
                         const int* tree_slot, const int* tree_ctx, const int* path, const int* n_path, int64_t max_path, int64_t n_trees,
                         int64_t kv_heads, int64_t head_dim, int64_t page_tokens, int64_t max_blocks_per_seq, int* new_ctx_or_null,

@@ -112,3 +112,15 @@ def test_commit_of_a_broken_path_counts_what_was_moved(dev):
         dev.paged_kv_commit(kv, i32(table[t:t + 1]), i32([0]), i32(ctx[t:t + 1]), i32(path[t:t + 1]), i32([len(paths[t])]), 3, new_ctx=new)
         assert dev.gemm_status() == (0 if good[t] == len(paths[t]) else 31), t
         assert int(new) == ctx[t] + good[t], t
+
+
+def test_commit_reports_a_length_beyond_the_path(dev):
+    """n_path above max_path: the path's entries are moved and counted, and the length is reported."""
+    import torch
+    kv = dev.PagedKV(1, 3, 1, 64, 16)
+    new = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for n_path, status in [(3, 0), (4, 31), (2 ** 31 - 1, 31)]:
+        kv.k.copy_(torch.arange(48, device="cuda").view(1, 3, 1, 16, 1).expand_as(kv.k))
+        dev.paged_kv_commit(kv, i32([[0, 1, 2]]), i32([0]), i32([20]), i32([[0, 4, 9]]), i32([n_path]), 3, new_ctx=new)
+        assert dev.gemm_status() == status and int(new) == 23
+        assert kv.k.view(48, 64)[20:24, 0].tolist() == [20, 24, 29, 23]

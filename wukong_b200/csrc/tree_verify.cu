@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(256, 3) kv_commit_kernel(uint4* __restrict__ k
                                                         int* __restrict__ new_ctx, int* __restrict__ status) {
   pdl_wait();
   pdl_trigger();
-  const int t = blockIdx.y, slot = slots[t], ctx = ctxs[t], n = min(n_path[t], max_path);
+  const int t = blockIdx.y, slot = slots[t], ctx = ctxs[t], length = n_path[t], n = min(length, max_path);
   if (slot < 0 || ctx < 0) return;
   const int per = layers * kv_heads * chunks, at0 = (int)blockIdx.x * 256 + threadIdx.x;
   const uint32_t page_stride = (uint32_t)kv_heads * (uint32_t)page_tokens * (uint32_t)chunks;      // a slab is no more than 2^32 units
@@ -545,7 +545,10 @@ __global__ void __launch_bounds__(256, 3) kv_commit_kernel(uint4* __restrict__ k
     }
     before = node[BATCH - 1];
   }
-  if (at0 == 0 && new_ctx) new_ctx[t] = ctx + max(n, 0);
+  if (at0 == 0) {
+    if (new_ctx) new_ctx[t] = ctx + max(n, 0);
+    if (length > max_path) atomicExch(status, WKB_STATUS_KV_POS_RANGE);
+  }
 }
 
 // A launch whose blocks form clusters of `ctas`, as a programmatic dependent like launch_pdl's.
