@@ -373,7 +373,7 @@ int wkb_tree_verify(const float* probs, int64_t ld_p, const float* draft_or_null
                     const float* u_final, int* path, int* tokens, int* n_path, int64_t max_path, void* stream);
 /* Commit of a verified step: the K / V of node path[t, i], 1 <= i < n_path[t], move from position tree_ctx[t] + path[t, i] to
  * tree_ctx[t] + i, in all layers (slabs `layer_stride` elements apart, bf16 [num_pages][kv_heads][page_tokens][head_dim]
- * each), and new_ctx[t] (may be null, must not be tree_ctx) = tree_ctx[t] + n_path[t], the context of the next step.  A path must
+ * each), and new_ctx[t] (may be null, shares no memory with the other int arrays) = tree_ctx[t] + n_path[t], the context of the next step.  A path must
  * ascend, and no two trees of a call may share a slot.  An entry that does not ascend, or whose positions lie past the
  * block-table row or the cache, ends that tree's moves and records 31 (wkb_gemm_status), and new_ctx[t] counts the entries
  * in front of it; a length above max_path counts as max_path and records 31 too; trees that are switched off are left alone.  A layer's slab is at most 64 GB. */

@@ -661,7 +661,9 @@ int wkb_paged_kv_commit(void* kcache, void* vcache, i64 layers, i64 layer_stride
       max_blocks_per_seq * page_tokens > 0x7fffff00 || max_path > 0x7fffffff ||
       (double)num_pages * (double)kv_heads * (double)page_tokens * (double)(head_dim / 8) > 4294967040.0)      // 64 GB a layer and cache
     return (int)cudaErrorInvalidValue;
-  if (new_ctx_or_null == tree_ctx) return (int)cudaErrorInvalidValue;      // read by every block of the tree
+  auto meets_new_ctx = [&](const int* a, i64 n) { return new_ctx_or_null && new_ctx_or_null < a + n && a < new_ctx_or_null + n_trees; };
+  if (meets_new_ctx(tree_slot, n_trees) || meets_new_ctx(tree_ctx, n_trees) || meets_new_ctx(n_path, n_trees) || meets_new_ctx(path, n_trees * max_path))
+    return (int)cudaErrorInvalidValue;      // read by every block of a tree
   if (layers > 1 && layer_stride < num_pages * kv_heads * page_tokens * head_dim) return (int)cudaErrorInvalidValue;
   if (((((uintptr_t)kcache) | ((uintptr_t)vcache)) & 15) != 0 || layer_stride % 8 != 0) return (int)cudaErrorMisalignedAddress;
   if (layers > 0x3fffffff / 2 / (head_dim / 8) / kv_heads) return (int)cudaErrorInvalidValue;
