@@ -124,3 +124,27 @@ def test_commit_reports_a_length_beyond_the_path(dev):
         dev.paged_kv_commit(kv, i32([[0, 1, 2]]), i32([0]), i32([20]), i32([[0, 4, 9]]), i32([n_path]), 3, new_ctx=new)
         assert dev.gemm_status() == status and int(new) == 23
         assert kv.k.view(48, 64)[20:24, 0].tolist() == [20, 24, 29, 23]
+
+
+# ---- refused calls --------------------------------------------------------------------------------------------------
+
+def attention_args(dev, **over):
+    import torch
+    z = lambda *s, dt=torch.int32: torch.zeros(s, dtype=dt, device="cuda")
+    a = dict(q=z(3, 256, dt=torch.float32), q_row_stride=256, kv=dev.PagedKV(2, 4, 2, 64), layer=1, block_table=z(1, 4), tree_slot=z(1), tree_ctx=z(1), tree_row0=z(2),
+             tree_mask=z(3, 1), out=z(3, 256, dt=torch.float32), q_heads=4, mbps=4, max_nodes=3, scale=1.0, scratch=dev.paged_attn_tree_scratch(3, 4, 2, 64))
+    a.update(over)
+    return a
+
+
+def test_queries_whose_rows_are_not_dense_are_refused(dev):
+    import torch
+    f = lambda *s: torch.zeros(s, device="cuda")
+    for good in (f(3, 256), f(3, 4, 64), f(3 * 256), f(3, 600)[:, 40:], f(3, 1, 256)):
+        dev.paged_attn_tree(**attention_args(dev, q=good, q_row_stride=good.stride(0) if good.dim() > 1 else 256))
+    for bad in (f(256, 3).t(), f(4, 3, 64).transpose(0, 1), f(3, 64, 4).transpose(1, 2), f(2 * 3 * 256)[::2], f(3, 512)[:, ::2], f(1).expand(3, 256), f(1)[0]):
+        with pytest.raises(ValueError):
+            dev.paged_attn_tree(**attention_args(dev, q=bad))
+    for stride in (1 << 61, 1 << 62, (1 << 63) - 8, 257 * 8):
+        with pytest.raises(ValueError):
+            dev.paged_attn_tree(**attention_args(dev, q_row_stride=stride))

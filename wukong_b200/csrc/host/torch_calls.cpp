@@ -73,6 +73,18 @@ int64_t pitch(const at::Tensor& t, int64_t cols, const char* what) {
   if (t.dim() != 2 || t.size(1) < cols || t.stride(1) != 1) throw Refused(std::string(what) + " must be a matrix of at least " + std::to_string(cols) + " columns with unit column stride");
   return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1));
 }
+// rows of dense values, `stride` apart: [n], [rows, values] or [rows, heads, values], from which any number of values is used
+void dense_rows(const at::Tensor& t, int64_t rows, int64_t stride, int64_t width, const char* what) {
+  int64_t dense = 1;
+  for (int64_t d = t.dim() - 1; d >= (t.dim() > 1 ? 1 : 0); --d) {
+    if (t.size(d) != 1 && t.stride(d) != dense) throw Refused(std::string(what) + " must hold the values of a row one behind the other");
+    dense *= t.size(d);
+  }
+  constexpr int64_t MOST = (int64_t)1 << 31;      // (no product wraps around)
+  if (rows > 0 && (t.dim() == 0 || rows > MOST || width > MOST || stride < 0 || stride > MOST ||
+                   (t.storage_offset() + (rows - 1) * stride + width) * (int64_t)t.element_size() > (int64_t)t.storage().nbytes()))
+    throw Refused(std::string(what) + " does not hold " + std::to_string(rows) + " rows of pitch " + std::to_string(stride));
+}
 int float_code(const at::Tensor& t, const char* what) {
   if (t.scalar_type() == at::kFloat) return 0;
   if (t.scalar_type() == at::kBFloat16) return 1;
@@ -133,13 +145,14 @@ PyObject* paged_attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor &q = c.tensor(0, "q"), &out = c.tensor(15, "out"), &mask = c.tensor(14, "tree_mask"), &scratch = c.tensor(20, "scratch");
     c.here(out);
     const Cache kv = cache_of(c, 2);
-    const int64_t stride = c.integer(1), layer = c.integer(9), q_heads = c.integer(16), width = q_heads * kv.head_dim;
+    const int64_t stride = c.integer(1), layer = c.integer(9), q_heads = c.integer(16);
+    if (q_heads < 1 || q_heads > 1 << 20) throw Refused("q_heads must be positive");
+    const int64_t width = q_heads * kv.head_dim;
     const int64_t rows = out.dim() == 2 ? out.size(0) : 0, trees = c.tensor(11, "tree_slot").numel();
     const int q_code = float_code(q, "q"), out_code = float_code(out, "out");
     if (layer < 0 || layer >= kv.layers) throw Refused("no such layer");
     c.on_device(q, "q");
-    if (rows > 0 && (stride < 0 || (q.storage_offset() + (rows - 1) * stride + width) * (int64_t)q.element_size() > (int64_t)q.storage().nbytes()))
-      throw Refused("q does not hold " + std::to_string(rows) + " rows of pitch " + std::to_string(stride));
+    dense_rows(q, rows, stride, width, "q");
     if (mask.dim() != 2 || mask.size(0) < rows) throw Refused("tree_mask must have a row for each row of out");
     const int64_t ldo = pitch(out, width, "out"), mbps = table_width(c, 10, c.integer(17));
     const int64_t at_layer = layer * kv.layer_stride * 2;
