@@ -148,3 +148,15 @@ def test_queries_whose_rows_are_not_dense_are_refused(dev):
     for stride in (1 << 61, 1 << 62, (1 << 63) - 8, 257 * 8):
         with pytest.raises(ValueError):
             dev.paged_attn_tree(**attention_args(dev, q_row_stride=stride))
+
+
+def test_a_block_table_without_rows_is_refused(dev):
+    """No tree can have a row in it; the kernels would read behind it."""
+    import torch
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    for empty in (z(0, 4), z(0)):
+        with pytest.raises(ValueError):
+            dev.paged_attn_tree(**attention_args(dev, block_table=empty))
+        with pytest.raises(ValueError):
+            dev.paged_kv_commit(dev.PagedKV(1, 2, 1, 64), empty, z(1), z(1), z(1, 3), z(1), 4)
+        dev.paged_kv_commit(dev.PagedKV(1, 2, 1, 64), empty, z(0), z(0), z(0, 3), z(0), 4)      # nothing to do

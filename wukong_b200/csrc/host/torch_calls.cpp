@@ -90,10 +90,11 @@ int float_code(const at::Tensor& t, const char* what) {
   if (t.scalar_type() == at::kBFloat16) return 1;
   throw Refused(std::string(what) + " must be f32 or bf16");
 }
-int64_t table_width(const Call& c, int i, int64_t mbps) {
+int64_t table_width(const Call& c, int i, int64_t mbps, int64_t trees) {
   const at::Tensor& t = c.tensor(i, "block_table");
   c.on_device(t, "block_table");
   if (t.scalar_type() != at::kInt || mbps < 1 || t.numel() % mbps || !t.is_contiguous()) throw Refused("block_table must be a contiguous int32 [slots, mbps]");
+  if (trees > 0 && t.numel() == 0) throw Refused("block_table has no rows");
   return mbps;
 }
 struct Cache {
@@ -154,7 +155,7 @@ PyObject* paged_attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
     c.on_device(q, "q");
     dense_rows(q, rows, stride, width, "q");
     if (mask.dim() != 2 || mask.size(0) < rows) throw Refused("tree_mask must have a row for each row of out");
-    const int64_t ldo = pitch(out, width, "out"), mbps = table_width(c, 10, c.integer(17));
+    const int64_t ldo = pitch(out, width, "out"), mbps = table_width(c, 10, c.integer(17), trees);
     const int64_t at_layer = layer * kv.layer_stride * 2;
     check(wkb_paged_attn_tree(q.data_ptr(), q_code, stride, kv.k + at_layer, kv.v + at_layer, kv.pages, (const uint32_t*)c.tensor(10, "block_table").data_ptr(),
                               (const int*)c.values(11, trees, at::kInt, "tree_slot"), (const int*)c.values(12, trees, at::kInt, "tree_ctx"),
@@ -244,7 +245,7 @@ PyObject* paged_kv_commit(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t trees = slot.numel();
     const Cache kv = cache_of(c, 0);
     if (path.dim() != 2 || path.size(0) != trees) throw Refused("path must be int32 [n, max_path]");
-    const int64_t mbps = table_width(c, 7, c.integer(12));
+    const int64_t mbps = table_width(c, 7, c.integer(12), trees);
     check(wkb_paged_kv_commit(kv.k, kv.v, kv.layers, kv.layer_stride, kv.pages, (const uint32_t*)c.tensor(7, "block_table").data_ptr(),
                               (const int*)c.values(8, trees, at::kInt, "tree_slot"), (const int*)c.values(9, trees, at::kInt, "tree_ctx"),
                               (const int*)c.values(10, path.numel(), at::kInt, "path"), (const int*)c.values(11, trees, at::kInt, "n_path"), path.size(1), trees,
