@@ -160,3 +160,27 @@ def test_a_block_table_without_rows_is_refused(dev):
         with pytest.raises(ValueError):
             dev.paged_kv_commit(dev.PagedKV(1, 2, 1, 64), empty, z(1), z(1), z(1, 3), z(1), 4)
         dev.paged_kv_commit(dev.PagedKV(1, 2, 1, 64), empty, z(0), z(0), z(0, 3), z(0), 4)      # nothing to do
+
+
+# ---- vocabulary probabilities ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cols", [1, 2, 3, 4, 31, 32, 33, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 2047, 2049, 4095, 4097, 8191, 8193, 16351, 16383, 50257])
+@pytest.mark.parametrize("rows", [1, 3, 400])
+def test_token_probs_bf16_rows_that_begin_and_end_in_a_word(dev, rows, cols):
+    """Every parity of a row's first and last column: what lies in the other half of the words at its ends is not the row's
+    (NaN, and a buffer that ends with the last column).  Tolerance as for all probabilities (2^-15 of the value)."""
+    import torch
+    rows = min(rows, (1 << 23) // cols)
+    g = torch.Generator(device="cuda").manual_seed(rows + cols)
+    for first in (0, 1):
+        for pitch in (cols, cols + 1):
+            flat = torch.full((first + (rows - 1) * pitch + cols,), math.nan, dtype=torch.bfloat16, device="cuda")
+            x = flat[first:].as_strided((rows, cols), (pitch, 1), first)
+            x.copy_(torch.randn((rows, cols), generator=g, device="cuda") * 3)
+            for t in (None, torch.zeros(rows, device="cuda")):
+                got = dev.token_probs(x, t)
+                if t is None:
+                    want = torch.softmax(x.double(), 1)
+                    assert bool(((got.double() - want).abs() <= want * 2.0 ** -15 + 1e-38).all())
+                else:
+                    assert torch.equal(got.argmax(1), (x == x.amax(1, keepdim=True)).double().argmax(1)) and bool((got.sum(1) == 1).all())

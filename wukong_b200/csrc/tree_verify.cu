@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(PT, (E > 32 ? 1 : E > 8 ? 2 : 4) * (512 / PT))
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const i64 row = blockIdx.x / size;
   // The CTAs' columns: equal runs of the row.  Of f32 a thread takes every PT-th one, of bf16 every PT-th pair in an aligned
-  // word, whose first pair may begin and whose last may end a column outside the run.
+  // word; where a run begins or ends in the middle of a word, its column is read by itself.
   constexpr int PAIR = sizeof(T) == 2 ? 2 : 1;
   const int run = probs_run(cols, (int)size), start = (int)rank * run, end = min(cols, start + run);
   const T* xr = x + row * ld + start;
@@ -122,9 +122,19 @@ __global__ void __launch_bounds__(PT, (E > 32 ? 1 : E > 8 ? 2 : 4) * (512 / PT))
   for (int e = 0; e < E; e += PAIR) {
     if (PAIR == 1) v[e] = own(e) ? logit(xr, at(e)) : -INFINITY;
     else {
-      const uint32_t w = at(e) < mine ? *reinterpret_cast<const uint32_t*>(xr + at(e)) : 0u;
-      v[e] = own(e) ? u2f(w << 16) : -INFINITY;
-      v[e + PAIR - 1] = at(e + PAIR - 1) < mine ? u2f(w & 0xffff0000u) : -INFINITY;
+      const bool both = own(e) && at(e + PAIR - 1) < mine;
+      const uint32_t w = both ? *reinterpret_cast<const uint32_t*>(xr + at(e)) : 0xff80ff80u;
+      v[e] = u2f(w << 16);
+      v[e + PAIR - 1] = u2f(w & 0xffff0000u);
+    }
+  }
+  if (PAIR == 2) {
+    if (first < start && PAIR - 1 < mine) v[PAIR - 1] = logit(xr, PAIR - 1);
+    if (mine > 0 && (mine - 1) % (PAIR * PT) == 0 && first + mine - 1 >= start) {      // this thread's last column is a word's first half
+      const float last = logit(xr, mine - 1);
+#pragma unroll
+      for (int e = 0; e < E; e += PAIR)
+        if (at(e) == mine - 1) v[e] = last;
     }
   }
   const float temp = temperature ? temperature[row] : 1.0f;
@@ -575,7 +585,7 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsig
 // at work (small batches) and a thread holds at most 32 columns (large vocabularies), or at 8.  CTAs of 256 threads,
 // which leave an SM more of them to overlap, while eight hold a row: 1024 x 7582 f32 in 14.8 us, of 512 threads 17.9;
 // 128 x 32000 in 9.1 and 10.9.  Only full batches of bf16 rows that two CTAs of 512 threads hold and 256 do not keep those:
-// 1024 x 32000 in 53.9 us, of 256 threads 58.2; 640 x 50257 in 69 and 73.
+// 640 x 50257 in 57.9 us, of 256 threads 58.7 (1024 x 32000 in 47.0 and 46.3).
 constexpr i64 PROBS_MAX = 8 * (64 * 512 - 32);      // (a run of bf16 may begin with half a pair)
 struct ProbsShape {
   int ctas, regs, threads;
@@ -583,7 +593,7 @@ struct ProbsShape {
 template <typename T>
 static ProbsShape probs_shape(const T* x, i64 ld, i64 rows, i64 cols) {
   constexpr bool PAIRS = sizeof(T) == 2;
-  // the column in front of a run: only where a row may begin with half a word (1024 x 32768 bf16: 53.5 us without it, 85 with it)
+  // the column in front of a run: only where a row may begin with half a word (1024 x 32768 bf16: 47.6 us without it, 72 with it)
   const int half = PAIRS && (((reinterpret_cast<uintptr_t>(x) >> 1) | (uintptr_t)ld) & 1);
   const bool small = cols <= 2 * 32 * 256 - 32 * half || (cols <= 8 * (32 * 256 - 32 * half) && (!PAIRS || rows <= WKB_SM_COUNT));
   ProbsShape s{1, 4, small ? 256 : 512};
