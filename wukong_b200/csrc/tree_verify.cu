@@ -584,8 +584,8 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsig
 // A row's columns over the CTAs of a cluster and the registers of their threads: clusters grow until two CTAs per SM are
 // at work (small batches) and a thread holds at most 32 columns (large vocabularies), or at 8.  CTAs of 256 threads,
 // which leave an SM more of them to overlap, while eight hold a row: 1024 x 7582 f32 in 14.8 us, of 512 threads 17.9;
-// 128 x 32000 in 9.1 and 10.9.  Only full batches of bf16 rows that two CTAs of 512 threads hold and 256 do not keep those:
-// 640 x 50257 in 57.9 us, of 256 threads 58.7 (1024 x 32000 in 47.0 and 46.3).
+// 128 x 32000 in 9.1 and 10.9; of bf16 1024 x 7582 in 13.1 and 18.1, 1024 x 32000 in 46.3 and 47.0, 640 x 50257 in 58.7
+// and 57.9.
 constexpr i64 PROBS_MAX = 8 * (64 * 512 - 32);      // (a run of bf16 may begin with half a pair)
 struct ProbsShape {
   int ctas, regs, threads;
@@ -595,7 +595,7 @@ static ProbsShape probs_shape(const T* x, i64 ld, i64 rows, i64 cols) {
   constexpr bool PAIRS = sizeof(T) == 2;
   // the column in front of a run: only where a row may begin with half a word (1024 x 32768 bf16: 47.6 us without it, 72 with it)
   const int half = PAIRS && (((reinterpret_cast<uintptr_t>(x) >> 1) | (uintptr_t)ld) & 1);
-  const bool small = cols <= 2 * 32 * 256 - 32 * half || (cols <= 8 * (32 * 256 - 32 * half) && (!PAIRS || rows <= WKB_SM_COUNT));
+  const bool small = cols <= 8 * (32 * 256 - 32 * half);
   ProbsShape s{1, 4, small ? 256 : 512};
   auto need = [&] { return probs_run(cols, s.ctas) + half; };
   while (s.ctas < 8 && (need() > 32 * s.threads || (rows * s.ctas < 2 * WKB_SM_COUNT && cols > (i64)s.ctas * 4 * s.threads))) s.ctas *= 2;
