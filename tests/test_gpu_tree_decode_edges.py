@@ -184,3 +184,32 @@ def test_token_probs_bf16_rows_that_begin_and_end_in_a_word(dev, rows, cols):
                     assert bool(((got.double() - want).abs() <= want * 2.0 ** -15 + 1e-38).all())
                 else:
                     assert torch.equal(got.argmax(1), (x == x.amax(1, keepdim=True)).double().argmax(1)) and bool((got.sum(1) == 1).all())
+
+
+# ---- accuracy in the mean -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("trees,qh,kvh,hd", [([(200, 20)], 4, 2, 128), ([(257, 5)], 12, 12, 64), ([(700, 33), (1500, 61)], 8, 2, 128), ([(9001, 3)], 4, 4, 128), ([(5000, 64)], 8, 8, 64),
+                                             ([(30011, 16)], 8, 1, 128), ([(20000, 9)], 8, 2, 64)])
+@pytest.mark.parametrize("tq", ["f32", "bf16"])
+def test_f32_results_in_the_mean(dev, trees, qh, kvh, hd, tq):
+    """Norm of the error over the norm of the result, unit-normal inputs.  A query and a weight as two bf16 parts are off by at
+    most 2^-16 of themselves; with scale 1 / sqrt(hd) a score is then off by 2^-16 in the mean and a weight by that and its own
+    2^-16, independently from key to key, so a sum over the keys is off by 2^-15 of itself.  The tensor pipe's sums lose one
+    part of 2^-24 a step at most, a step being 16 keys: keys * 2^-28 in all.  The bar tells a lost part at every length: weights
+    of one bf16 part alone exceed it, by the same emulation, which the second assertion holds."""
+    import torch
+    c = Case(dev, trees, qh, kvh, hd, seed=hd, q_dtype={"f32": torch.float32, "bf16": torch.bfloat16}[tq])
+    out = torch.zeros((c.rows, qh * hd), device="cuda")
+    c.run(dev, out)
+    want, _, _ = c.expected()
+    bar = 2.0 ** -15 + max(n + k for n, k in trees) * 2.0 ** -28
+    assert float((out.double() - want).norm() / want.norm()) <= bar
+    ctx, nodes = trees[0]
+    pos = np.arange(ctx)
+    pg, off = (torch.from_numpy(a).cuda() for a in (c.table[0, pos // 16], pos % 16))
+    k, v = (x[0][pg, 0, off].double() for x in (c.kv.k, c.kv.v))
+    p = torch.softmax(c.q[:nodes, :hd].double() @ k.T * c.scale, 1)
+    p = p / p.amax(1, keepdim=True)
+    short = (p.bfloat16().double() @ v) / p.sum(1, keepdim=True)
+    full = (p @ v) / p.sum(1, keepdim=True)
+    assert float((short - full).norm() / full.norm()) > bar

@@ -12,8 +12,10 @@
 // Two teams take alternate key blocks with tensor-memory columns of their own, so one team's exponentials run while the
 // other's products do; a single team leaves that to the SM's other CTA.  The running maximum m of a row moves only when a
 // block exceeds it by 2^8; the accumulator is rescaled then and not at every block.  f32 queries are two bf16 parts (hi +
-// lo, two products); for f32 results P is two parts as well (5e-6 of the result over 8192 keys, of which the products'
-// accumulation is the larger share).
+// lo, two products); for f32 results P is two parts as well: 16 bits of each, 3e-6 of the result in the mean for unit-normal
+// queries (2e-6 for bf16 ones), 5e-6 for queries half as large again.  bf16 results keep P in one part: 2.1e-3 in the mean,
+// of which the result's own rounding is 1.7e-3; the second part would leave that alone, for 10 to 21 % of the time (tree of 64
+// nodes over 32749 tokens 57.7 -> 69.8 us, Llama-shape batch 137 -> 161 us called).
 //
 // Bound.  K and V are read once from HBM (569.9 MB for 571.6 MB of work in the Llama-shape batch of 64 trees) and stream at
 // the copy rate inside a unit: 1.41 us a block of head_dim 128 on all SMs together, 0.72 us of head_dim 64.  The batch takes 118 us

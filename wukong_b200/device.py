@@ -294,7 +294,8 @@ def paged_attn_tree_scratch(max_nodes, q_heads, kv_heads, head_dim, device="cuda
 
 def paged_attn_tree(q, q_row_stride, kv, layer, block_table, tree_slot, tree_ctx, tree_row0, tree_mask, out, q_heads, mbps, max_nodes, scale, scratch):
     """Attention of the nodes of draft trees over the paged bf16 cache (wkb_paged_attn_tree): row r = node i of tree t sees
-    the tree_ctx[t] committed tokens and the nodes that its mask names.  q f32 or bf16, out f32 or bf16 [rows, q_heads * head_dim]."""
+    the tree_ctx[t] committed tokens and the nodes that its mask names.  q f32 or bf16, out f32 or bf16 [rows, q_heads * head_dim].
+    f32 results are good to about 3e-6 in the mean, not to f32's last bits: queries and weights have 16 significant bits."""
     return _calls().paged_attn_tree(q, q_row_stride, kv.k, kv.v, kv.layers, kv.num_pages, kv.kv_heads, kv.page_tokens, kv.head_dim, layer, block_table,
                                     tree_slot, tree_ctx, tree_row0, tree_mask, out, q_heads, mbps, max_nodes, scale, scratch)
 
