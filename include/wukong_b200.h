@@ -359,7 +359,8 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, int64_t q_row_stride, const 
 int wkb_token_probs(const void* logits, int in_dtype, int64_t ld, const float* temperature_or_null, float* out, int64_t ld_out,
                     int64_t rows, int64_t cols, void* stream);
 /* Verification of drafted tokens from given random numbers.  Row r of `probs` holds the target's probabilities after node r,
- * row r of `draft` (null: none) the distribution that the children of node r were drawn from, f32 [rows, cols] with row
+ * row r of `draft` (null: none) the distribution that the children of node r were drawn from -- each by itself, with
+ * replacement: a token may come twice, and siblings drawn to be distinct would bias the result --, f32 [rows, cols] with row
  * pitches ld_p / ld_q; token[r] is the node's token, parent[r] its parent's index within the tree (below its own; the root's
  * is not read).  The walk starts at the root.  With p, q the current node's rows, r_0 = p and Z_0 = 1, its children x_1, x_2,
  * ... are tried in row order:

@@ -308,7 +308,8 @@ def token_probs(logits, temperature=None, out=None):
 
 def tree_verify(probs, draft, token, parent, tree_row0, u_node, u_final, max_nodes, max_path, out=None):
     """Accept / reject the drafted tokens of each tree and draw the token that follows (wkb_tree_verify).  probs, draft (or
-    None): f32 [rows, vocabulary].  Returns (path int32 [n, max_path], n_path int32 [n], tokens int32 [n, max_path])."""
+    None): f32 [rows, vocabulary]; with draft, the emitted tokens follow the target's distribution when each child was drawn from
+    its parent's row by itself, with replacement.  Returns (path int32 [n, max_path], n_path int32 [n], tokens int32 [n, max_path])."""
     path, n_path, tokens = out or (None, None, None)
     return _calls().tree_verify(probs, draft, token, parent, tree_row0, u_node, u_final, max_nodes, max_path, path, n_path, tokens)
 
