@@ -392,6 +392,8 @@ void* wkb_blockmgr_new(int64_t num_blocks, int64_t block_size, int64_t num_slots
 void wkb_blockmgr_delete(void* h);
 int64_t wkb_blockmgr_append(void* h, int64_t slot, uint32_t* phys, int64_t* off);
 int64_t wkb_blockmgr_reserve(void* h, int64_t slot, int64_t tokens);
+/* Pages for `tokens` more positions; unlike reserve, the context stays where it is (0, or -1 with the state unchanged). */
+int64_t wkb_blockmgr_ensure_capacity(void* h, int64_t slot, int64_t tokens);
 void wkb_blockmgr_release(void* h, int64_t slot);
 int64_t wkb_blockmgr_can_grow(void* h, int64_t slot, int64_t tokens);
 int64_t wkb_blockmgr_free_blocks(void* h);

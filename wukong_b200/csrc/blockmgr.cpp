@@ -69,7 +69,7 @@ struct BlockManager {
     ctx[(size_t)slot] = need;
     return start;
   }
-  // Pages for `tokens` more positions without advancing the context (admission-time reservation).
+  // Pages for `tokens` more positions without advancing the context (admission-time reservation, nodes of a draft tree).
   bool ensure_capacity(int64_t slot, int64_t tokens) {
     if (!can_grow(slot, tokens)) return false;
     int64_t need = ctx[(size_t)slot] + tokens;
@@ -158,6 +158,7 @@ void* wkb_blockmgr_new(int64_t num_blocks, int64_t block_size, int64_t num_slots
 void wkb_blockmgr_delete(void* h) { delete (BlockManager*)h; }
 int64_t wkb_blockmgr_append(void* h, int64_t slot, uint32_t* phys, int64_t* off) { return ((BlockManager*)h)->append(slot, phys, off); }
 int64_t wkb_blockmgr_reserve(void* h, int64_t slot, int64_t tokens) { return ((BlockManager*)h)->reserve(slot, tokens); }
+int64_t wkb_blockmgr_ensure_capacity(void* h, int64_t slot, int64_t tokens) { return ((BlockManager*)h)->ensure_capacity(slot, tokens) ? 0 : -1; }
 void wkb_blockmgr_release(void* h, int64_t slot) { ((BlockManager*)h)->release(slot); }
 int64_t wkb_blockmgr_can_grow(void* h, int64_t slot, int64_t tokens) { return ((BlockManager*)h)->can_grow(slot, tokens) ? 1 : 0; }
 int64_t wkb_blockmgr_free_blocks(void* h) { return (int64_t)((BlockManager*)h)->free_list.size(); }

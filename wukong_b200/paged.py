@@ -40,6 +40,11 @@ class BlockManager:
             raise OutOfBlocks()
         return start
 
+    def ensure_capacity(self, slot, tokens):
+        """Pages for `tokens` more positions; the context stays where it is."""
+        if lib().wkb_blockmgr_ensure_capacity(self._h, slot, tokens) != 0:
+            raise OutOfBlocks()
+
     def free(self, slot):
         lib().wkb_blockmgr_release(self._h, slot)
 
