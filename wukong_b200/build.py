@@ -1,8 +1,10 @@
 """Build step: compile every CUDA source under csrc/ for sm_100a into one C-ABI shared library,
 in-tree (wukong_b200/libwukong_b200.so), and csrc/host/torch_calls.cpp -- calls on torch tensors that skip the Python level
--- into an extension module beside it (wukong_b200/_torch_calls.so).  nvcc cross-compiles without a GPU."""
+-- into an extension module beside it (wukong_b200/_torch_calls.so).  nvcc cross-compiles without a GPU.  The library needs
+nothing else; where torch or g++ is missing the module is left out, and the calls that go through it say so."""
 import glob
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -34,23 +36,35 @@ def needs_build():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build_calls(force=False, verbose=False):
-    """The extension module of csrc/host: linked against torch and, beside it, the C-ABI library."""
-    header = os.path.join(HERE, "..", "include", "wukong_b200.h")
-    if not force and os.path.exists(CALLS_OUT) and os.path.getmtime(CALLS_OUT) > max(os.path.getmtime(p) for p in (CALLS, header, os.path.abspath(__file__))):
-        return CALLS_OUT
-    import torch
-    root = os.path.dirname(os.path.abspath(torch.__file__))
-    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I" + sysconfig.get_paths()["include"],
-           "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(cuda, "include"), CALLS,
-           "-o", CALLS_OUT, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + HERE, "-l:libwukong_b200.so",
-           "-Wl,-rpath,$ORIGIN:" + os.path.join(root, "lib")]
+def run_host_compiler(cmd, verbose):
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0 or verbose:
         sys.stderr.write("== torch_calls.cpp\n%s\n" % r.stdout)
     if r.returncode != 0:
         raise RuntimeError("g++ failed")
+
+
+def build_calls(force=False, verbose=False):
+    """The extension module of csrc/host: linked against torch and, beside it, the C-ABI library."""
+    try:
+        import torch
+    except ImportError:
+        sys.stderr.write("_torch_calls is left out: torch is not installed\n")
+        return None
+    header = os.path.join(HERE, "..", "include", "wukong_b200.h")
+    if not force and os.path.exists(CALLS_OUT) and \
+            os.path.getmtime(CALLS_OUT) > max(os.path.getmtime(p) for p in (CALLS, header, os.path.abspath(__file__))):
+        return CALLS_OUT
+    if not shutil.which("g++"):
+        sys.stderr.write("_torch_calls is left out: there is no g++\n")
+        return None
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(cuda, "include"), CALLS, "-o", CALLS_OUT, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + HERE,
+           "-l:libwukong_b200.so", "-Wl,-rpath,$ORIGIN:" + os.path.join(root, "lib")]
+    run_host_compiler(cmd, verbose)
     return CALLS_OUT
 
 
