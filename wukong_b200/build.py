@@ -15,6 +15,7 @@ OUT = os.path.join(HERE, "libwukong_b200.so")
 OBJ = os.path.join(HERE, "build")
 CALLS = os.path.join(CSRC, "host", "torch_calls.cpp")
 CALLS_OUT = os.path.join(HERE, "_torch_calls.so")
+CALLS_FOR = os.path.join(OBJ, "torch_calls.torch")      # the torch version that it was built against
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -51,8 +52,9 @@ def build_calls(force=False, verbose=False):
     except ImportError:
         sys.stderr.write("_torch_calls is left out: torch is not installed\n")
         return None
-    header = os.path.join(HERE, "..", "include", "wukong_b200.h")
-    if not force and os.path.exists(CALLS_OUT) and \
+    header, version = os.path.join(HERE, "..", "include", "wukong_b200.h"), str(torch.__version__)
+    built_for = open(CALLS_FOR).read() if os.path.exists(CALLS_FOR) else None
+    if not force and built_for == version and os.path.exists(CALLS_OUT) and \
             os.path.getmtime(CALLS_OUT) > max(os.path.getmtime(p) for p in (CALLS, header, os.path.abspath(__file__))):
         return CALLS_OUT
     if not shutil.which("g++"):
@@ -60,11 +62,14 @@ def build_calls(force=False, verbose=False):
         return None
     root = os.path.dirname(os.path.abspath(torch.__file__))
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), '-DWKB_TORCH_VERSION="%s"' % version,
            "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I" + os.path.join(cuda, "include"), CALLS, "-o", CALLS_OUT, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + HERE,
            "-l:libwukong_b200.so", "-Wl,-rpath,$ORIGIN:" + os.path.join(root, "lib")]
     run_host_compiler(cmd, verbose)
+    os.makedirs(OBJ, exist_ok=True)
+    with open(CALLS_FOR, "w") as fh:
+        fh.write(version)
     return CALLS_OUT
 
 

@@ -271,4 +271,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_calls(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__torch_calls(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", WKB_TORCH_VERSION) != 0) Py_CLEAR(m);
+  return m;
+}

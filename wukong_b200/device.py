@@ -262,6 +262,9 @@ def _calls():
             from . import _torch_calls
         except ImportError as e:
             raise WukongB200Error("the _torch_calls extension is missing or does not load (%s): run `python -m wukong_b200.build`" % e)
+        if _torch_calls.torch_version != str(torch.__version__):
+            raise WukongB200Error("the _torch_calls extension was built for torch %s, this is %s: run `python -m wukong_b200.build`" %
+                                  (_torch_calls.torch_version, torch.__version__))
         _torch_calls.set_error(WukongB200Error)
         _calls_module = _torch_calls
     return _calls_module
