@@ -213,3 +213,41 @@ def test_f32_results_in_the_mean(dev, trees, qh, kvh, hd, tq):
     short = (p.bfloat16().double() @ v) / p.sum(1, keepdim=True)
     full = (p @ v) / p.sum(1, keepdim=True)
     assert float((short - full).norm() / full.norm()) > bar
+
+
+# ---- Python level ---------------------------------------------------------------------------------------------------
+
+def test_a_full_launch_queue_does_not_stop_other_threads(dev):
+    """A thread that launches faster than the GPU works waits in the driver, and the other threads go on meanwhile, as with
+    the library's other calls: for most of a second the queue here is blocked by one kernel, and the longest pause of
+    the counting thread stays below a third of that."""
+    import threading
+    import time
+    import torch
+    x, out = torch.zeros((1, 8), device="cuda"), torch.empty((1, 8), device="cuda")
+    dev.token_probs(x, None, out)
+    torch.cuda.synchronize()
+    blocked = []
+
+    def launch():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(1 << 30)
+            blocked.append(time.perf_counter())
+            for _ in range(6000):
+                dev.token_probs(x, None, out)
+            stream.synchronize()
+
+    t0 = time.perf_counter()
+    worker = threading.Thread(target=launch)
+    worker.start()
+    last, pause = None, 0.0
+    while worker.is_alive():
+        time.sleep(0.0005)
+        now = time.perf_counter()
+        if blocked:
+            pause = max(pause, now - (last or blocked[0]))
+            last = now
+    whole = time.perf_counter() - t0
+    assert whole > 0.45, "the GPU was not blocked"
+    assert pause < 0.15, (pause, whole)

@@ -121,6 +121,15 @@ void check(int rc, const char* what) {
   PyErr_Format(g_error ? g_error : PyExc_RuntimeError, "%s failed with status %d", what, rc);
   throw PyRaised();
 }
+// A C entry without the interpreter lock: a launch waits while the GPU's queue is full, and other threads (a host function of
+// the stream among them, which the queue may be waiting for) have to go on.
+template <typename... P, typename... A>
+int unlocked(int (*entry)(P...), A... args) {
+  PyThreadState* state = PyEval_SaveThread();
+  const int rc = entry(static_cast<P>(args)...);
+  PyEval_RestoreThread(state);
+  return rc;
+}
 template <typename F>
 PyObject* guarded(F&& f) {
   try {
@@ -157,7 +166,7 @@ PyObject* paged_attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (mask.dim() != 2 || mask.size(0) < rows) throw Refused("tree_mask must have a row for each row of out");
     const int64_t ldo = pitch(out, width, "out"), mbps = table_width(c, 10, c.integer(17), trees);
     const int64_t at_layer = layer * kv.layer_stride * 2;
-    check(wkb_paged_attn_tree(q.data_ptr(), q_code, stride, kv.k + at_layer, kv.v + at_layer, kv.pages, (const uint32_t*)c.tensor(10, "block_table").data_ptr(),
+    check(unlocked(wkb_paged_attn_tree, q.data_ptr(), q_code, stride, kv.k + at_layer, kv.v + at_layer, kv.pages, (const uint32_t*)c.tensor(10, "block_table").data_ptr(),
                               (const int*)c.values(11, trees, at::kInt, "tree_slot"), (const int*)c.values(12, trees, at::kInt, "tree_ctx"),
                               (const int*)c.values(13, trees + 1, at::kInt, "tree_row0"), (const uint32_t*)c.values(14, mask.numel(), at::kInt, "tree_mask"), mask.size(1),
                               out.data_ptr(), out_code, ldo, rows, trees, c.integer(18), q_heads, kv.kv_heads, kv.head_dim, kv.page_tokens, mbps, (float)c.real(19),
@@ -181,7 +190,7 @@ PyObject* token_probs(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor& out = c.none(2) ? made : c.tensor(2, "out");
     c.on_device(out, "out");
     if (out.scalar_type() != at::kFloat || out.sizes() != x.sizes()) throw Refused("out must be f32 of the logits' shape");
-    check(wkb_token_probs(x.data_ptr(), code, ld, c.none(1) ? nullptr : (const float*)c.values(1, rows, at::kFloat, "temperature"), (float*)out.data_ptr(),
+    check(unlocked(wkb_token_probs, x.data_ptr(), code, ld, c.none(1) ? nullptr : (const float*)c.values(1, rows, at::kFloat, "temperature"), (float*)out.data_ptr(),
                           pitch(out, cols, "out"), rows, cols, c.stream()),
           "wkb_token_probs");
     return c.none(2) ? THPVariable_Wrap(std::move(made)) : same(args[2]);
@@ -221,7 +230,7 @@ PyObject* tree_verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
       pn = (int*)c.values(10, trees, at::kInt, "n_path");
       pt = (int*)c.values(11, trees * max_path, at::kInt, "tokens");
     }
-    check(wkb_tree_verify((const float*)p.data_ptr(), pitch(p, cols, "probs"), draft, ldq, (const int*)c.values(2, rows, at::kInt, "token"),
+    check(unlocked(wkb_tree_verify, (const float*)p.data_ptr(), pitch(p, cols, "probs"), draft, ldq, (const int*)c.values(2, rows, at::kInt, "token"),
                           (const int*)c.values(3, rows, at::kInt, "parent"), (const int*)c.values(4, trees + 1, at::kInt, "tree_row0"), rows, trees, max_nodes, cols,
                           (const float*)c.values(5, rows, at::kFloat, "u_node"), (const float*)c.values(6, trees, at::kFloat, "u_final"), pp, pt, pn, max_path,
                           c.stream()),
@@ -246,7 +255,7 @@ PyObject* paged_kv_commit(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Cache kv = cache_of(c, 0);
     if (path.dim() != 2 || path.size(0) != trees) throw Refused("path must be int32 [n, max_path]");
     const int64_t mbps = table_width(c, 7, c.integer(12), trees);
-    check(wkb_paged_kv_commit(kv.k, kv.v, kv.layers, kv.layer_stride, kv.pages, (const uint32_t*)c.tensor(7, "block_table").data_ptr(),
+    check(unlocked(wkb_paged_kv_commit, kv.k, kv.v, kv.layers, kv.layer_stride, kv.pages, (const uint32_t*)c.tensor(7, "block_table").data_ptr(),
                               (const int*)c.values(8, trees, at::kInt, "tree_slot"), (const int*)c.values(9, trees, at::kInt, "tree_ctx"),
                               (const int*)c.values(10, path.numel(), at::kInt, "path"), (const int*)c.values(11, trees, at::kInt, "n_path"), path.size(1), trees,
                               kv.kv_heads, kv.head_dim, kv.page_tokens, mbps, c.none(13) ? nullptr : (int*)c.values(13, trees, at::kInt, "new_ctx"), c.stream()),
