@@ -251,3 +251,12 @@ def test_a_full_launch_queue_does_not_stop_other_threads(dev):
     whole = time.perf_counter() - t0
     assert whole > 0.45, "the GPU was not blocked"
     assert pause < 0.15, (pause, whole)
+
+
+def test_errors_of_torch_keep_their_types(dev):
+    """Results that do not fit the device: torch.OutOfMemoryError as from torch's own calls (logits of 2^20 equal rows, whose
+    probabilities would take 2 TB)."""
+    import torch
+    x = torch.zeros(1 << 19, device="cuda").expand(1 << 20, 1 << 19)
+    with pytest.raises(torch.OutOfMemoryError):
+        dev.token_probs(x)

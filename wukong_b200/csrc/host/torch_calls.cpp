@@ -2,7 +2,8 @@
 // call into the C ABI, without a Python-level step per tensor.  These calls run once a layer or once a step and often
 // eagerly; through ctypes and Python checks a call took 9 to 17 us of the host, more than most of them take on the GPU.
 //
-// Wrong types, extents, strides or devices raise ValueError; a non-zero status of the C entry raises the package's error.
+// Wrong types, extents, strides or devices raise ValueError; a non-zero status of the C entry raises the package's error;
+// errors of torch (memory for a result) keep their type.
 // No C++ exception leaves a function.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -11,6 +12,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <stdexcept>
@@ -137,8 +139,8 @@ PyObject* guarded(F&& f) {
   } catch (const PyRaised&) {
   } catch (const Refused& e) {
     PyErr_SetString(PyExc_ValueError, e.what());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }
