@@ -336,7 +336,7 @@ int wkb_paged_kv_append(const float* ksrc, const float* vsrc, int64_t src_row_st
  * of tree_mask[r * mask_words + j / 32] is set (the node itself and its ancestors; other patterns are allowed).  What a row
  * does not see never reaches its output, NaN included; a row that sees nothing gives zeros.  Of V elements that are not finite a
  * row's result is the sum over those that it sees, however small their weights; a K that is not finite may make the rows that see it NaN.  q and out: dtype 0 f32, 1 bf16,
- * row strides in elements, multiples of 8, at most 2^31; all bases 16-byte aligned; out overlaps no input. 
+ * row strides in elements, multiples of 8, at most 2^31; all bases 16-byte aligned; out overlaps no input; |scale| <= 1e38.
  * f32 queries enter the products as two bf16 parts (16 significant bits); sums, maxima and joins are f32.  bf16 outputs carry
  * softmax weights of one bf16 part (2e-3 of the result in the mean, of which its own rounding is 1.7e-3), f32 outputs of two: 3e-6 of the result in the mean
  * for unit-normal q and k at scale 1 / sqrt(head_dim) (2e-6 for bf16 queries; f32 arithmetic throughout would leave 1e-6), growing

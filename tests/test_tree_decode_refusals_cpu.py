@@ -59,3 +59,10 @@ def test_commit_into_an_array_that_it_reads(L, new_ctx):
     assert commit(L, new_ctx=new_ctx, **at) == BAD
     for apart in (P - 32, P + 32, P + 96, P + 256, P + 480, P + 544):
         assert commit(L, new_ctx=apart, **at) == MISALIGNED
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 3e38, -3e38])
+def test_attention_scale_that_is_not_a_number_of_use(L, scale):
+    """NaN would have been taken for the smallest scale there is, and infinite products with zeros are NaN everywhere."""
+    assert attn(L, scale=scale) == BAD
+    assert attn(L, scale=-1e30) == MISALIGNED and attn(L, scale=0.0) == MISALIGNED

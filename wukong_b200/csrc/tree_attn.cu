@@ -160,6 +160,7 @@ int wkb_paged_attn_tree(const void* q, int q_dtype, i64 q_row_stride, const void
     return (int)cudaErrorInvalidValue;
   if (num_pages > 0x7fffff00 / (kv_heads * page_tokens)) return (int)cudaErrorInvalidValue;
   if ((q_dtype != 0 && q_dtype != 1) || (out_dtype != 0 && out_dtype != 1)) return (int)cudaErrorInvalidValue;
+  if (!(fabsf(scale) <= 1e38f)) return (int)cudaErrorInvalidValue;      // (NaN; in base 2 it has to be finite)
   if (q_row_stride < 0 || out_row_stride < 0 || (rows > 1 && out_row_stride < q_heads * head_dim)) return (int)cudaErrorInvalidValue;      // result rows do not overlap
   if (q_row_stride % 8 != 0 || out_row_stride % 8 != 0) return (int)cudaErrorMisalignedAddress;
   if (((((uintptr_t)q) | ((uintptr_t)kcache) | ((uintptr_t)vcache) | ((uintptr_t)out) | ((uintptr_t)scratch)) & 15) != 0) return (int)cudaErrorMisalignedAddress;
