@@ -17,9 +17,9 @@
 // of which the result's own rounding is 1.7e-3; the second part would leave that alone, for 10 to 21 % of the time (tree of 64
 // nodes over 32749 tokens 57.7 -> 69.8 us, Llama-shape batch 137 -> 161 us called).
 //
-// Bound.  K and V are read once from HBM (569.9 MB for 571.6 MB of work in the Llama-shape batch of 64 trees) and stream at
-// the copy rate inside a unit: 1.41 us a block of head_dim 128 on all SMs together, 0.72 us of head_dim 64.  The batch takes 118 us
-// against 87 us of its bytes; the rest is the beginnings and ends of units (8 k cycles each, partly under the rings'
+// Bound.  K and V are read once from HBM (569.9 MB for 571.6 MB of work in the Llama-shape batch of 64 trees; once for each
+// 128 query rows where a head has more and its K and V do not fit L2) and stream at the copy rate inside a unit: 1.41 us a block of head_dim 128 on all SMs together, 0.72 us of head_dim 64.  The batch takes 111
+// to 117 us from card to card (137 in a loop of seconds, where the board's power cap lowers the clock to 1.53 GHz) against 87 us of its bytes; the rest is the beginnings and ends of units (8 k cycles each, partly under the rings'
 // prefetch), the first trip to memory and the join (4 us).  With 128 rows a unit it is the chain S -> softmax -> P V of
 // the teams, 2200 cycles a block against 1330 of the tensor pipe and the shared-memory port.
 //
@@ -233,7 +233,7 @@ __device__ __forceinline__ TreeWork tree_work(const Geo& g, const int* slot, con
   return w;
 }
 // A unit counts as its blocks and UNIT_COST more: what beginning and ending one takes, in blocks (0: 161 us, 2: 118, 3: 116,
-// 4: 114, 7: 118, 10: 123 for the 64 trees of a Llama-shape batch).
+// 4: 114, 7: 118, 10: 123 on one card, for the 64 trees of a Llama-shape batch).
 constexpr int UNIT_COST = 4;
 __device__ __forceinline__ int unit_items(const Geo& g, const TreeWork& w) { return g.split ? w.blocks + UNIT_COST : 1; }
 __device__ __forceinline__ int tree_items(const Geo& g, const TreeWork& w) { return unit_items(g, w) * w.rowblks * g.kv_heads; }

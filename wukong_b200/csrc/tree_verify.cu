@@ -243,7 +243,7 @@ struct alignas(16) Ask {
 // rejection (before the next sibling is tried) and the final draw need a pass over the vocabulary, a contiguous run of
 // columns per warp of the cluster; the row is read from HBM once and the run that holds the draw a second time, from L2.
 // The leader alone decides, so every CTA takes the same steps.  Sums are in a fixed order.  Bound: the latency of the four
-// dependent trips to memory for a few trees (8.2 us for one chain over 50257 columns, 5 of them a warp's instructions and
+// dependent trips to memory for a few trees (8.1 to 9 us for one chain over 50257 columns, 5 of them a warp's instructions and
 // barriers), the longest walk's passes for many (27 us for 64 trees over 32000).
 constexpr int HOLD = 16;
 template <bool DRAFT>
@@ -616,7 +616,8 @@ static int launch_probs(const T* x, i64 ld, const float* temperature, float* out
   const ProbsShape s = probs_shape(x, ld, rows, cols);
   return s.threads == 256 ? launch_probs<T, 256>(s, x, ld, temperature, out, ld_out, rows, cols, st) : launch_probs<T, 512>(s, x, ld, temperature, out, ld_out, rows, cols, st);
 }
-// CTAs of a tree's cluster: as many as keep two per SM at work, each with 2048 columns at least.
+// CTAs of a tree's cluster: doubled while the trees' CTAs are fewer than two per SM and each has more than 2048 columns, up to 8.
+// So the last doubling may pass the 296 CTAs that run at a time (64 trees over 32000 columns: 512 of them, in two waves, 27.5 us).
 static int verify_ctas(i64 n_trees, i64 cols) {
   int c = 1;
   while (c < 8 && n_trees * c < 2 * WKB_SM_COUNT && cols > (i64)c * 2048) c *= 2;
