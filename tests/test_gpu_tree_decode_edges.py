@@ -91,6 +91,27 @@ def test_infinities_in_the_context_whatever_the_tree_and_the_weights(dev, hd, gr
     assert dev.gemm_status() == 0
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd,group,nodes", [(64, 1, 12), (128, 4, 12), (128, 4, 50)])
+def test_rows_with_nan_queries_beside_infinities_of_v(dev, hd, group, nodes, dtype):
+    """A row whose query is NaN is NaN in every column, and its neighbours are what they are without it."""
+    import torch
+    tq = {"f32": torch.float32, "bf16": torch.bfloat16}[dtype]
+    c = Case(dev, [(777, nodes), (3000, nodes)], group, 1, hd, seed=4, q_dtype=tq)
+    for dim, pos in [(3, 5), (4, 777 + 1), (60, 776)]:
+        plant(c, c.kv.v, 0, pos, 0, dim, math.inf)
+    clean = torch.zeros((c.rows, group * hd), dtype=tq, device="cuda")
+    c.run(dev, clean)
+    c.check(clean)
+    c.q[5] = math.nan
+    c.q[nodes + 2, 7] = math.nan
+    out = torch.zeros_like(clean)
+    c.run(dev, out)
+    assert bool(out[5].isnan().all()) and bool(out[nodes + 2, :hd].isnan().all())
+    clean[5] = clean[nodes + 2, :hd] = out[5] = out[nodes + 2, :hd] = 0
+    assert torch.equal(clean, out) and dev.gemm_status() == 0
+
+
 # ---- commit ---------------------------------------------------------------------------------------------------------
 
 def test_commit_of_a_broken_path_counts_what_was_moved(dev):
